@@ -292,6 +292,76 @@ PM_API size_t pm_lmhead_sample_workspace_bytes(const pm_lmhead *h, const pm_rows
 PM_API int pm_lmhead_sample(const pm_lmhead *h, const pm_rows *rows, const pm_noise *noise,
                             const pm_sample_out *out, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Top log-probabilities (no counterpart in the reference, whose sampler
+ * returns the whole log-softmax row, pagedmoe/verify_decode.py:835): the k
+ * largest logits of every row in descending order (ties: the lowest id) and
+ * their log-probabilities under softmax(logits * inv_temperature) over the
+ * allowed tokens -- what an API answers with beside a token, a beam's list of
+ * continuations, a teacher's targets for pm_distill.  Tokens that are
+ * disallowed or -inf are no candidates: places left over hold id -1 and
+ * log-probability -inf.  A row with a NaN or +inf among its allowed logits
+ * gives ids -1 and NaN.  1 <= k <= 256. */
+typedef struct pm_top_rows {
+    const void *logits;          /* [rows, row_stride] of dtype */
+    int32_t dtype;               /* PM_DTYPE_* */
+    int64_t rows;
+    int64_t vocab;
+    int64_t row_stride;          /* elements between rows (>= vocab) */
+    const uint32_t *mask;        /* [rows, mask_stride] allowed-token bits, or NULL */
+    int64_t mask_stride;         /* words, >= ceil(vocab / 32); 0: one mask for every row */
+    int32_t k;
+    double inv_temperature;      /* > 0 */
+} pm_top_rows;
+
+/* ids, logprobs: [rows, k]; lse: [rows] log-sum-exp of logits *
+ * inv_temperature, or NULL. */
+PM_API int pm_top_logprobs(const pm_top_rows *t, int32_t *ids, float *logprobs, float *lse, void *stream);
+
+/* One step of beam search (no counterpart in the reference, which decodes one
+ * sequence a request): row w of item i holds the logits after beam w, with
+ * score scores[i, w].  The n best continuations of every item over its beams
+ * and the vocabulary, by
+ *     total = score + (logit - log-sum-exp of the beam's allowed logits)
+ * in 64 bits, divided by length ^ length_penalty (length: lengths[i, w] + 1),
+ * best first; ties go to the lower beam, then the larger logit, then the
+ * lower token.  A finished beam (done != 0) offers one candidate, token eos
+ * at its own score and length, and its logits are not read.  A beam of score
+ * -inf, and one whose allowed logits hold a NaN, a +inf or nothing finite,
+ * offers none.  Places left over hold score -inf, parent -1, token -1,
+ * length 0.  keep_slots (n == beams): the best child of every beam that lives
+ * on takes that beam's place, the others fill the free places in ascending
+ * order, so that moving states in place touches only the beams that ended.
+ * 1 <= beams <= 64, 1 <= n <= 256, |length_penalty| <= 16. */
+typedef struct pm_beam {
+    const void *logits;          /* [items * beams, row_stride] of dtype */
+    int32_t dtype;               /* PM_DTYPE_* */
+    int64_t items;
+    int32_t beams;
+    int64_t vocab;
+    int64_t row_stride;
+    const uint32_t *mask;        /* [items * beams, mask_stride], or NULL */
+    int64_t mask_stride;         /* words; 0: one mask for every row */
+    const float *scores;         /* [items, beams] */
+    const uint8_t *done;         /* [items, beams], or NULL */
+    const int32_t *lengths;      /* [items, beams] tokens so far, or NULL (length_penalty must be 0) */
+    int32_t eos;                 /* the token that ends a beam, -1: none (done must be NULL) */
+    double length_penalty;
+    int32_t n;
+    int32_t keep_slots;
+} pm_beam;
+
+typedef struct pm_beam_out {
+    float *scores;               /* [items, n] totals, not divided by the length */
+    int32_t *parents;            /* [items, n] beam of the item, -1: none */
+    int32_t *tokens;             /* [items, n], -1: none */
+    int32_t *lengths;            /* [items, n], or NULL */
+    uint8_t *done;               /* [items, n] (token == eos, or the parent was done), or NULL */
+} pm_beam_out;
+
+PM_API size_t pm_beam_select_workspace_bytes(const pm_beam *b);
+PM_API int pm_beam_select(const pm_beam *b, const pm_beam_out *out, void *workspace, size_t workspace_bytes,
+                          void *stream);
+
 /* pm_sample_rows on scratch owned by the library (no counterpart in the
  * reference, which runs on MLX's allocator): for callers that cannot hand
  * over a device workspace or must not allocate between decode steps.

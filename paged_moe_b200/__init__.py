@@ -4,6 +4,8 @@ Public API:
     make_sampler, make_logits_processors   drop-ins for mlx-lm's factories
     sample_rows, apply_processors, logprobs batched fast paths ([B, V] at once)
     verify                                  draft acceptance of a verify pass
+    top_logprobs                            the k best tokens of every row, with log-probabilities
+    beam_select                             one step of beam search
     sampling                                request defaults (pagedmoe/sampling.py)
 
 The CUDA library (libpm_sample.so) is loaded on the first call that launches
@@ -15,7 +17,8 @@ when the library is missing or does not load.
 from . import _lib
 from . import sampling  # noqa: F401  (host-side defaults, pure Python)
 from .params import ProcessorSettings, SamplerSettings  # noqa: F401
-from .engine import apply_processors, argmax_confidence, logprobs, sample_rows  # noqa: E402,F401
+from .engine import apply_processors, argmax_confidence, logprobs, sample_rows, top_logprobs  # noqa: E402,F401
+from .beam import beam_select  # noqa: E402,F401
 from .sample_utils import make_logits_processors, make_sampler  # noqa: E402,F401
 from .verify import verify  # noqa: E402,F401
 

@@ -106,6 +106,30 @@ class LmHead(C.Structure):
     ]
 
 
+class TopRows(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_int64), ("vocab", C.c_int64),
+        ("row_stride", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("k", C.c_int32),
+        ("inv_temperature", C.c_double),
+    ]
+
+
+class Beam(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("dtype", C.c_int32), ("items", C.c_int64), ("beams", C.c_int32),
+        ("vocab", C.c_int64), ("row_stride", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+        ("scores", C.c_void_p), ("done", C.c_void_p), ("lengths", C.c_void_p), ("eos", C.c_int32),
+        ("length_penalty", C.c_double), ("n", C.c_int32), ("keep_slots", C.c_int32),
+    ]
+
+
+class BeamOut(C.Structure):
+    _fields_ = [
+        ("scores", C.c_void_p), ("parents", C.c_void_p), ("tokens", C.c_void_p), ("lengths", C.c_void_p),
+        ("done", C.c_void_p),
+    ]
+
+
 # Exported symbols and their signatures: (restype, argtypes)
 _P = C.c_void_p
 SIGNATURES = {
@@ -126,6 +150,9 @@ SIGNATURES = {
     "pm_think_budget": (C.c_int, [_P, _P, C.c_int64, C.c_int64, _P, _P, C.c_int64, _P, _P, C.c_int32, C.c_int32,
                                   C.c_int32, C.c_int32, _P, _P]),
     "pm_draft_ngram": (C.c_int, [_P, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
+    "pm_top_logprobs": (C.c_int, [_P, _P, _P, _P, _P]),
+    "pm_beam_select_workspace_bytes": (C.c_size_t, [_P]),
+    "pm_beam_select": (C.c_int, [_P, _P, _P, C.c_size_t, _P]),
     "pm_lmhead_logits": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P]),
     "pm_lmhead_sample_workspace_bytes": (C.c_size_t, [_P, _P]),
     "pm_lmhead_sample": (C.c_int, [_P, _P, _P, _P, _P, C.c_size_t, _P]),

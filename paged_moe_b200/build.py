@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libpm_sample.so")
-SOURCES = ["pm_sample.cu", "pm_masked.cu", "pm_lmhead.cu"]
+SOURCES = ["pm_sample.cu", "pm_masked.cu", "pm_lmhead.cu", "pm_beam.cu"]
 OBJDIR = os.path.join(HERE, "_build")
 
 NVCC_FLAGS = [
@@ -80,17 +80,21 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with _BuildLock():
         if not force and not _stale():
             return SO
-        return _build_locked(verbose)
+        return _build_locked(verbose, force)
 
 
-def _build_locked(verbose: bool) -> str:
+def _build_locked(verbose: bool, force: bool) -> str:
     os.makedirs(OBJDIR, exist_ok=True)
     cc = nvcc()
     procs = []
     objs = []
+    newest_header = max(os.path.getmtime(h) for h in _headers() + [os.path.abspath(__file__)])
     for src in sources():
         obj = os.path.join(OBJDIR, os.path.basename(src) + ".o")
         objs.append(obj)
+        # an object newer than its source, every header and the flags here is kept
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(newest_header, os.path.getmtime(src)):
+            continue
         cmd = [cc, *NVCC_FLAGS, "-c", "-o", obj + f".{os.getpid()}.tmp", src]
         if verbose:
             print(" ".join(cmd), flush=True)

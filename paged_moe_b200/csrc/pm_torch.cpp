@@ -10,6 +10,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
+#include <cstring>
 #include <optional>
 #include <string>
 #include <vector>
@@ -215,6 +218,190 @@ int64_t verify_workspace_bytes(torch::Tensor logits, torch::Tensor params, bool 
   return (int64_t)pm_verify_workspace_bytes(&r, &va);
 }
 
+// ---------------------------------------------------------------------------
+// Top log-probabilities and beam search.  Arguments are checked here, before
+// any CUDA call: shapes and types first, devices last.
+// ---------------------------------------------------------------------------
+[[noreturn]] void bad_value(const std::string& what) { throw std::invalid_argument(what); }
+[[noreturn]] void bad_type(const std::string& what) { throw pybind11::type_error(what); }
+
+int logits_code(const torch::Tensor& t) {
+  if (t.scalar_type() == torch::kFloat32) return PM_DTYPE_F32;
+  if (t.scalar_type() == torch::kBFloat16) return PM_DTYPE_BF16;
+  bad_type("logits must be float32 or bfloat16, got " + std::string(torch::toString(t.scalar_type())));
+}
+
+// [rows, vocab] with unit stride: the tensor itself where it lies so.
+torch::Tensor as_rows(const torch::Tensor& t) {
+  if (t.dim() < 2) bad_value("logits must have at least two dimensions, the vocabulary last");
+  torch::Tensor r = t;
+  const int64_t V = t.size(-1);
+  if (V < 1) bad_value("the vocabulary is empty");
+  if (t.dim() > 2) {
+    int64_t rows = 1;
+    for (int64_t d = 0; d + 1 < t.dim(); ++d) rows *= t.size(d);
+    r = t.reshape({rows, V});
+  }
+  // a single row's stride says nothing: one that is below V would be refused
+  if ((V > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < V)) r = r.contiguous();
+  return r;
+}
+
+int64_t row_stride(const torch::Tensor& rows) {
+  return rows.size(0) > 1 ? rows.stride(0) : std::max(rows.stride(0), rows.size(1));
+}
+
+void on_device(const torch::Tensor& t, const torch::Device& dev, const char* name) {
+  if (t.device() != dev) bad_value(std::string(name) + " must be on " + dev.str() + ", got " + t.device().str());
+}
+
+void need_cuda(const torch::Tensor& t, const char* name) {
+  if (!t.is_cuda()) bad_value(std::string(name) + " must be a CUDA tensor");
+}
+
+// The allowed-token words of `rows` rows: contiguous [rows, words], or [words]
+// for every row (stride 0).
+struct Mask {
+  torch::Tensor t;
+  const uint32_t* words = nullptr;
+  int64_t stride = 0;
+};
+Mask check_mask(const OptT& mask, int64_t rows, int64_t V) {
+  Mask m;
+  if (!mask.has_value()) return m;
+  if (mask->scalar_type() != torch::kInt32 && mask->scalar_type() != torch::kUInt32)
+    bad_type("mask must be packed 32-bit words (int32 or uint32)");
+  if (mask->dim() < 1 || mask->size(-1) < (V + 31) / 32) bad_value("mask has fewer than ceil(vocab/32) words per row");
+  m.t = mask->contiguous();
+  if (m.t.dim() > 1) {
+    m.stride = m.t.size(-1);
+    if (m.t.numel() != rows * m.stride) bad_value("mask must be [words] or one row of words per row of logits");
+  }
+  m.words = reinterpret_cast<const uint32_t*>(m.t.data_ptr());
+  return m;
+}
+
+// pm_top_logprobs: [ids [N, k], logprobs [N, k], lse [N] or empty]
+std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, double temp, OptT mask, bool want_lse) {
+  pm_top_rows t;
+  std::memset(&t, 0, sizeof(t));
+  t.dtype = logits_code(logits);
+  if (logits.dim() != 2) bad_value("logits must be [rows, vocab]");
+  if (k < 1) bad_value("k must be at least 1");
+  if (!(temp > 0.0) || std::isinf(temp)) bad_value("temp must be positive");
+  torch::Tensor x = as_rows(logits);
+  const Mask m = check_mask(mask, x.size(0), x.size(1));
+  need_cuda(x, "logits");
+  if (m.words) on_device(m.t, x.device(), "mask");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t N = x.size(0);
+  t.logits = x.data_ptr();
+  t.rows = N;
+  t.vocab = x.size(1);
+  t.row_stride = row_stride(x);
+  t.mask = m.words;
+  t.mask_stride = m.stride;
+  t.k = (int32_t)std::min<int64_t>(k, 0x7fffffff);
+  t.inv_temperature = 1.0 / temp;
+  if (k > 256) check(PM_ERR_UNSUPPORTED, "pm_top_logprobs");  // before any allocation
+  torch::Tensor buf = torch::empty({N * (2 * k + (want_lse ? 1 : 0))}, x.options().dtype(torch::kInt32));
+  torch::Tensor ids = buf.narrow(0, 0, N * k).view({N, k});
+  torch::Tensor lp = buf.narrow(0, N * k, N * k).view(torch::kFloat32).view({N, k});
+  torch::Tensor lse = want_lse ? buf.narrow(0, 2 * N * k, N).view(torch::kFloat32) : buf.narrow(0, 0, 0);
+  check(pm_top_logprobs(&t, ids.data_ptr<int32_t>(), lp.data_ptr<float>(), want_lse ? lse.data_ptr<float>() : nullptr,
+                        stream_of(x.device())),
+        "pm_top_logprobs");
+  return {ids, lp, lse};
+}
+
+// pm_beam_select: [scores, parents, tokens, lengths or empty, done or empty]
+std::vector<torch::Tensor> beam_select(torch::Tensor logits, torch::Tensor scores, int64_t n, OptT mask, OptT done,
+                                       int64_t eos, OptT lengths, double length_penalty, bool keep_slots) {
+  pm_beam b;
+  std::memset(&b, 0, sizeof(b));
+  b.dtype = logits_code(logits);
+  if (scores.dim() != 2) bad_value("scores must be [items, beams]");
+  if (scores.scalar_type() != torch::kFloat32) bad_type("scores must be float32");
+  const int64_t B = scores.size(0), W = scores.size(1);
+  if (W < 1) bad_value("there must be at least one beam");
+  torch::Tensor x = as_rows(logits);
+  if (x.size(0) != B * W || (logits.dim() == 3 && logits.size(0) != B) || logits.dim() > 3)
+    bad_value("logits must be [items, beams, vocab] or [items * beams, vocab]");
+  const int64_t V = x.size(1);
+  if (n < 1) bad_value("n must be at least 1");
+  if (keep_slots && n != W) bad_value("keep_slots needs n equal to the number of beams");
+  if (eos < -1 || eos > 0x7fffffff) bad_value("eos must be a token id");
+  if (!(std::fabs(length_penalty) <= 16.0)) bad_value("length_penalty must lie within [-16, 16]");
+  if (length_penalty != 0.0 && !lengths.has_value()) bad_value("length_penalty needs lengths");
+  if (done.has_value()) {
+    if (eos < 0) bad_value("done needs eos, the token that finished beams go on with");
+    if (done->scalar_type() != torch::kBool && done->scalar_type() != torch::kUInt8) bad_type("done must be bool");
+    if (done->dim() != 2 || done->size(0) != B || done->size(1) != W) bad_value("done must be [items, beams]");
+    done = done->contiguous();
+  }
+  if (lengths.has_value()) {
+    if (lengths->scalar_type() != torch::kInt32) bad_type("lengths must be int32");
+    if (lengths->dim() != 2 || lengths->size(0) != B || lengths->size(1) != W)
+      bad_value("lengths must be [items, beams]");
+    lengths = lengths->contiguous();
+  }
+  const Mask m = check_mask(mask, B * W, V);
+  need_cuda(x, "logits");
+  scores = scores.contiguous();
+  on_device(scores, x.device(), "scores");
+  if (m.words) on_device(m.t, x.device(), "mask");
+  if (done.has_value()) on_device(*done, x.device(), "done");
+  if (lengths.has_value()) on_device(*lengths, x.device(), "lengths");
+  const c10::cuda::CUDAGuard guard(x.device());
+  b.logits = x.data_ptr();
+  b.items = B;
+  b.beams = (int32_t)std::min<int64_t>(W, 0x7fffffff);
+  b.vocab = V;
+  b.row_stride = row_stride(x);
+  b.mask = m.words;
+  b.mask_stride = m.stride;
+  b.scores = scores.data_ptr<float>();
+  b.done = reinterpret_cast<const uint8_t*>(ptr(done));
+  b.lengths = reinterpret_cast<const int32_t*>(ptr(lengths));
+  b.eos = (int32_t)eos;
+  b.length_penalty = length_penalty;
+  b.n = (int32_t)std::min<int64_t>(n, 0x7fffffff);
+  b.keep_slots = keep_slots ? 1 : 0;
+  const size_t need = pm_beam_select_workspace_bytes(&b);
+  if (need == 0) check(PM_ERR_UNSUPPORTED, "pm_beam_select");
+  // workspace and outputs are allocated per call: two captured graphs, or
+  // two streams, never share them
+  torch::Tensor ws = torch::empty({(int64_t)need}, x.options().dtype(torch::kUInt8));
+  const int64_t E = B * n;
+  torch::Tensor buf = torch::empty({E * 3 + (lengths.has_value() ? E : 0) + (eos >= 0 ? (E + 3) / 4 : 0)},
+                                   x.options().dtype(torch::kInt32));
+  std::vector<torch::Tensor> res(5, buf.narrow(0, 0, 0));
+  int64_t at = 0;
+  auto take = [&] {
+    torch::Tensor t = buf.narrow(0, at, E).view({B, n});
+    at += E;
+    return t;
+  };
+  pm_beam_out o;
+  std::memset(&o, 0, sizeof(o));
+  res[0] = take().view(torch::kFloat32);
+  res[1] = take();
+  res[2] = take();
+  o.scores = res[0].data_ptr<float>();
+  o.parents = res[1].data_ptr<int32_t>();
+  o.tokens = res[2].data_ptr<int32_t>();
+  if (lengths.has_value()) {
+    res[3] = take();
+    o.lengths = res[3].data_ptr<int32_t>();
+  }
+  if (eos >= 0) {
+    res[4] = buf.narrow(0, at, (E + 3) / 4).view(torch::kUInt8).narrow(0, 0, E).view(torch::kBool).view({B, n});
+    o.done = reinterpret_cast<uint8_t*>(res[4].data_ptr());
+  }
+  check(pm_beam_select(&b, &o, ws.data_ptr(), need, stream_of(x.device())), "pm_beam_select");
+  return res;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -223,5 +410,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample_workspace_bytes", &sample_workspace_bytes);
   m.def("verify", &verify);
   m.def("verify_workspace_bytes", &verify_workspace_bytes);
+  m.def("top_logprobs", &top_logprobs);
+  m.def("beam_select", &beam_select);
   m.def("version", [] { return std::string(pm_version()); });
 }

@@ -379,6 +379,25 @@ def logprobs(logits: torch.Tensor, processors=None, history=None, history_len=No
     return out, lse
 
 
+def top_logprobs(logits: torch.Tensor, k: int, temp: float = 1.0, mask: Optional[torch.Tensor] = None,
+                 return_lse: bool = False):
+    """The k largest logits of every row and their log-probabilities.
+
+    logits [N, V] fp32 or bf16 on a CUDA device; mask: packed allowed-token
+    words [N, W], or [W] for every row.  Log-probabilities are those of
+    softmax(logits / temp) over the allowed tokens: what an API answers with
+    beside a token, or a teacher's targets for distill_loss.
+
+    Returns {"ids": [N, k] int32, "logprobs": [N, k] fp32} in descending
+    order (ties: the lowest id), and "lse" [N] fp32, the log-sum-exp of
+    logits / temp, when asked.  Disallowed and -inf tokens are no candidates:
+    places left over hold id -1 and -inf.  A row with a NaN or +inf among its
+    allowed logits gives ids -1 and NaN.  1 <= k <= 256.
+    """
+    ids, lp, lse = L.ext().top_logprobs(logits, k, temp, mask, return_lse)
+    return {"ids": ids, "logprobs": lp, "lse": lse} if return_lse else {"ids": ids, "logprobs": lp}
+
+
 def argmax_confidence(logits: torch.Tensor, processors=None, history=None, mask=None):
     """Greedy token and its softmax probability per row: the reduction of
     each MTP draft-chain step (reference pagedmoe/mtp.py:731-746, argmax and
