@@ -362,6 +362,33 @@ PM_API size_t pm_beam_select_workspace_bytes(const pm_beam *b);
 PM_API int pm_beam_select(const pm_beam *b, const pm_beam_out *out, void *workspace, size_t workspace_bytes,
                           void *stream);
 
+/* Moves per-beam states to the beams that continue them (no counterpart in
+ * the reference): row i * beams + j of every state becomes row i * beams +
+ * parents[i, j] as it was before the call; a parent outside [0, beams) leaves
+ * the row its own.  One launch moves up to PM_MAX_STATES states, in place
+ * (dst == src, the same strides; only rows whose parent is another are
+ * touched) or into a second buffer (every row is written).  A row is `outer`
+ * runs of run_bytes bytes each.  With lengths [items, beams] and pos_bytes >
+ * 0 only the first lengths[parent's row] positions of a run move, pos_bytes
+ * bytes each; what lies behind them in the destination stays as it was.
+ * States must not overlap one another. */
+#define PM_MAX_STATES 128
+
+typedef struct pm_state {
+    const void *src;
+    void *dst;
+    int64_t src_row_stride;      /* bytes between rows */
+    int64_t dst_row_stride;
+    int64_t outer;               /* runs of a row, >= 1 */
+    int64_t src_outer_stride;    /* bytes between a row's runs */
+    int64_t dst_outer_stride;
+    int64_t run_bytes;           /* bytes of a run */
+    int64_t pos_bytes;           /* bytes of one position of a run, 0: the state has no positions */
+} pm_state;
+
+PM_API int pm_beam_reorder(const pm_state *states, int32_t n_states, const int32_t *parents, int64_t parents_stride,
+                           const int32_t *lengths, int64_t items, int32_t beams, void *stream);
+
 /* pm_sample_rows on scratch owned by the library (no counterpart in the
  * reference, which runs on MLX's allocator): for callers that cannot hand
  * over a device workspace or must not allocate between decode steps.

@@ -5,7 +5,7 @@ Public API:
     sample_rows, apply_processors, logprobs batched fast paths ([B, V] at once)
     verify                                  draft acceptance of a verify pass
     top_logprobs                            the k best tokens of every row, with log-probabilities
-    beam_select                             one step of beam search
+    beam_select, beam_reorder               one step of beam search, and its states moved
     sampling                                request defaults (pagedmoe/sampling.py)
 
 The CUDA library (libpm_sample.so) is loaded on the first call that launches
@@ -18,7 +18,7 @@ from . import _lib
 from . import sampling  # noqa: F401  (host-side defaults, pure Python)
 from .params import ProcessorSettings, SamplerSettings  # noqa: F401
 from .engine import apply_processors, argmax_confidence, logprobs, sample_rows, top_logprobs  # noqa: E402,F401
-from .beam import beam_select  # noqa: E402,F401
+from .beam import beam_reorder, beam_select  # noqa: E402,F401
 from .sample_utils import make_logits_processors, make_sampler  # noqa: E402,F401
 from .verify import verify  # noqa: E402,F401
 

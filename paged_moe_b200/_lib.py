@@ -130,6 +130,14 @@ class BeamOut(C.Structure):
     ]
 
 
+class State(C.Structure):
+    _fields_ = [
+        ("src", C.c_void_p), ("dst", C.c_void_p), ("src_row_stride", C.c_int64), ("dst_row_stride", C.c_int64),
+        ("outer", C.c_int64), ("src_outer_stride", C.c_int64), ("dst_outer_stride", C.c_int64),
+        ("run_bytes", C.c_int64), ("pos_bytes", C.c_int64),
+    ]
+
+
 # Exported symbols and their signatures: (restype, argtypes)
 _P = C.c_void_p
 SIGNATURES = {
@@ -153,6 +161,7 @@ SIGNATURES = {
     "pm_top_logprobs": (C.c_int, [_P, _P, _P, _P, _P]),
     "pm_beam_select_workspace_bytes": (C.c_size_t, [_P]),
     "pm_beam_select": (C.c_int, [_P, _P, _P, C.c_size_t, _P]),
+    "pm_beam_reorder": (C.c_int, [_P, C.c_int32, _P, C.c_int64, _P, C.c_int64, C.c_int32, _P]),
     "pm_lmhead_logits": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P]),
     "pm_lmhead_sample_workspace_bytes": (C.c_size_t, [_P, _P]),
     "pm_lmhead_sample": (C.c_int, [_P, _P, _P, _P, _P, C.c_size_t, _P]),

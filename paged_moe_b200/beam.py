@@ -1,4 +1,5 @@
-"""Beam search on the device: the selection over beams and vocabulary.
+"""Beam search on the device: the selection over beams and vocabulary, and
+the reordering of the states that belong to the beams.
 
 The reference decodes one sequence per request (pagedmoe/verify_decode.py:727
 generate_step); this is the step that keeps several.  It reads the logits
@@ -8,7 +9,7 @@ on the device: a whole step runs without the host.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence, Union
 
 import torch
 
@@ -52,3 +53,41 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
     if eos is not None:
         res["done"] = out[4]
     return res
+
+
+def beam_reorder(states: Union[torch.Tensor, Sequence[torch.Tensor]], parents: torch.Tensor,
+                 out: Union[torch.Tensor, Sequence[torch.Tensor], None] = None,
+                 lengths: Optional[torch.Tensor] = None,
+                 seq_dim: Union[int, None, Sequence[Optional[int]]] = None):
+    """Moves every state's rows to the beams that continue them.
+
+    states: one tensor or several of any type, [B*W, ...] with the beams of an
+    item next to one another (key-value caches, recurrent states, token
+    histories).  parents [B, W] int32, as beam_select gives them (a slice
+    [:, :W] of more candidates will do): row b*W + j takes what row b*W +
+    parents[b, j] held before the call.  A parent outside [0, W) leaves the
+    row its own.
+
+    Without out the states are reordered in place, and only rows whose parent
+    is another row are touched.  With out (one tensor per state, the same
+    shapes; a double buffer) every row is written there and the states stay.
+
+    lengths [B, W] or [B*W] int32 (those before the reorder) with seq_dim, the
+    dimension of a state that counts positions (one for all states, or one
+    per state, None for a state without): only the first lengths[parent] positions
+    move; positions behind them stay as they were.
+
+    A state has to be dense from its position dimension on (without
+    positions: any split into leading dimensions that collapse and a dense
+    rest), and states, and out, must not overlap.  All states move in one
+    launch (up to 128).  Returns out, or the states.
+    """
+    one = isinstance(states, torch.Tensor)
+    s = [states] if one else list(states)
+    o = None if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    dims = seq_dim if isinstance(seq_dim, (list, tuple)) else [seq_dim] * len(s)
+    flat = [-1 if d is None else d + t.dim() if d < 0 else d for d, t in zip(dims, s)] if len(dims) == len(s) else []
+    if any(d is not None and f < 0 for d, f in zip(dims, flat)):
+        raise ValueError("seq_dim is out of range")
+    L.ext().beam_reorder(s, parents, o, lengths, flat)
+    return states if out is None else out

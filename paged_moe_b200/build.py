@@ -15,7 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libpm_sample.so")
-SOURCES = ["pm_sample.cu", "pm_masked.cu", "pm_lmhead.cu", "pm_beam.cu"]
+SOURCES = ["pm_sample.cu", "pm_masked.cu", "pm_lmhead.cu", "pm_beam.cu",
+           "pm_reorder.cu"]
 OBJDIR = os.path.join(HERE, "_build")
 
 NVCC_FLAGS = [

@@ -402,6 +402,113 @@ std::vector<torch::Tensor> beam_select(torch::Tensor logits, torch::Tensor score
   return res;
 }
 
+// One state of beam_reorder as (row, run) geometry.  dim: the dimension of
+// positions, or -1.  The dimensions from `dim` on have to be dense; those
+// between the rows and it have to collapse into one.
+void state_geometry(const torch::Tensor& t, int64_t dim, const std::string& name, int64_t* outer, int64_t* outer_stride,
+                    int64_t* run, int64_t* pos) {
+  const int64_t size = t.element_size(), D = t.dim();
+  for (int64_t d = 0; d < D; ++d)
+    if (t.size(d) > 1 && t.stride(d) == 0) bad_value(name + " has rows or elements that share memory (expanded)");
+  // dense from the last dimension up to `first`
+  int64_t first = D, n = 1;
+  while (first > 1 && (t.size(first - 1) == 1 || t.stride(first - 1) == n)) n *= t.size(--first);
+  if (dim >= 0 && first > dim) bad_value(name + " must be dense from its position dimension on");
+  const int64_t split = dim >= 0 ? dim : first;
+  int64_t dense = 1;
+  for (int64_t d = split; d < D; ++d) dense *= t.size(d);
+  *run = dense * size;
+  *pos = dim >= 0 ? (t.size(dim) ? dense / t.size(dim) * size : size) : 0;
+  *outer = 1;
+  *outer_stride = 0;
+  for (int64_t d = split - 1; d >= 1; --d) {
+    if (t.size(d) == 1) continue;
+    if (*outer == 1) {
+      *outer_stride = t.stride(d) * size;
+    } else if (t.stride(d) * size != *outer_stride * *outer) {
+      bad_value(name + " has dimensions between its rows and its dense part that do not collapse into one");
+    }
+    *outer *= t.size(d);
+  }
+  if (*outer == 0) { *outer = 1; *run = 0; }
+}
+
+// pm_beam_reorder over any number of states, PM_MAX_STATES a launch.
+void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
+                  std::optional<std::vector<torch::Tensor>> out, OptT lengths, std::vector<int64_t> dims) {
+  if (parents.dim() != 2) bad_value("parents must be [items, beams]");
+  if (parents.scalar_type() != torch::kInt32) bad_type("parents must be int32");
+  const int64_t B = parents.size(0), W = parents.size(1);
+  if (W < 1) bad_value("there must be at least one beam");
+  if (out.has_value() && out->size() != states.size()) bad_value("out must hold one tensor per state");
+  if (dims.size() != states.size()) bad_value("seq_dim must be one dimension, or one per state");
+  if (lengths.has_value()) {
+    if (lengths->scalar_type() != torch::kInt32) bad_type("lengths must be int32");
+    if (lengths->numel() != B * W || lengths->dim() > 2 || (lengths->dim() == 2 && lengths->size(1) != W))
+      bad_value("lengths must be [items, beams] or [items * beams]");
+    lengths = lengths->contiguous();
+  }
+  std::vector<pm_state> s(states.size());
+  std::vector<const void*> read, written;
+  for (size_t i = 0; i < states.size(); ++i) {
+    const torch::Tensor& a = states[i];
+    const std::string name = "state " + std::to_string(i);
+    if (a.dim() < 1 || a.size(0) != B * W) bad_value(name + " must have items * beams rows");
+    int64_t dim = dims[i];
+    if (dim >= 0 && !lengths.has_value()) bad_value("seq_dim needs lengths");
+    if (dim == 0 || dim >= a.dim()) bad_value(name + ": seq_dim must lie behind the row dimension");
+    std::memset(&s[i], 0, sizeof(pm_state));
+    state_geometry(a, dim, name, &s[i].outer, &s[i].src_outer_stride, &s[i].run_bytes, &s[i].pos_bytes);
+    const int64_t size = a.element_size();
+    s[i].src = a.data_ptr();
+    s[i].src_row_stride = a.stride(0) * size;
+    const torch::Tensor& b = out.has_value() ? (*out)[i] : a;
+    s[i].dst = b.data_ptr();
+    s[i].dst_row_stride = b.stride(0) * size;
+    s[i].dst_outer_stride = s[i].src_outer_stride;
+    if (out.has_value()) {
+      if (b.sizes() != a.sizes() || b.scalar_type() != a.scalar_type())
+        bad_value("out of " + name + " must have its shape and type");
+      int64_t outer, run, pos;
+      state_geometry(b, dim, "out of " + name, &outer, &s[i].dst_outer_stride, &run, &pos);
+      if (run != s[i].run_bytes || outer != s[i].outer) {
+        // one of the two is dense where the other has several runs: its runs
+        // follow one another
+        const bool shorter = run < s[i].run_bytes;
+        if ((shorter ? s[i].outer : outer) != 1) bad_value("out of " + name + " must be laid out like it");
+        s[i].run_bytes = std::min(run, s[i].run_bytes);
+        s[i].outer = std::max(outer, s[i].outer);
+        (shorter ? s[i].src_outer_stride : s[i].dst_outer_stride) = s[i].run_bytes;
+      }
+    }
+    if (a.numel() == 0) { s[i].run_bytes = 0; continue; }
+    read.push_back(s[i].src);
+    written.push_back(s[i].dst);
+  }
+  // the same memory twice would be moved twice, or read after it was written
+  std::vector<const void*> seen = written;
+  std::sort(seen.begin(), seen.end());
+  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) bad_value("two states share their memory");
+  if (out.has_value())
+    for (const void* p : read)
+      if (std::binary_search(seen.begin(), seen.end(), p)) bad_value("out shares its memory with a state");
+  need_cuda(parents, "parents");
+  const torch::Device dev = parents.device();
+  if (lengths.has_value()) on_device(*lengths, dev, "lengths");
+  for (size_t i = 0; i < states.size(); ++i) {
+    on_device(states[i], dev, "states");
+    if (out.has_value()) on_device((*out)[i], dev, "out");
+  }
+  if ((W > 1 && parents.stride(1) != 1) || (B > 1 && parents.stride(0) < W)) parents = parents.contiguous();
+  const c10::cuda::CUDAGuard guard(dev);
+  for (size_t i = 0; i < s.size(); i += PM_MAX_STATES)
+    check(pm_beam_reorder(s.data() + i, (int32_t)std::min<size_t>(PM_MAX_STATES, s.size() - i),
+                          parents.data_ptr<int32_t>(), B > 1 ? parents.stride(0) : W,
+                          reinterpret_cast<const int32_t*>(ptr(lengths)), B, (int32_t)std::min<int64_t>(W, 0x7fffffff),
+                          stream_of(dev)),
+          "pm_beam_reorder");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -412,5 +519,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("verify_workspace_bytes", &verify_workspace_bytes);
   m.def("top_logprobs", &top_logprobs);
   m.def("beam_select", &beam_select);
+  m.def("beam_reorder", &beam_reorder);
   m.def("version", [] { return std::string(pm_version()); });
 }

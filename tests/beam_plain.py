@@ -94,3 +94,22 @@ def beam_select(x, scores, n, allowed=None, done=None, eos=-1, lengths=None, alp
             o = slots[j]
             S[b, o], P[b, o], T[b, o], Ln[b, o], D[b, o] = c[3], c[1], c[4], c[5], c[6]
     return S, P, T, Ln, D
+
+
+def reorder(state, parents, into=None, lengths=None, seq_dim=None):
+    """state [B*W, ...]; what lands in `into` (the state itself if None)."""
+    B, W = parents.shape
+    out = (state if into is None else into).copy()
+    for b in range(B):
+        for j in range(W):
+            p = int(parents[b, j])
+            if p < 0 or p >= W:
+                p = j
+            src = state[b * W + p]
+            if lengths is None or seq_dim is None:
+                out[b * W + j] = src
+            else:
+                n = min(max(int(lengths[b, p]), 0), state.shape[seq_dim])
+                at = (slice(None),) * (seq_dim - 1) + (slice(0, n),)
+                out[b * W + j][at] = src[at]
+    return out

@@ -118,3 +118,77 @@ def test_beam_select_c_workspace_and_outputs():
     o.tokens = None
     assert lib.pm_beam_select(C.byref(b), C.byref(o), 0x9000, need, None) == L.PM_ERR_ARG
     assert lib.pm_beam_select(C.byref(_beam(items=0)), C.byref(o), None, 0, None) == L.PM_OK
+
+
+_PAR = torch.zeros((2, 3), dtype=torch.int32)
+
+
+@pytest.mark.parametrize("states,kw,err", [
+    (torch.zeros(5, 4), {}, ValueError),                               # rows
+    (torch.zeros(6, 4), dict(parents=_PAR.long()), TypeError),
+    (torch.zeros(6, 4), dict(parents=_PAR[0]), ValueError),
+    (torch.zeros(6, 4), dict(seq_dim=1), ValueError),                  # without lengths
+    (torch.zeros(6, 4), dict(seq_dim=0, lengths=_PAR), ValueError),
+    (torch.zeros(6, 4), dict(seq_dim=2, lengths=_PAR), ValueError),
+    (torch.zeros(6, 4), dict(seq_dim=-3, lengths=_PAR), ValueError),
+    (torch.zeros(6, 4), dict(seq_dim=[1, 1], lengths=_PAR), ValueError),
+    (torch.zeros(6, 4), dict(lengths=_PAR.long()), TypeError),
+    (torch.zeros(6, 4), dict(lengths=_PAR[:, :2]), ValueError),
+    (torch.zeros(1, 4).expand(6, 4), {}, ValueError),                  # rows that share memory
+    (torch.zeros(6, 4, 1).expand(6, 4, 5), {}, ValueError),
+    (torch.zeros(6, 4, 5, 7).permute(0, 3, 1, 2)[:, :, ::2], {}, ValueError),  # does not collapse
+    (torch.zeros(6, 5, 4).transpose(1, 2), dict(seq_dim=1, lengths=_PAR), ValueError),  # not dense behind dim 1
+    (torch.zeros(6, 4), dict(out=torch.zeros(6, 5)), ValueError),
+    (torch.zeros(6, 4), dict(out=torch.zeros(6, 4, dtype=torch.int32)), ValueError),
+    (torch.zeros(6, 4), dict(out=[]), ValueError),
+    (torch.zeros(6, 4), {}, ValueError),                               # host tensors
+])
+def test_beam_reorder_refuses(states, kw, err):
+    a = dict(parents=_PAR)
+    a.update(kw)
+    with pytest.raises(err):
+        pm.beam_reorder(states, **a)
+
+
+def test_beam_reorder_refuses_the_same_memory_twice():
+    t, u = torch.zeros(6, 4), torch.zeros(6, 4)
+    with pytest.raises(ValueError, match="share"):
+        pm.beam_reorder([t, t], _PAR)
+    with pytest.raises(ValueError, match="share"):
+        pm.beam_reorder([t, u], _PAR, out=[u, torch.zeros(6, 4)])
+    with pytest.raises(ValueError, match="share"):
+        pm.beam_reorder(t, _PAR, out=t)
+
+
+def _state(**kw):
+    s = L.State()
+    s.src = s.dst = 0x10000
+    s.src_row_stride = s.dst_row_stride = 256
+    s.outer, s.run_bytes = 1, 256
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+@pytest.mark.parametrize("bad,call,rc", [
+    (dict(outer=0), {}, L.PM_ERR_ARG), (dict(run_bytes=-1), {}, L.PM_ERR_ARG), (dict(src=None), {}, L.PM_ERR_ARG),
+    (dict(pos_bytes=100), {}, L.PM_ERR_ARG), (dict(dst_row_stride=512), {}, L.PM_ERR_ARG),
+    ({}, dict(beams=0), L.PM_ERR_ARG), ({}, dict(beams=65, stride=65), L.PM_ERR_UNSUPPORTED),
+    ({}, dict(parents=None), L.PM_ERR_ARG), ({}, dict(stride=1), L.PM_ERR_ARG), ({}, dict(items=-1), L.PM_ERR_ARG),
+    ({}, dict(n=129), L.PM_ERR_UNSUPPORTED), ({}, dict(n=-1), L.PM_ERR_ARG),
+])
+def test_beam_reorder_c_checks(bad, call, rc):
+    a = dict(n=1, parents=0x2000, stride=4, items=2, beams=4)
+    a.update(call)
+    arr = (L.State * max(1, a["n"]))(*[_state(**bad) for _ in range(max(1, a["n"]))])
+    got = L.load().pm_beam_reorder(arr, a["n"], a["parents"], a["stride"], None, a["items"], a["beams"], None)
+    assert got == rc
+
+
+def test_beam_reorder_c_nothing_to_do():
+    arr = (L.State * 1)(_state(run_bytes=0))
+    lib = L.load()
+    assert lib.pm_beam_reorder(arr, 1, 0x2000, 4, None, 2, 4, None) == L.PM_OK
+    assert lib.pm_beam_reorder(None, 0, None, 0, None, 2, 4, None) == L.PM_OK
+    arr = (L.State * 1)(_state())
+    assert lib.pm_beam_reorder(arr, 1, None, 0, None, 0, 4, None) == L.PM_OK
