@@ -389,6 +389,61 @@ typedef struct pm_state {
 PM_API int pm_beam_reorder(const pm_state *states, int32_t n_states, const int32_t *parents, int64_t parents_stride,
                            const int32_t *lengths, int64_t items, int32_t beams, void *stream);
 
+/* Distillation loss of a draft model from a teacher's top log-probabilities
+ * (no counterpart in the reference, which loads its drafters ready trained,
+ * pagedmoe/mtp.py): the KL divergence that lowers the rejections of
+ * pm_verify's residual mode.  Row r has the student's logits x and up to k
+ * teacher entries (ids, logprobs), those of pm_top_logprobs at the same
+ * temperature T; ids outside [0, vocab) are no entries.  With q = softmax(x / T):
+ *   PM_TAIL_DROP    p = the entries' probabilities divided by their sum:
+ *       loss = sum p_v (log p_v - log q_v)
+ *       dloss/dx_v = (q_v - p_v) / T
+ *   PM_TAIL_BUCKET  p as given; the rest p_t = max(0, 1 - sum p) and q_t = the
+ *       student's mass outside the entries are one more outcome:
+ *       loss = sum p_v (log p_v - log q_v) + p_t (log p_t - log q_t)
+ *       dloss/dx_v = (q_v - p_v) / T on the entries, q_v (1 - p_t / q_t) / T elsewhere
+ *       (q_t below 2^-100 counts as 2^-100; without a token outside the
+ *       entries the bucket is left out)
+ * An id listed twice has the sum of its entries' probabilities.  A row whose
+ * entries hold no mass has loss 0 and gradient 0 under PM_TAIL_DROP.  weights
+ * [rows] multiply the rows; a row of weight 0 is not read, its loss and
+ * gradient are 0.  PM_REDUCE_MEAN divides by the sum of the weights (by
+ * rows without weights; a sum of 0 gives 0).  1 <= k <= 256. */
+#define PM_TAIL_DROP 0
+#define PM_TAIL_BUCKET 1
+#define PM_REDUCE_NONE 0
+#define PM_REDUCE_SUM 1
+#define PM_REDUCE_MEAN 2
+
+typedef struct pm_distill {
+    const void *logits;          /* [rows, row_stride] of dtype */
+    int32_t dtype;               /* PM_DTYPE_* */
+    int64_t rows;
+    int64_t vocab;
+    int64_t row_stride;
+    const int32_t *ids;          /* [rows, k] */
+    const float *logprobs;       /* [rows, k] */
+    int32_t k;
+    double inv_temperature;
+    int32_t tail;                /* PM_TAIL_* */
+    int32_t reduction;           /* PM_REDUCE_* */
+    const float *weights;        /* [rows], or NULL */
+} pm_distill;
+
+/* loss: [rows] under PM_REDUCE_NONE, else one value; NULL: only the gradient.
+ * grad: [rows, grad_stride] of the logits' type, or NULL: only the loss; it
+ * must not overlap the logits.  grad_loss: the gradient of whatever follows
+ * with respect to the loss, [rows] under PM_REDUCE_NONE, else one value; NULL
+ * means 1. */
+PM_API size_t pm_distill_workspace_bytes(const pm_distill *d);
+PM_API int pm_distill_loss(const pm_distill *d, float *loss, void *grad, int64_t grad_stride,
+                           const float *grad_loss, void *workspace, size_t workspace_bytes, void *stream);
+
+/* grad *= *factor (device memory) over [rows, vocab], nothing where it is 1:
+ * a gradient computed with its loss, once the loss's own gradient is known. */
+PM_API int pm_distill_scale(void *grad, int32_t dtype, int64_t rows, int64_t vocab, int64_t grad_stride,
+                            const float *factor, void *stream);
+
 /* pm_sample_rows on scratch owned by the library (no counterpart in the
  * reference, which runs on MLX's allocator): for callers that cannot hand
  * over a device workspace or must not allocate between decode steps.

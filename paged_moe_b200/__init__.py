@@ -6,6 +6,7 @@ Public API:
     verify                                  draft acceptance of a verify pass
     top_logprobs                            the k best tokens of every row, with log-probabilities
     beam_select, beam_reorder               one step of beam search, and its states moved
+    distill_loss                            KL loss of a draft model from a teacher's top_logprobs, with its gradient
     sampling                                request defaults (pagedmoe/sampling.py)
 
 The CUDA library (libpm_sample.so) is loaded on the first call that launches
@@ -19,6 +20,7 @@ from . import sampling  # noqa: F401  (host-side defaults, pure Python)
 from .params import ProcessorSettings, SamplerSettings  # noqa: F401
 from .engine import apply_processors, argmax_confidence, logprobs, sample_rows, top_logprobs  # noqa: E402,F401
 from .beam import beam_reorder, beam_select  # noqa: E402,F401
+from .distill import distill_loss  # noqa: E402,F401
 from .sample_utils import make_logits_processors, make_sampler  # noqa: E402,F401
 from .verify import verify  # noqa: E402,F401
 

@@ -35,6 +35,12 @@ PM_F_FULL = 0x200
 
 PM_STATIC_SCRATCH_BYTES = 32 << 20
 
+PM_TAIL_DROP = 0
+PM_TAIL_BUCKET = 1
+PM_REDUCE_NONE = 0
+PM_REDUCE_SUM = 1
+PM_REDUCE_MEAN = 2
+
 PM_VERIFY_MATCH = 0
 PM_VERIFY_RESIDUAL = 1
 
@@ -138,6 +144,14 @@ class State(C.Structure):
     ]
 
 
+class Distill(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_int64), ("vocab", C.c_int64),
+        ("row_stride", C.c_int64), ("ids", C.c_void_p), ("logprobs", C.c_void_p), ("k", C.c_int32),
+        ("inv_temperature", C.c_double), ("tail", C.c_int32), ("reduction", C.c_int32), ("weights", C.c_void_p),
+    ]
+
+
 # Exported symbols and their signatures: (restype, argtypes)
 _P = C.c_void_p
 SIGNATURES = {
@@ -162,6 +176,9 @@ SIGNATURES = {
     "pm_beam_select_workspace_bytes": (C.c_size_t, [_P]),
     "pm_beam_select": (C.c_int, [_P, _P, _P, C.c_size_t, _P]),
     "pm_beam_reorder": (C.c_int, [_P, C.c_int32, _P, C.c_int64, _P, C.c_int64, C.c_int32, _P]),
+    "pm_distill_workspace_bytes": (C.c_size_t, [_P]),
+    "pm_distill_loss": (C.c_int, [_P, _P, _P, C.c_int64, _P, _P, C.c_size_t, _P]),
+    "pm_distill_scale": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int64, _P, _P]),
     "pm_lmhead_logits": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P]),
     "pm_lmhead_sample_workspace_bytes": (C.c_size_t, [_P, _P]),
     "pm_lmhead_sample": (C.c_int, [_P, _P, _P, _P, _P, C.c_size_t, _P]),

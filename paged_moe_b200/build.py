@@ -16,7 +16,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libpm_sample.so")
 SOURCES = ["pm_sample.cu", "pm_masked.cu", "pm_lmhead.cu", "pm_beam.cu",
-           "pm_reorder.cu"]
+           "pm_reorder.cu", "pm_distill.cu"]
 OBJDIR = os.path.join(HERE, "_build")
 
 NVCC_FLAGS = [

@@ -509,6 +509,78 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
           "pm_beam_reorder");
 }
 
+// pm_distill_loss over logits [..., V] viewed as rows: [loss or empty, grad or
+// empty].  The gradient is [N, V], dense.
+std::vector<torch::Tensor> distill(torch::Tensor logits, torch::Tensor ids, torch::Tensor logprobs, double temp,
+                                   int64_t tail, OptT weights, int64_t reduction, bool want_loss, bool want_grad,
+                                   OptT grad_loss) {
+  pm_distill d;
+  std::memset(&d, 0, sizeof(d));
+  d.dtype = logits_code(logits);
+  if (!(temp > 0.0) || std::isinf(temp)) bad_value("temp must be positive");
+  torch::Tensor x = as_rows(logits.detach());
+  const int64_t N = x.size(0), V = x.size(1);
+  if (ids.dim() < 1 || ids.size(-1) < 1 || ids.numel() != N * ids.size(-1))
+    bad_value("teacher_ids must be [rows, k], one row per row of logits");
+  const int64_t K = ids.size(-1);
+  if (logprobs.sizes() != ids.sizes()) bad_value("teacher_logprobs must have the shape of teacher_ids");
+  if (ids.scalar_type() != torch::kInt32 && ids.scalar_type() != torch::kInt64) bad_type("teacher_ids must be int32 or int64");
+  if (logprobs.scalar_type() != torch::kFloat32 && logprobs.scalar_type() != torch::kBFloat16)
+    bad_type("teacher_logprobs must be float32 or bfloat16");
+  if (weights.has_value()) {
+    if (weights->scalar_type() != torch::kFloat32) bad_type("weights must be float32");
+    if (weights->numel() != N) bad_value("weights must hold one value per row");
+  }
+  if (grad_loss.has_value()) {
+    if (grad_loss->numel() != (reduction == PM_REDUCE_NONE ? N : 1)) bad_value("the loss's gradient has another size");
+  }
+  need_cuda(x, "logits");
+  const torch::Device dev = x.device();
+  on_device(ids, dev, "teacher_ids");
+  on_device(logprobs, dev, "teacher_logprobs");
+  if (weights.has_value()) on_device(*weights, dev, "weights");
+  if (grad_loss.has_value()) on_device(*grad_loss, dev, "the loss's gradient");
+  const c10::cuda::CUDAGuard guard(dev);
+  if (ids.scalar_type() == torch::kInt64)  // ids past 32 bits are no entries either
+    ids = torch::where((ids >= 0).logical_and(ids < V), ids, torch::full({}, -1, ids.options())).to(torch::kInt32);
+  ids = ids.contiguous();
+  logprobs = logprobs.detach().to(torch::kFloat32).contiguous();
+  if (weights.has_value()) weights = weights->detach().contiguous();
+  if (grad_loss.has_value()) grad_loss = grad_loss->detach().to(torch::kFloat32).contiguous();
+  d.logits = x.data_ptr();
+  d.rows = N;
+  d.vocab = V;
+  d.row_stride = row_stride(x);
+  d.ids = ids.data_ptr<int32_t>();
+  d.logprobs = logprobs.data_ptr<float>();
+  d.k = (int32_t)std::min<int64_t>(K, 0x7fffffff);
+  d.inv_temperature = 1.0 / temp;
+  d.tail = (int32_t)tail;
+  d.reduction = (int32_t)reduction;
+  d.weights = reinterpret_cast<const float*>(ptr(weights));
+  const size_t need = pm_distill_workspace_bytes(&d);
+  if (need == 0) check(PM_ERR_UNSUPPORTED, "pm_distill_loss");
+  torch::Tensor ws = torch::empty({(int64_t)need}, x.options().dtype(torch::kUInt8));
+  torch::Tensor loss, grad;
+  if (want_loss)
+    loss = torch::empty(reduction == PM_REDUCE_NONE ? std::vector<int64_t>{N} : std::vector<int64_t>{},
+                        x.options().dtype(torch::kFloat32));
+  if (want_grad) grad = torch::empty({N, V}, x.options());
+  check(pm_distill_loss(&d, want_loss ? loss.data_ptr<float>() : nullptr, want_grad ? grad.data_ptr() : nullptr, V,
+                        reinterpret_cast<const float*>(ptr(grad_loss)), ws.data_ptr(), need, stream_of(dev)),
+        "pm_distill_loss");
+  return {loss, grad};
+}
+
+// grad [N, V] *= factor (one value on the device), in place.
+void distill_scale(torch::Tensor grad, torch::Tensor factor) {
+  const c10::cuda::CUDAGuard guard(grad.device());
+  factor = factor.detach().to(torch::kFloat32).contiguous();
+  check(pm_distill_scale(grad.data_ptr(), logits_code(grad), grad.size(0), grad.size(1), grad.stride(0),
+                         factor.data_ptr<float>(), stream_of(grad.device())),
+        "pm_distill_scale");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -520,5 +592,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("top_logprobs", &top_logprobs);
   m.def("beam_select", &beam_select);
   m.def("beam_reorder", &beam_reorder);
+  m.def("distill", &distill);
+  m.def("distill_scale", &distill_scale);
   m.def("version", [] { return std::string(pm_version()); });
 }
