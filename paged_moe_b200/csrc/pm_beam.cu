@@ -1,19 +1,24 @@
 // pm_beam.cu -- top log-probabilities of rows of logits, and one step of
 // beam search over them.
 //
-// k_top_rows: one CTA streams a row once, in tiles.  Every thread keeps a
-// running maximum m and sum s = sum e^((x - m) / T) of its elements (the sum
-// is rescaled when the maximum grows), and offers every value above the
-// CTA's threshold to a key buffer in shared memory.  A key is
-// (ordered logit bits, ~id): larger logits first, then lower ids, all keys
-// different.  When the buffer holds more than a few hundred keys it is cut to
-// its k largest, and the k-th becomes the threshold: a value that only equals
-// it has a higher id than all that are kept, so the test is strict.
+// k_top_rows: a row is streamed once, by one CTA or, where there are few
+// rows, by a cluster of up to eight that take consecutive parts of it.  Tiles
+// of 256 threads x four 16-byte vectors are loaded one ahead of the one in
+// work.  The loop only adds exponentials and takes maxima: a thread keeps the
+// largest element of its even and of its odd tiles, and the upper 16 bits of
+// each tile's largest go to shared memory.  There is no barrier in it.
 //
-// The log-sum-exp is joined in 64 bits: totals of different beams are
-// compared with one another, and what is lost there would reorder them.
-// Which thread sums which element depends on the element's index alone, never
-// on the row's address, so equal rows get equal bits wherever they lie.
+// The k largest are looked for afterwards.  Each warp sorts its lanes' 64
+// maxima; the least of the eight warps' ceil(k/8)-th largest is a bound that
+// at least k elements reach.  Only the threads' tiles whose maximum reaches
+// it are read once more, about 1.2 k to 2 k of them, and only elements that
+// reach it become keys, (ordered logit bits, ~id): larger logits first, then
+// lower ids, all keys different.  Up to 256 keys are ranked by counting, one
+// a thread; more go through a radix select.  A part with more keys than the
+// buffer holds (long ties, as in a constant row) takes the plain way: one
+// vector of every thread at a time against a running threshold.
+// The cluster's lists and sums meet in its first CTA through distributed
+// shared memory.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -28,10 +33,14 @@
 namespace pm {
 
 constexpr int kTopThreads = 256;
-constexpr int kTopTile = 4096;    // elements of a tile: 16 a thread
+constexpr int kTopWarps = kTopThreads / 32;
+constexpr int kTopU = 4;          // vectors of a thread in a tile
+constexpr int kTopResident = 4;   // CTAs of an SM
 constexpr int kTopMax = 256;      // largest k
-constexpr int kTopSlack = 256;    // keys above k that the buffer holds before it is cut
-constexpr int kTopBuf = kTopTile + kTopMax + kTopSlack;
+constexpr int kTopSplit = 8;      // most CTAs of a row (a portable cluster)
+constexpr int kTopBuf = 2560;     // keys: 2 x the largest k, and one vector of every thread
+constexpr int kTopList = 2048;    // threads' tiles that are read once more
+constexpr int kTopFew = 256;      // keys that are ranked by counting, one a thread
 
 struct TopArgs {
   const void* logits;
@@ -52,106 +61,335 @@ struct TopArgs {
 };
 
 struct TopShared {
-  uint64_t buf[kTopBuf];
+  alignas(16) uint64_t buf[kTopBuf];
   uint64_t best[kTopMax];
+  ExpSum sums[kTopWarps];
+  ExpSum part;
   unsigned hist[256];
   int scal[4];
-  int count;
+  int count;              // keys in buf
+  int got;                // keys in best
+  int listed;
   float thr;
-  float wmax[kTopThreads / 32];
-  double wsum[kTopThreads / 32];
+  float top;              // the part's maximum
+  float wmax[kTopWarps], wbound[kTopWarps];
+  uint16_t list[kTopList];  // (tile of the part) * 256 + thread
+  // then [tiles of the part][256] upper halves of the tiles' ordered maxima
 };
 
+// The float before x, for x > -inf.
+__device__ __forceinline__ float float_below(float x) {
+  uint32_t o = ordkey(x) - 1u;
+  if (o == 0x7fffffffu) --o;  // the place of -0, which compares equal to +0
+  return key_value((uint64_t)o << 32);
+}
+
+// Cuts buf[0, cnt) to its K largest, sorted, in buf and best; sets count, got
+// and the threshold.  Every thread, between barriers.
+__device__ __forceinline__ void top_cut(TopShared& sh, int cnt, int K) {
+  const int tid = threadIdx.x;
+  if (cnt <= kTopFew) {
+    // one key a thread: its rank is the number of larger keys
+    const uint64_t key = tid < cnt ? sh.buf[tid] : 0ull;
+    int rank = 0;
+    if (tid < cnt) {
+      int j = 0;
+      for (; j + 1 < cnt; j += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.buf[j]);
+        rank += (o.x > key) + (o.y > key);
+      }
+      if (j < cnt) rank += sh.buf[j] > key;
+    }
+    __syncthreads();
+    if (tid < cnt && rank < K) {
+      sh.buf[rank] = key;
+      sh.best[rank] = key;
+      if (rank == K - 1) sh.thr = key_value(key);
+    }
+    if (tid == 0) {
+      sh.count = sh.got = cnt < K ? cnt : K;
+      if (cnt < K) sh.thr = kNegInf;
+    }
+  } else {
+    const int got = block_topk_sorted(sh.buf, cnt, K, sh.best, kTopMax, sh.hist, sh.scal);
+    for (int i = tid; i < got; i += kTopThreads) sh.buf[i] = sh.best[i];
+    if (tid == 0) {
+      sh.count = sh.got = got;
+      sh.thr = got == K ? key_value(sh.best[K - 1]) : kNegInf;
+    }
+  }
+  __syncthreads();
+}
+
+// Offers the elements of one vector above `thr`.
 template <typename T>
-__global__ void __launch_bounds__(kTopThreads) k_top_rows(TopArgs a) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  TopShared& sh = *reinterpret_cast<TopShared*>(raw);
+__device__ __forceinline__ void top_offer(TopShared& sh, uint4 raw, uint32_t first, float thr) {
+  float v[RowVec<T>::n];
+  RowVec<T>::unpack(raw, v);
+#pragma unroll
+  for (int e = 0; e < RowVec<T>::n; ++e)
+    if (v[e] > thr) {
+      const int pos = atomicAdd(&sh.count, 1);
+      if (pos < kTopBuf) sh.buf[pos] = rankkey(v[e], first + e);
+    }
+}
+
+// Allowed bits of the n elements from i on.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const uint8_t* mask, int i, int V) {
+  return i < V ? (__ldg(mask + (i >> 3)) >> (i & 7)) & ((1u << RowVec<T>::n) - 1u) : 0u;
+}
+
+template <typename T, bool MASKED, bool ALIGNED>
+__device__ __forceinline__ uint4 top_load(const T* row, int off, const uint8_t* mask, int i, int V) {
+  uint4 raw = load_raw<T, ALIGNED>(row, off, i, V);
+  if (MASKED) raw = RowVec<T>::select(raw, top_bits<T>(mask, i, V));
+  return raw;
+}
+
+// The plain way through elements [i0, i1): any order, any ties.  The buffer
+// never holds more than 2 K keys before a step offers at most one vector of
+// every thread, and elements come in ascending order of ids, so that one
+// which only equals the threshold is out.
+template <typename T, bool MASKED, bool ALIGNED>
+__device__ __noinline__ void top_plain(TopShared& sh, const T* row, int off, const uint8_t* mask, int i0, int i1,
+                                       int V, int K) {
   constexpr int n = RowVec<T>::n;
-  constexpr int U = kTopTile / (kTopThreads * n);
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (tid == 0) { sh.count = 0; sh.thr = kNegInf; }
+  __syncthreads();
+  for (int i = i0; i < i1; i += kTopThreads * n) {
+    top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i + tid * n, V), (uint32_t)(i + tid * n), sh.thr);
+    __syncthreads();
+    const int cnt = sh.count;
+    __syncthreads();
+    if (cnt > 2 * K) top_cut(sh, cnt, K);
+  }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same shared variable of CTA `rank` of the cluster.
+template <typename V>
+__device__ __forceinline__ const V* of_rank(const V* p, uint32_t rank) {
+  uint64_t out;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<const V*>(out);
+}
+
+template <typename T, bool MASKED, bool ALIGNED>
+__global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs a) {
+  extern __shared__ __align__(16) unsigned char shared_bytes[];
+  TopShared& sh = *reinterpret_cast<TopShared*>(shared_bytes);
+  constexpr int n = RowVec<T>::n;
+  constexpr int kTile = kTopThreads * kTopU * n;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t r = blockIdx.x;
-  const int K = a.k;
-  if (a.scores && (a.scores[r] == kNegInf || isnan(a.scores[r]) || (a.done && a.done[r]))) {
-    if (tid == 0) a.lse64[r] = __longlong_as_double(0x7ff8000000000000ll);
+  const uint32_t rank = cluster_rank(), split = cluster_size();
+  const int64_t r = blockIdx.x / split;
+  const int K = a.k, V = (int)a.vocab;
+  uint16_t* tops = reinterpret_cast<uint16_t*>(&sh + 1);
+  // the whole cluster leaves here or none of it
+  if (a.scores && (!(a.scores[r] > kNegInf) || (a.done && a.done[r]))) {
+    if (tid == 0 && rank == 0) a.lse64[r] = nan64();
     return;
   }
   const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
-  const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
-  const uint32_t* mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
-  const float c = (float)(1.4426950408889634 * a.inv_t);
-  if (tid == 0) { sh.count = 0; sh.thr = kNegInf; }
-  __syncthreads();
+  const int off = ALIGNED ? 0 : (int)(reinterpret_cast<uintptr_t>(row) & 15);
+  const uint8_t* mask = MASKED ? reinterpret_cast<const uint8_t*>(a.mask + r * a.mask_stride) : nullptr;
+  const ExpScale scale(a.inv_t);
 
-  float m = kNegInf, s = 0.0f;
-  for (int64_t t0 = 0; t0 < a.vocab; t0 += kTopTile) {
-    const float thr = sh.thr;
-    float v[U][n];
+  const int tiles = (V + kTile - 1) / kTile;
+  const int per = (tiles + (int)split - 1) / (int)split;
+  const int t0 = (int)rank * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+
+  auto at = [&](int t, int u) { return t * kTile + (u * kTopThreads + tid) * n; };
+  auto load_bits = [&](int t, uint32_t (&bits)[kTopU]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_vec<T>(row, t0 + (int64_t)(u * kTopThreads + tid) * n, a.vocab, aligned, mask, v[u]);
-    float tm = kNegInf;
+    for (int u = 0; u < kTopU; ++u) bits[u] = t < t1 ? top_bits<T>(mask, at(t, u), V) : 0u;
+  };
+  auto load_tile = [&](int t, const uint32_t (&bits)[kTopU], uint4 (&raw)[kTopU]) {
+    constexpr uint32_t fill = RowVec<T>::kFill;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < kTopU; ++u)
+      raw[u] = t < t1 && (!MASKED || bits[u]) ? load_raw<T, ALIGNED>(row, off, at(t, u), V)
+                                              : make_uint4(fill, fill, fill, fill);
+  };
+  ExpSum acc;
+  acc.clear();
+  auto work = [&](int t, uint4 (&raw)[kTopU], const uint32_t (&bits)[kTopU], float& m) {
+    float vm[kTopU];
 #pragma unroll
-      for (int e = 0; e < n; ++e) tm = fmaxf(tm, v[u][e]);
-    if (tm > m) { s *= ex2_approx((m - tm) * c); m = tm; }
-    if (m > kNegInf) {
-      float ts = 0.0f;  // the tile's sum first: rounding grows with 16 + tiles, not 16 x tiles
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < n; ++e) ts += ex2_approx((v[u][e] - m) * c);
-      s += ts;
-    } else {
-      // nothing finite so far; a NaN still has to show
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < n; ++e)
-          if (v[u][e] != v[u][e]) s = v[u][e];
+    for (int u = 0; u < kTopU; ++u) {
+      if (MASKED) raw[u] = RowVec<T>::select(raw[u], bits[u]);
+      vm[u] = RowVec<T>::largest(raw[u]);
     }
-    if (tm > thr) {
+    const float tm = fmaxf(max3(vm[0], vm[1], vm[2]), vm[3]);
+    tops[(t - t0) * kTopThreads + tid] = (uint16_t)(ordkey(tm) >> 16);
+    m = fmaxf(m, tm);
+    if (tm > kNegInf) add_exps<T, kTopU>(acc, raw, tm, scale);
+    else acc.add(nan_of<T, kTopU>(raw), kNegInf64);
+  };
+
+  if (tid == 0) { sh.count = 0; sh.got = 0; sh.listed = 0; sh.thr = kNegInf; }
+  float m0 = kNegInf, m1 = kNegInf;  // of the even and the odd tiles
+  {
+    uint4 even[kTopU], odd[kTopU];
+    uint32_t be[kTopU] = {}, bo[kTopU] = {};
+    if (MASKED) load_bits(t0, be);
+    load_tile(t0, be, even);
+    if (MASKED) load_bits(t0 + 1, bo);
+    for (int t = t0; t < t1; t += 2) {
+      uint32_t bn[kTopU] = {};
+      load_tile(t + 1, bo, odd);
+      if (MASKED) load_bits(t + 2, bn);
+      work(t, even, be, m0);
+      load_tile(t + 2, bn, even);
+      if (MASKED) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int u = 0; u < kTopU; ++u) be[u] = bn[u];
+        load_bits(t + 3, bn);
+      }
+      if (t + 1 < t1) work(t + 1, odd, bo, m1);
+      if (MASKED) {
 #pragma unroll
-        for (int e = 0; e < n; ++e)
-          if (v[u][e] > thr)
-            sh.buf[atomicAdd(&sh.count, 1)] =
-                rankkey(v[u][e], (uint32_t)(t0 + (int64_t)(u * kTopThreads + tid) * n + e));
+        for (int u = 0; u < kTopU; ++u) bo[u] = bn[u];
+      }
     }
-    __syncthreads();
-    const int cnt = sh.count;
-    if (cnt > K + kTopSlack || (cnt > K && t0 == 0)) {
-      const int got = block_topk_sorted(sh.buf, cnt, K, sh.best, kTopMax, sh.hist, sh.scal);
-      for (int i = tid; i < got; i += kTopThreads) sh.buf[i] = sh.best[i];
-      if (tid == 0) { sh.count = got; sh.thr = key_value(sh.best[got - 1]); }
-    }
-    __syncthreads();
   }
 
-  // join the threads' (m, s)
-  const float wm = warp_max(m);
-  double d = m > kNegInf ? (double)s * (double)ex2_approx((m - wm) * c) : (double)s;
+  // the bound: the 32 largest of the warp's 64 maxima in descending order
+  auto sorted = [&](float o) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(kFull, d, o);
-  if (lane == 0) { sh.wmax[warp] = wm; sh.wsum[warp] = d; }
-  const int cnt = sh.count;
-  const int got = block_topk_sorted(sh.buf, cnt, K, sh.best, kTopMax, sh.hist, sh.scal);
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        const float p = __shfl_xor_sync(kFull, o, j);
+        o = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(o, p) : fminf(o, p);
+      }
+    return o;
+  };
+  const float m = fmaxf(m0, m1);
+  {
+    const float hi = sorted(m), lo = sorted(fminf(m0, m1));
+    float o = fmaxf(hi, __shfl_sync(kFull, lo, 31 - lane));
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) {
+      const float p = __shfl_xor_sync(kFull, o, j);
+      o = (lane & j) == 0 ? fmaxf(o, p) : fminf(o, p);
+    }
+    o = __shfl_sync(kFull, o, (K + kTopWarps - 1) / kTopWarps - 1);
+    if (lane == 0) sh.wbound[warp] = o;
+  }
   __syncthreads();
-  float M = kNegInf;
+  float bound = sh.wbound[0];
 #pragma unroll
-  for (int w = 0; w < kTopThreads / 32; ++w) M = fmaxf(M, sh.wmax[w]);
-  double S = 0.0;
+  for (int w = 1; w < kTopWarps; ++w) bound = fminf(bound, sh.wbound[w]);
+  const float below = bound > kNegInf ? float_below(bound) : kNegInf;
+  if (m > below) {
+    // without a bound every tile that holds anything
+    const uint32_t least = (ordkey(bound) >> 16) + (bound > kNegInf ? 0u : 1u);
+    for (int t = t0; t < t1; ++t)
+      if (tops[(t - t0) * kTopThreads + tid] >= least) {
+        const int pos = atomicAdd(&sh.listed, 1);
+        if (pos < kTopList) sh.list[pos] = (uint16_t)((t - t0) * kTopThreads + tid);
+      }
+  }
+  __syncthreads();
+  const int listed = sh.listed;
+  if (listed <= kTopList) {
+    for (int j = tid; j < listed * kTopU; j += kTopThreads) {
+      const int g = sh.list[j / kTopU], u = j % kTopU;
+      const int i = (t0 + g / kTopThreads) * kTile + (u * kTopThreads + g % kTopThreads) * n;
+      top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), (uint32_t)i, below);
+    }
+  }
+  __syncthreads();
+  if (listed > kTopList || sh.count > kTopBuf)
+    top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTile, t1 * kTile, V, K);
+
+  // the part's list, maximum and sum
+  acc = warp_join(acc);
+  const float wm = warp_max(m);
+  if (lane == 0) { sh.sums[warp] = acc; sh.wmax[warp] = wm; }
+  __syncthreads();
+  if (tid == 0) {
+    ExpSum s = sh.sums[0];
+    float top = sh.wmax[0];
 #pragma unroll
-  for (int w = 0; w < kTopThreads / 32; ++w)
-    S += sh.wmax[w] > kNegInf ? sh.wsum[w] * (double)ex2_approx((sh.wmax[w] - M) * c) : sh.wsum[w];
-  const bool bad = !(S == S) || isinf(M) && M > 0.0f;
-  const double lse = bad ? __longlong_as_double(0x7ff8000000000000ll) : M == kNegInf ? (double)kNegInf : (double)M * a.inv_t + log(S);
+    for (int w = 1; w < kTopWarps; ++w) {
+      s.add(sh.sums[w].s, sh.sums[w].rho);
+      top = fmaxf(top, sh.wmax[w]);
+    }
+    sh.part = s;
+    sh.top = top;
+  }
+  const int cnt = sh.count;
+  __syncthreads();
+  top_cut(sh, cnt, K);
+
+  if (split > 1) {
+    cluster_sync();
+    if (rank == 0) {
+      // a full list's last key bounds the row's k-th from below
+      uint64_t least = 0;
+      for (uint32_t c = 0; c < split; ++c)
+        if (*of_rank(&sh.got, c) == K) {
+          const uint64_t last = *of_rank(&sh.best[K - 1], c);
+          least = last > least ? last : least;
+        }
+      if (tid == 0) {
+        ExpSum s = sh.part;
+        float top = sh.top;
+        for (uint32_t c = 1; c < split; ++c) {
+          const ExpSum* p = of_rank(&sh.part, c);
+          s.add(p->s, p->rho);
+          top = fmaxf(top, *of_rank(&sh.top, c));
+        }
+        sh.part = s;
+        sh.top = top;
+        sh.count = 0;
+      }
+      __syncthreads();
+      for (int i = tid; i < K * (int)split; i += kTopThreads) {
+        const uint32_t c = (uint32_t)(i / K);
+        const int j = i % K;
+        if (j < *of_rank(&sh.got, c)) {
+          const uint64_t key = *of_rank(&sh.best[j], c);
+          if (key >= least) sh.buf[atomicAdd(&sh.count, 1)] = key;
+        }
+      }
+      __syncthreads();
+      const int all = sh.count;
+      __syncthreads();
+      top_cut(sh, all, K);
+    }
+    cluster_sync();  // the others' shared memory lives until the first CTA has read it
+    if (rank != 0) return;
+  }
+
+  const ExpSum sum = sh.part;
+  const float M = sh.top;
+  const bool bad = !(sum.s == sum.s) || M == -kNegInf;
+  const double lse = bad ? nan64() : M > kNegInf ? scale.log_of(sum, M) : kNegInf64;
+  const int got = bad ? 0 : sh.got;
   if (tid == 0) {
     if (a.lse) a.lse[r] = (float)lse;
-    if (a.lse64) a.lse64[r] = M == kNegInf ? __longlong_as_double(0x7ff8000000000000ll) : lse;
+    if (a.lse64) a.lse64[r] = M > kNegInf ? lse : nan64();
   }
   for (int i = tid; i < K; i += kTopThreads) {
-    const bool have = i < got && !bad;
+    const bool have = i < got;
     const float x = have ? key_value(sh.best[i]) : kNegInf;
     a.ids[r * K + i] = have ? (int32_t)key_index(sh.best[i]) : -1;
     if (a.vals) a.vals[r * K + i] = x;
@@ -176,18 +414,12 @@ struct PickArgs {
   pm_beam_out out;
 };
 
-// One warp per item: the beams' lists are merged by taking the best head n
-// times; lane l holds the heads of beams l and l + 32.
-__global__ void __launch_bounds__(32) k_beam_pick(PickArgs a) {
-  __shared__ int s_par[kTopMax], s_tok[kTopMax];
-  __shared__ double s_tot[kTopMax];
-  const int64_t item = blockIdx.x;
-  const int lane = threadIdx.x, W = a.beams, n = a.n;
-  const double none = (double)kNegInf;
+__device__ __forceinline__ void pick_merge(const PickArgs& a, int64_t row0, int* s_par, int* s_tok, double* s_tot) {
+  const int lane = threadIdx.x & 31, W = a.beams, n = a.n;
+  const double none = kNegInf64;
   double score[2], lse[2], div[2], head[2];
   int at[2];
   bool ended[2];
-  const int64_t row0 = item * W;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int w = lane + 32 * h;
@@ -240,11 +472,62 @@ __global__ void __launch_bounds__(32) k_beam_pick(PickArgs a) {
     }
     if (!have && lane == 0) { s_par[j] = -1; s_tok[j] = -1; s_tot[j] = none; }
   }
-  __syncwarp();
+}
+
+// One CTA per item.  Up to 256 candidates (beams x n) are ranked by counting,
+// one a thread: a candidate's place is the number of better ones, and of
+// equal ones before it.  More are merged by the first warp, which takes the
+// best head n times; lane l holds the heads of beams l and l + 32.
+constexpr int kPickThreads = 256;
+
+__global__ void __launch_bounds__(kPickThreads) k_beam_pick(PickArgs a) {
+  __shared__ int s_par[kTopMax], s_tok[kTopMax];
+  __shared__ double s_tot[kTopMax];
+  __shared__ double s_rank[kPickThreads];
   __shared__ int s_slot[kTopMax];
+  const int64_t item = blockIdx.x;
+  const int tid = threadIdx.x, W = a.beams, n = a.n, all = W * n;
+  const double none = kNegInf64;
+  const int64_t row0 = item * W;
+  cudaGridDependencySynchronize();
+  if (all <= kPickThreads) {
+    double total = none, rank = none;
+    int token = -1;
+    const int w = tid / n, j = tid % n;
+    if (tid < all) {
+      const int64_t r = row0 + w;
+      const double score = (double)a.scores[r], lse = a.lse64[r];
+      const bool ended = a.done && a.done[r];
+      if (score > none) {
+        if (ended) {
+          if (j == 0) { total = score; token = a.eos; }
+        } else if (lse == lse) {
+          const int id = a.ids[r * n + j];
+          if (id >= 0) { total = score + ((double)a.vals[r * n + j] - lse); token = id; }
+        }
+      }
+      rank = total;
+      if (a.lengths && a.alpha != 0.0) {
+        const int len = a.lengths[r] + (ended ? 0 : 1);
+        rank = total / pow((double)(len > 1 ? len : 1), a.alpha);
+      }
+      s_rank[tid] = rank;
+    }
+    for (int i = tid; i < n; i += kPickThreads) { s_par[i] = -1; s_tok[i] = -1; s_tot[i] = none; }
+    __syncthreads();
+    if (tid < all && rank > none) {
+      int place = 0;
+      for (int i = 0; i < all; ++i) place += s_rank[i] > rank || (s_rank[i] == rank && i < tid);
+      if (place < n) { s_par[place] = w; s_tok[place] = token; s_tot[place] = total; }
+    }
+    __syncthreads();
+  } else {
+    if (tid < 32) pick_merge(a, row0, s_par, s_tok, s_tot);
+    __syncthreads();
+  }
   if (!a.keep_slots) {
-    for (int j = lane; j < n; j += 32) s_slot[j] = j;
-  } else if (lane == 0) {
+    for (int j = tid; j < n; j += kPickThreads) s_slot[j] = j;
+  } else if (tid == 0) {
     uint64_t taken = 0;
     for (int j = 0; j < n; ++j) {
       const int p = s_par[j];
@@ -258,8 +541,8 @@ __global__ void __launch_bounds__(32) k_beam_pick(PickArgs a) {
         taken |= 1ull << f;
       }
   }
-  __syncwarp();
-  for (int j = lane; j < n; j += 32) {
+  __syncthreads();
+  for (int j = tid; j < n; j += kPickThreads) {
     const int64_t o = item * n + s_slot[j];
     const int p = s_par[j];
     a.out.scores[o] = (float)s_tot[j];
@@ -279,6 +562,7 @@ __global__ void __launch_bounds__(32) k_beam_pick(PickArgs a) {
 namespace {
 
 constexpr int64_t kMaxVocab = 262144;
+constexpr int64_t kMaxRows = 0x7fffffff;  // a row that is split is one of a few hundred
 
 int check_logits(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                  const uint32_t* mask, int64_t mask_stride) {
@@ -286,25 +570,58 @@ int check_logits(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
   if (dtype != PM_DTYPE_F32 && dtype != PM_DTYPE_BF16) return PM_ERR_ARG;
   if (rows > 0 && !logits) return PM_ERR_ARG;
   if (mask && mask_stride != 0 && mask_stride < (vocab + 31) / 32) return PM_ERR_ARG;
-  if (vocab > kMaxVocab || rows > 0x7fffffff) return PM_ERR_UNSUPPORTED;
+  if (vocab > kMaxVocab || rows > kMaxRows) return PM_ERR_UNSUPPORTED;
   return PM_OK;
 }
 
-template <typename T>
-int launch_top_t(const pm::TopArgs& a, cudaStream_t st) {
+// CTAs of a row: enough to fill the resident CTAs of every SM, no more
+// than it has tiles.
+int top_split(int64_t rows, int64_t tiles) {
+  const int64_t slots = (int64_t)pmh::num_sms() * pm::kTopResident;
+  int c = 1;
+  while (c < pm::kTopSplit && 2 * c <= tiles && rows * 2 * c <= slots) c *= 2;
+  return c;
+}
+
+template <typename T, bool MASKED, bool ALIGNED>
+cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
+  auto* kernel = pm::k_top_rows<T, MASKED, ALIGNED>;
   static pmh::DeviceOnce once;
   cudaError_t e = cudaSuccess;
+  constexpr int64_t kTile = (int64_t)pm::kTopThreads * pm::kTopU * pm::RowVec<T>::n;
+  auto bytes = [](int64_t tiles) { return sizeof(pm::TopShared) + (size_t)tiles * pm::kTopThreads * 2; };
   once([&] {
-    e = cudaFuncSetAttribute(pm::k_top_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(pm::TopShared));
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kMaxVocab / kTile));
   });
-  if (e != cudaSuccess) return pmh::cuda_fail(e);
-  pm::k_top_rows<T><<<(unsigned)a.rows, pm::kTopThreads, sizeof(pm::TopShared), st>>>(a);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? PM_OK : pmh::cuda_fail(e);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (a.vocab + kTile - 1) / kTile;
+  const int split = top_split(a.rows, tiles);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * split));
+  cfg.blockDim = dim3(pm::kTopThreads);
+  cfg.dynamicSmemBytes = bytes((tiles + split - 1) / split);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <typename T>
+cudaError_t launch_top_t(const pm::TopArgs& a, cudaStream_t st) {
+  // rows that all start on a 16-byte boundary are read one vector at a time
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 &&
+                       (a.rows == 1 || a.row_stride * sizeof(T) % 16 == 0);
+  if (a.mask) return aligned ? launch_top_v<T, true, true>(a, st) : launch_top_v<T, true, false>(a, st);
+  return aligned ? launch_top_v<T, false, true>(a, st) : launch_top_v<T, false, false>(a, st);
 }
 
 int launch_top(int dtype, const pm::TopArgs& a, cudaStream_t st) {
-  return dtype == PM_DTYPE_F32 ? launch_top_t<float>(a, st) : launch_top_t<__nv_bfloat16>(a, st);
+  const cudaError_t e = dtype == PM_DTYPE_F32 ? launch_top_t<float>(a, st) : launch_top_t<__nv_bfloat16>(a, st);
+  return e == cudaSuccess ? PM_OK : pmh::cuda_fail(e);
 }
 
 int check_beam(const pm_beam* b) {
@@ -393,7 +710,16 @@ extern "C" int pm_beam_select(const pm_beam* b, const pm_beam_out* out, void* wo
   p.vals = a.vals;
   p.lse64 = a.lse64;
   p.out = *out;
-  pm::k_beam_pick<<<(unsigned)b->items, 32, 0, st>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  // launched while the rows' kernel drains; it waits for that grid itself
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)b->items);
+  cfg.blockDim = dim3(pm::kPickThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, pm::k_beam_pick, p);
   return e == cudaSuccess ? PM_OK : pmh::cuda_fail(e);
 }

@@ -73,6 +73,30 @@ __device__ __forceinline__ double block_add(double v, double* scratch) {
 __device__ __forceinline__ void put_grad(float* g, float v) { *g = v; }
 __device__ __forceinline__ void put_grad(__nv_bfloat16* g, float v) { *g = __float2bfloat16_rn(v); }
 
+// Elements [i, i + n) of a row as fp32, -inf where the row has ended or the
+// mask bit is clear.  Vectors without an allowed element are not read.
+template <typename T>
+__device__ __forceinline__ void load_vec(const T* row, int64_t i, int64_t V, bool aligned, const uint32_t* mask,
+                                         float* v) {
+  constexpr int n = RowVec<T>::n;
+  uint32_t bits = (1u << n) - 1u;
+  if (i + n > V) bits = i >= V ? 0u : (1u << (V - i)) - 1u;
+  if (mask && bits) bits &= __ldg(mask + (i >> 5)) >> (i & 31);
+#pragma unroll
+  for (int e = 0; e < n; ++e) v[e] = kNegInf;
+  if (!bits) return;
+  if (aligned && i + n <= V) {
+    float t[n];
+    RowVec<T>::unpack(__ldg(reinterpret_cast<const uint4*>(row + i)), t);
+#pragma unroll
+    for (int e = 0; e < n; ++e) v[e] = (bits >> e) & 1 ? t[e] : kNegInf;
+  } else {
+#pragma unroll
+    for (int e = 0; e < n; ++e)
+      if ((bits >> e) & 1) v[e] = RowVec<T>::get(row + i + e);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kDistThreads) k_distill(DistillArgs a) {
   extern __shared__ __align__(16) uint32_t marks[];  // one bit per token

@@ -1,4 +1,14 @@
-// pm_rowvec.cuh -- rows of fp32 or bf16 logits read as 16-byte vectors.
+// pm_rowvec.cuh -- rows of fp32 or bf16 logits read as 16-byte vectors, and
+// sums of their exponentials.
+//
+// Sums of e^(x / T) are kept as s 2^rho with s and rho in 64 bits.  A thread
+// sums a tile's vectors in fp32 as 2^(x c - R), c = fl32(log2(e) / T) and R
+// the integer nearest to the tile's largest x c: x c - R is one fused
+// multiply-add, R is exact, and tiles of different R are added with exact
+// powers of two.  So neither the order of the tiles nor how a row is split
+// over CTAs changes more than the last bits of a 64-bit sum: a row's
+// log-sum-exp does not depend on the batch around it.  What c lacks of
+// log2(e) / T is put back once per row, for the row's maximum.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -10,17 +20,41 @@
 namespace pm {
 
 constexpr float kNegInf = -__builtin_inff();
+constexpr double kNegInf64 = -__builtin_inf();
+constexpr double kLog2e64 = 1.4426950408889634;
+constexpr double kLn264 = 0.6931471805599453;
+// Beyond this |x c| an integer R no longer lies within half a unit of x c.
+constexpr float kWildExponent = 1048576.0f;
+
+__device__ __forceinline__ double nan64() { return __longlong_as_double(0x7ff8000000000000ll); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 template <typename T> struct RowVec;
 template <> struct RowVec<float> {
   static constexpr int n = 4;
+  static constexpr uint32_t kFill = 0xff800000u;  // -inf
   static __device__ __forceinline__ void unpack(uint4 r, float* v) {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
   }
   static __device__ __forceinline__ float get(const float* p) { return *p; }
+  static __device__ __forceinline__ float largest(uint4 r) {
+    return max3(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), __uint_as_float(r.z), __uint_as_float(r.w));
+  }
+  // the vector with -inf where bit e of `bits` is clear
+  static __device__ __forceinline__ uint4 select(uint4 r, uint32_t bits) {
+    r.x = bits & 1 ? r.x : kFill; r.y = bits & 2 ? r.y : kFill;
+    r.z = bits & 4 ? r.z : kFill; r.w = bits & 8 ? r.w : kFill;
+    return r;
+  }
 };
 template <> struct RowVec<__nv_bfloat16> {
   static constexpr int n = 8;
+  static constexpr uint32_t kFill = 0xff80ff80u;  // -inf twice
   static __device__ __forceinline__ void unpack(uint4 r, float* v) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -30,30 +64,164 @@ template <> struct RowVec<__nv_bfloat16> {
     }
   }
   static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+  static __device__ __forceinline__ float largest(uint4 r) {
+    const __nv_bfloat162 m = __hmax2(__hmax2(pair(r.x), pair(r.y)), __hmax2(pair(r.z), pair(r.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ uint32_t keep(uint32_t w, uint32_t bits) {
+    // one byte per half word: 0xff where the bit is set
+    const uint32_t m = ((bits & 1) ? 0xffffu : 0u) | ((bits & 2) ? 0xffff0000u : 0u);
+    return (w & m) | (kFill & ~m);
+  }
+  static __device__ __forceinline__ uint4 select(uint4 r, uint32_t bits) {
+    return make_uint4(keep(r.x, bits), keep(r.y, bits >> 2), keep(r.z, bits >> 4), keep(r.w, bits >> 6));
+  }
 };
 
-// Elements [i, i + n) of a row as fp32, -inf where the row has ended or the
-// mask bit is clear.  Vectors without an allowed element are not read.
-template <typename T>
-__device__ __forceinline__ void load_vec(const T* row, int64_t i, int64_t V, bool aligned, const uint32_t* mask,
-                                         float* v) {
+// Elements [i, i + n) of a row, -inf behind its end.  A vector that lies
+// across the end is read element by element.  Rows that do not start on a
+// 16-byte boundary (off: bytes past one) are read as the two aligned vectors
+// that hold the wanted one, each of which holds at least one of its elements.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4 load_raw(const T* row, int off, int i, int V) {
   constexpr int n = RowVec<T>::n;
-  uint32_t bits = (1u << n) - 1u;
-  if (i + n > V) bits = i >= V ? 0u : (1u << (V - i)) - 1u;
-  if (mask && bits) bits &= __ldg(mask + (i >> 5)) >> (i & 31);
-#pragma unroll
-  for (int e = 0; e < n; ++e) v[e] = kNegInf;
-  if (!bits) return;
-  if (aligned && i + n <= V) {
-    float t[n];
-    RowVec<T>::unpack(__ldg(reinterpret_cast<const uint4*>(row + i)), t);
-#pragma unroll
-    for (int e = 0; e < n; ++e) v[e] = (bits >> e) & 1 ? t[e] : kNegInf;
-  } else {
+  if (i + n <= V) {
+    if (ALIGNED) return __ldg(reinterpret_cast<const uint4*>(row + i));
+    const char* at = reinterpret_cast<const char*>(row + i) - off;
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(at));
+    if (off == 0) return a;
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(at + 16));
+    uint32_t w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x, w5 = b.y, w6 = b.z, w7 = b.w;
+    if (off & 8) { w0 = w2; w1 = w3; w2 = w4; w3 = w5; w4 = w6; w5 = w7; }
+    if (off & 4) { w0 = w1; w1 = w2; w2 = w3; w3 = w4; w4 = w5; }
+    if (sizeof(T) == 2) {
+      const int s = (off & 2) * 8;
+      w0 = __funnelshift_r(w0, w1, s); w1 = __funnelshift_r(w1, w2, s);
+      w2 = __funnelshift_r(w2, w3, s); w3 = __funnelshift_r(w3, w4, s);
+    }
+    return make_uint4(w0, w1, w2, w3);
+  }
+  constexpr uint32_t fill = RowVec<T>::kFill;
+  uint4 r = make_uint4(fill, fill, fill, fill);
+  if (i < V) {
+    uint32_t w[4] = {fill, fill, fill, fill};
 #pragma unroll
     for (int e = 0; e < n; ++e)
-      if ((bits >> e) & 1) v[e] = RowVec<T>::get(row + i + e);
+      if (i + e < V) {
+        if (sizeof(T) == 4) {
+          w[e & 3] = __ldg(reinterpret_cast<const uint32_t*>(row) + i + e);
+        } else {
+          const uint32_t h = __ldg(reinterpret_cast<const uint16_t*>(row) + i + e);
+          w[(e >> 1) & 3] = e & 1 ? (w[(e >> 1) & 3] & 0xffffu) | h << 16 : (w[(e >> 1) & 3] & 0xffff0000u) | h;
+        }
+      }
+    r = make_uint4(w[0], w[1], w[2], w[3]);
   }
+  return r;
+}
+
+// 2^d for d <= 0: exact for whole numbers.
+__device__ __forceinline__ double pow2_down(double d) {
+  if (d < -1000.0) return 0.0;
+  const double w = rint(d);
+  if (w == d) return __hiloint2double((1023 + (int)d) << 20, 0);
+  return exp2(d);
+}
+
+// A running sum s 2^rho.
+struct ExpSum {
+  double s, rho;
+  __device__ __forceinline__ void clear() { s = 0.0; rho = kNegInf64; }
+  // += t 2^r; r = -inf stands for nothing but may carry a NaN in t
+  __device__ __forceinline__ void add(double t, double r) {
+    if (r > rho) {
+      s = s * pow2_down(rho - r) + t;  // from nothing: s is 0, or a NaN that stays
+      rho = r;
+    } else if (r == rho) {
+      s += t;
+    } else {
+      s += r > kNegInf64 ? t * pow2_down(r - rho) : t;
+    }
+  }
+};
+
+__device__ __forceinline__ ExpSum warp_join(ExpSum a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double t = __shfl_xor_sync(kFull, a.s, o), r = __shfl_xor_sync(kFull, a.rho, o);
+    // the same two numbers in the same order on both lanes
+    ExpSum b;
+    const bool low = (threadIdx.x & o) == 0;
+    b.s = low ? a.s : t;
+    b.rho = low ? a.rho : r;
+    b.add(low ? t : a.s, low ? r : a.rho);
+    a = b;
+  }
+  return a;
+}
+
+// Constants of a row's exponentials.
+struct ExpScale {
+  float c;        // fl32(log2(e) / T)
+  double exact;   // log2(e) / T
+  __device__ __forceinline__ explicit ExpScale(double inv_t) : exact(kLog2e64 * inv_t) { c = (float)exact; }
+  // natural log of s 2^rho for a row of maximum m
+  __device__ __forceinline__ double log_of(const ExpSum& a, float m) const {
+    const double lost = fabsf(m * c) < kWildExponent ? (double)m * (exact - (double)c) : 0.0;
+    return (a.rho + lost) * kLn264 + log(a.s);
+  }
+};
+
+// Adds the 2^(x c) of U vectors whose largest element is tm > -inf.
+template <typename T, int U>
+__device__ __forceinline__ void add_exps(ExpSum& acc, const uint4 (&raw)[U], float tm, const ExpScale& k) {
+  constexpr int n = RowVec<T>::n;
+  const float top = tm * k.c;
+  if (fabsf(top) < kWildExponent) {
+    const float R = rintf(top);
+    const uint64_t c2 = pk(k.c, k.c), r2 = pk(-R, -R);
+    uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[n];
+      RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+      for (int e = 0; e < n; e += 4) {
+        const uint64_t a = fma2(pk(v[e], v[e + 1]), c2, r2), b = fma2(pk(v[e + 2], v[e + 3]), c2, r2);
+        sum0 = add2(sum0, pk(ex2_approx(lo_f(a)), ex2_approx(hi_f(a))));
+        sum1 = add2(sum1, pk(ex2_approx(lo_f(b)), ex2_approx(hi_f(b))));
+      }
+    }
+    const uint64_t sum = add2(sum0, sum1);
+    acc.add((double)lo_f(sum) + (double)hi_f(sum), (double)R);
+  } else {
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[n];
+      RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+      for (int e = 0; e < n; ++e) sum += ex2_approx((v[e] - tm) * k.c);
+    }
+    acc.add((double)sum, (double)tm * k.exact);
+  }
+}
+
+// NaN if one of the vectors holds a NaN, else 0 (for vectors without a
+// largest element).
+template <typename T, int U>
+__device__ __forceinline__ double nan_of(const uint4 (&raw)[U]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[RowVec<T>::n];
+    RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+    for (int e = 0; e < RowVec<T>::n; ++e)
+      if (v[e] != v[e]) s = v[e];
+  }
+  return (double)s;
 }
 
 }  // namespace pm
