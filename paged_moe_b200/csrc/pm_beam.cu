@@ -17,8 +17,8 @@
 // a thread; more go through a radix select.  A part with more keys than the
 // buffer holds (long ties, as in a constant row) takes the plain way: one
 // vector of every thread at a time against a running threshold.
-// The cluster's lists and sums meet in its first CTA through distributed
-// shared memory.
+// The cluster's CTAs put their lists and sums into the first one's shared
+// memory, which ranks them once more.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -63,18 +63,21 @@ struct TopArgs {
 struct TopShared {
   alignas(16) uint64_t buf[kTopBuf];
   uint64_t best[kTopMax];
-  ExpSum sums[kTopWarps];
-  ExpSum part;
+  double wrho[kTopWarps], wsum[kTopWarps];
+  ExpSum part[kTopSplit];
+  float top[kTopSplit];   // the parts' maxima
+  uint64_t last[kTopSplit];  // the parts' k-th keys, 0 where they have fewer
+  int parts_got[kTopSplit];
   unsigned hist[256];
   int scal[4];
   int count;              // keys in buf
   int got;                // keys in best
   int listed;
   float thr;
-  float top;              // the part's maximum
   float wmax[kTopWarps], wbound[kTopWarps];
   uint16_t list[kTopList];  // (tile of the part) * 256 + thread
-  // then [tiles of the part][256] upper halves of the tiles' ordered maxima
+  // then [tiles of the part][256] upper halves of the tiles' ordered maxima,
+  // and, where a row is split, [parts][k] keys of the parts' lists
 };
 
 // The float before x, for x > -inf.
@@ -178,16 +181,15 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // The same shared variable of CTA `rank` of the cluster.
 template <typename V>
-__device__ __forceinline__ const V* of_rank(const V* p, uint32_t rank) {
+__device__ __forceinline__ V* of_rank(V* p, uint32_t rank) {
   uint64_t out;
   asm("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
-  return reinterpret_cast<const V*>(out);
+  return reinterpret_cast<V*>(out);
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 template <typename T, bool MASKED, bool ALIGNED>
 __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs a) {
@@ -205,6 +207,7 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
     if (tid == 0 && rank == 0) a.lse64[r] = nan64();
     return;
   }
+  if (split > 1) cluster_arrive();  // waited for before the first store into another CTA
   const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
   const int off = ALIGNED ? 0 : (int)(reinterpret_cast<uintptr_t>(row) & 15);
   const uint8_t* mask = MASKED ? reinterpret_cast<const uint8_t*>(a.mask + r * a.mask_stride) : nullptr;
@@ -269,34 +272,65 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
     }
   }
 
-  // the bound: the 32 largest of the warp's 64 maxima in descending order
-  auto sorted = [&](float o) {
-#pragma unroll
-    for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        const float p = __shfl_xor_sync(kFull, o, j);
-        o = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(o, p) : fminf(o, p);
-      }
-    return o;
-  };
+  // the bound: the warp's `place`-th largest of its lanes' 64 maxima
   const float m = fmaxf(m0, m1);
-  {
+  const int place = (K + kTopWarps - 1) / kTopWarps;
+  float o;
+  if (place <= 8) {
+    // taken one by one, the first of equal lanes
+    uint32_t mine = ordkey(m);
+    const uint32_t second = ordkey(fminf(m0, m1));
+    bool first = true;
+    uint32_t most = 0;
+    for (int i = 0; i < place; ++i) {
+      most = __reduce_max_sync(kFull, mine);
+      const unsigned at_most = __ballot_sync(kFull, mine == most);
+      if (lane == __ffs(at_most) - 1) {
+        mine = first ? second : 0u;
+        first = false;
+      }
+    }
+    o = key_value((uint64_t)most << 32);
+  } else {
+    // the 32 largest in descending order
+    auto sorted = [&](float v) {
+#pragma unroll
+      for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+          const float p = __shfl_xor_sync(kFull, v, j);
+          v = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(v, p) : fminf(v, p);
+        }
+      return v;
+    };
     const float hi = sorted(m), lo = sorted(fminf(m0, m1));
-    float o = fmaxf(hi, __shfl_sync(kFull, lo, 31 - lane));
+    o = fmaxf(hi, __shfl_sync(kFull, lo, 31 - lane));
 #pragma unroll
     for (int j = 16; j > 0; j >>= 1) {
       const float p = __shfl_xor_sync(kFull, o, j);
       o = (lane & j) == 0 ? fmaxf(o, p) : fminf(o, p);
     }
-    o = __shfl_sync(kFull, o, (K + kTopWarps - 1) / kTopWarps - 1);
-    if (lane == 0) sh.wbound[warp] = o;
+    o = __shfl_sync(kFull, o, place - 1);
   }
+  // and the CTA's largest exponent and element
+  double rho = acc.rho;
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) rho = fmax(rho, __shfl_xor_sync(kFull, rho, j));
+  const float wm = warp_max(m);
+  if (lane == 0) { sh.wbound[warp] = o; sh.wrho[warp] = rho; sh.wmax[warp] = wm; }
   __syncthreads();
   float bound = sh.wbound[0];
 #pragma unroll
   for (int w = 1; w < kTopWarps; ++w) bound = fminf(bound, sh.wbound[w]);
   const float below = bound > kNegInf ? float_below(bound) : kNegInf;
+  rho = sh.wrho[0];
+#pragma unroll
+  for (int w = 1; w < kTopWarps; ++w) rho = fmax(rho, sh.wrho[w]);
+  // nothing at all: s is 0, or a NaN that stays
+  double s = acc.rho > kNegInf64 ? acc.s * pow2_down(acc.rho - rho) : acc.s;
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) s += __shfl_xor_sync(kFull, s, j);
+  if (lane == 0) sh.wsum[warp] = s;
   if (m > below) {
     // without a bound every tile that holds anything
     const uint32_t least = (ordkey(bound) >> 16) + (bound > kNegInf ? 0u : 1u);
@@ -320,67 +354,68 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
     top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTile, t1 * kTile, V, K);
 
   // the part's list, maximum and sum
-  acc = warp_join(acc);
-  const float wm = warp_max(m);
-  if (lane == 0) { sh.sums[warp] = acc; sh.wmax[warp] = wm; }
-  __syncthreads();
   if (tid == 0) {
-    ExpSum s = sh.sums[0];
+    ExpSum part = {sh.wsum[0], rho};
     float top = sh.wmax[0];
 #pragma unroll
     for (int w = 1; w < kTopWarps; ++w) {
-      s.add(sh.sums[w].s, sh.sums[w].rho);
+      part.s += sh.wsum[w];
       top = fmaxf(top, sh.wmax[w]);
     }
-    sh.part = s;
-    sh.top = top;
+    sh.part[0] = part;
+    sh.top[0] = top;
   }
   const int cnt = sh.count;
   __syncthreads();
   top_cut(sh, cnt, K);
 
   if (split > 1) {
-    cluster_sync();
-    if (rank == 0) {
-      // a full list's last key bounds the row's k-th from below
-      uint64_t least = 0;
-      for (uint32_t c = 0; c < split; ++c)
-        if (*of_rank(&sh.got, c) == K) {
-          const uint64_t last = *of_rank(&sh.best[K - 1], c);
-          least = last > least ? last : least;
-        }
-      if (tid == 0) {
-        ExpSum s = sh.part;
-        float top = sh.top;
-        for (uint32_t c = 1; c < split; ++c) {
-          const ExpSum* p = of_rank(&sh.part, c);
-          s.add(p->s, p->rho);
-          top = fmaxf(top, *of_rank(&sh.top, c));
-        }
-        sh.part = s;
-        sh.top = top;
-        sh.count = 0;
+    uint64_t* keys = reinterpret_cast<uint64_t*>(tops + per * kTopThreads);
+    cluster_wait();  // every CTA of the cluster runs
+    const int mine = sh.got;
+    for (int i = tid; i < mine; i += kTopThreads) *of_rank(&keys[rank * K + i], 0) = sh.best[i];
+    if (tid == 0) {
+      if (rank > 0) {
+        *of_rank(&sh.part[rank], 0) = sh.part[0];
+        *of_rank(&sh.top[rank], 0) = sh.top[0];
       }
-      __syncthreads();
-      for (int i = tid; i < K * (int)split; i += kTopThreads) {
-        const uint32_t c = (uint32_t)(i / K);
-        const int j = i % K;
-        if (j < *of_rank(&sh.got, c)) {
-          const uint64_t key = *of_rank(&sh.best[j], c);
-          if (key >= least) sh.buf[atomicAdd(&sh.count, 1)] = key;
-        }
-      }
-      __syncthreads();
-      const int all = sh.count;
-      __syncthreads();
-      top_cut(sh, all, K);
+      *of_rank(&sh.parts_got[rank], 0) = mine;
+      *of_rank(&sh.last[rank], 0) = mine == K ? sh.best[K - 1] : 0ull;
     }
-    cluster_sync();  // the others' shared memory lives until the first CTA has read it
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
     if (rank != 0) return;
+    // a full list's last key bounds the row's k-th from below
+    uint64_t least = 0;
+    for (uint32_t c = 0; c < split; ++c) least = sh.last[c] > least ? sh.last[c] : least;
+    if (tid == 0) {
+      ExpSum part = sh.part[0];
+      float top = sh.top[0];
+      for (uint32_t c = 1; c < split; ++c) {
+        part.add(sh.part[c].s, sh.part[c].rho);
+        top = fmaxf(top, sh.top[c]);
+      }
+      sh.part[0] = part;
+      sh.top[0] = top;
+      sh.count = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < K * (int)split; i += kTopThreads) {
+      const int c = i / K;
+      if (i - c * K < sh.parts_got[c]) {
+        const uint64_t key = keys[i];
+        if (key >= least) sh.buf[atomicAdd(&sh.count, 1)] = key;
+      }
+    }
+    __syncthreads();
+    const int all = sh.count;
+    __syncthreads();
+    top_cut(sh, all, K);
   }
 
-  const ExpSum sum = sh.part;
-  const float M = sh.top;
+  const ExpSum sum = sh.part[0];
+  const float M = sh.top[0];
   const bool bad = !(sum.s == sum.s) || M == -kNegInf;
   const double lse = bad ? nan64() : M > kNegInf ? scale.log_of(sum, M) : kNegInf64;
   const int got = bad ? 0 : sh.got;
@@ -589,9 +624,13 @@ cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
   static pmh::DeviceOnce once;
   cudaError_t e = cudaSuccess;
   constexpr int64_t kTile = (int64_t)pm::kTopThreads * pm::kTopU * pm::RowVec<T>::n;
-  auto bytes = [](int64_t tiles) { return sizeof(pm::TopShared) + (size_t)tiles * pm::kTopThreads * 2; };
+  // a part's maxima, and the parts' lists of a row that is split
+  auto bytes = [](int64_t tiles, int split, int k) {
+    return sizeof(pm::TopShared) + (size_t)tiles * pm::kTopThreads * 2 + (split > 1 ? (size_t)split * k * 8 : 0);
+  };
   once([&] {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kMaxVocab / kTile));
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)bytes(kMaxVocab / kTile, pm::kTopSplit, pm::kTopMax));
   });
   if (e != cudaSuccess) return e;
   const int64_t tiles = (a.vocab + kTile - 1) / kTile;
@@ -599,7 +638,7 @@ cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * split));
   cfg.blockDim = dim3(pm::kTopThreads);
-  cfg.dynamicSmemBytes = bytes((tiles + split - 1) / split);
+  cfg.dynamicSmemBytes = bytes((tiles + split - 1) / split, split, a.k);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
