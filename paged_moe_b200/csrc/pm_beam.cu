@@ -14,7 +14,7 @@
 // it are read once more, about 1.2 k to 2 k of them, and only elements that
 // reach it become keys, (ordered logit bits, ~id): larger logits first, then
 // lower ids, all keys different.  Up to 256 keys are ranked by counting, one
-// a thread; more go through a radix select.  A part with more keys than the
+// a thread; more are sorted.  A part with more keys than the
 // buffer holds (long ties, as in a constant row) takes the plain way: one
 // vector of every thread at a time against a running threshold.
 // The cluster's CTAs put their lists and sums into the first one's shared
@@ -41,6 +41,7 @@ constexpr int kTopSplit = 8;      // most CTAs of a row (a portable cluster)
 constexpr int kTopBuf = 2560;     // keys: 2 x the largest k, and one vector of every thread
 constexpr int kTopList = 2048;    // threads' tiles that are read once more
 constexpr int kTopFew = 256;      // keys that are ranked by counting, one a thread
+constexpr int kTopSort = 2048;    // keys that are sorted
 
 struct TopArgs {
   const void* logits;
@@ -66,7 +67,6 @@ struct TopShared {
   double wrho[kTopWarps], wsum[kTopWarps];
   ExpSum part[kTopSplit];
   float top[kTopSplit];   // the parts' maxima
-  uint64_t last[kTopSplit];  // the parts' k-th keys, 0 where they have fewer
   int parts_got[kTopSplit];
   unsigned hist[256];
   int scal[4];
@@ -87,6 +87,27 @@ __device__ __forceinline__ float float_below(float x) {
   return key_value((uint64_t)o << 32);
 }
 
+// Sorts buf[0, cnt) in descending order, cnt <= kTopSort: a bitonic network over
+// the next power of two.  Pairs at most 32 apart lie in 64 keys of one warp,
+// so that only the wider steps need the CTA's barrier.
+__device__ __forceinline__ void top_sort(uint64_t* buf, int cnt) {
+  const int tid = threadIdx.x;
+  int P = 64;
+  while (P < cnt) P <<= 1;
+  for (int i = cnt + tid; i < P; i += kTopThreads) buf[i] = 0ull;
+  __syncthreads();
+  for (int k = 2; k <= P; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int p = tid; p < P / 2; p += kTopThreads) {
+        const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1));
+        const uint64_t a = buf[i], b = buf[i + j];
+        if ((i & k) == 0 ? a < b : a > b) { buf[i] = b; buf[i + j] = a; }
+      }
+      if (j > 32 || (j == 1 && k >= 64)) __syncthreads(); else __syncwarp();
+    }
+  }
+}
+
 // Cuts buf[0, cnt) to its K largest, sorted, in buf and best; sets count, got
 // and the threshold.  Every thread, between barriers.
 __device__ __forceinline__ void top_cut(TopShared& sh, int cnt, int K) {
@@ -97,6 +118,7 @@ __device__ __forceinline__ void top_cut(TopShared& sh, int cnt, int K) {
     int rank = 0;
     if (tid < cnt) {
       int j = 0;
+#pragma unroll 8
       for (; j + 1 < cnt; j += 2) {
         const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.buf[j]);
         rank += (o.x > key) + (o.y > key);
@@ -112,6 +134,14 @@ __device__ __forceinline__ void top_cut(TopShared& sh, int cnt, int K) {
     if (tid == 0) {
       sh.count = sh.got = cnt < K ? cnt : K;
       if (cnt < K) sh.thr = kNegInf;
+    }
+  } else if (cnt <= kTopSort) {
+    top_sort(sh.buf, cnt);
+    const int got = cnt < K ? cnt : K;
+    if (tid < got) sh.best[tid] = sh.buf[tid];
+    if (tid == 0) {
+      sh.count = sh.got = got;
+      sh.thr = got == K ? key_value(sh.buf[K - 1]) : kNegInf;
     }
   } else {
     const int got = block_topk_sorted(sh.buf, cnt, K, sh.best, kTopMax, sh.hist, sh.scal);
@@ -129,11 +159,16 @@ template <typename T>
 __device__ __forceinline__ void top_offer(TopShared& sh, uint4 raw, uint32_t first, float thr) {
   float v[RowVec<T>::n];
   RowVec<T>::unpack(raw, v);
+  uint32_t hits = 0;
+#pragma unroll
+  for (int e = 0; e < RowVec<T>::n; ++e) hits |= v[e] > thr ? 1u << e : 0u;
+  if (hits == 0) return;
+  int pos = atomicAdd(&sh.count, __popc(hits));
 #pragma unroll
   for (int e = 0; e < RowVec<T>::n; ++e)
-    if (v[e] > thr) {
-      const int pos = atomicAdd(&sh.count, 1);
+    if ((hits >> e) & 1) {
       if (pos < kTopBuf) sh.buf[pos] = rankkey(v[e], first + e);
+      ++pos;
     }
 }
 
@@ -238,11 +273,10 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
       if (MASKED) raw[u] = RowVec<T>::select(raw[u], bits[u]);
       vm[u] = RowVec<T>::largest(raw[u]);
     }
-    const float tm = fmaxf(max3(vm[0], vm[1], vm[2]), vm[3]);
+    const float tm = max_nan(max_nan(vm[0], vm[1]), vm[2], vm[3]);
     tops[(t - t0) * kTopThreads + tid] = (uint16_t)(ordkey(tm) >> 16);
     m = fmaxf(m, tm);
-    if (tm > kNegInf) add_exps<T, kTopU>(acc, raw, tm, scale);
-    else acc.add(nan_of<T, kTopU>(raw), kNegInf64);
+    add_exps<T, kTopU>(acc, raw, tm, scale);
   };
 
   if (tid == 0) { sh.count = 0; sh.got = 0; sh.listed = 0; sh.thr = kNegInf; }
@@ -250,9 +284,8 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
   {
     uint4 even[kTopU], odd[kTopU];
     uint32_t be[kTopU] = {}, bo[kTopU] = {};
-    if (MASKED) load_bits(t0, be);
+    if (MASKED) { load_bits(t0, be); load_bits(t0 + 1, bo); }
     load_tile(t0, be, even);
-    if (MASKED) load_bits(t0 + 1, bo);
     for (int t = t0; t < t1; t += 2) {
       uint32_t bn[kTopU] = {};
       load_tile(t + 1, bo, odd);
@@ -312,25 +345,15 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
     }
     o = __shfl_sync(kFull, o, place - 1);
   }
-  // and the CTA's largest exponent and element
-  double rho = acc.rho;
-#pragma unroll
-  for (int j = 16; j > 0; j >>= 1) rho = fmax(rho, __shfl_xor_sync(kFull, rho, j));
-  const float wm = warp_max(m);
-  if (lane == 0) { sh.wbound[warp] = o; sh.wrho[warp] = rho; sh.wmax[warp] = wm; }
+  // and the largest exponent and element
+  const double wrho = warp_max64(acc.rho);
+  const float wm = warp_max_ordered(m);
+  if (lane == 0) { sh.wbound[warp] = o; sh.wrho[warp] = wrho; sh.wmax[warp] = wm; }
   __syncthreads();
   float bound = sh.wbound[0];
 #pragma unroll
   for (int w = 1; w < kTopWarps; ++w) bound = fminf(bound, sh.wbound[w]);
   const float below = bound > kNegInf ? float_below(bound) : kNegInf;
-  rho = sh.wrho[0];
-#pragma unroll
-  for (int w = 1; w < kTopWarps; ++w) rho = fmax(rho, sh.wrho[w]);
-  // nothing at all: s is 0, or a NaN that stays
-  double s = acc.rho > kNegInf64 ? acc.s * pow2_down(acc.rho - rho) : acc.s;
-#pragma unroll
-  for (int j = 16; j > 0; j >>= 1) s += __shfl_xor_sync(kFull, s, j);
-  if (lane == 0) sh.wsum[warp] = s;
   if (m > below) {
     // without a bound every tile that holds anything
     const uint32_t least = (ordkey(bound) >> 16) + (bound > kNegInf ? 0u : 1u);
@@ -349,6 +372,9 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
       top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), (uint32_t)i, below);
     }
   }
+  const double rho = warp_max64(sh.wrho[lane % kTopWarps]);
+  const double s = warp_sum64(scaled_to(acc, rho));
+  if (lane == 0) sh.wsum[warp] = s;
   __syncthreads();
   if (listed > kTopList || sh.count > kTopBuf)
     top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTile, t1 * kTile, V, K);
@@ -380,38 +406,47 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
         *of_rank(&sh.top[rank], 0) = sh.top[0];
       }
       *of_rank(&sh.parts_got[rank], 0) = mine;
-      *of_rank(&sh.last[rank], 0) = mine == K ? sh.best[K - 1] : 0ull;
     }
     __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    // a full list's last key bounds the row's k-th from below
-    uint64_t least = 0;
-    for (uint32_t c = 0; c < split; ++c) least = sh.last[c] > least ? sh.last[c] : least;
-    if (tid == 0) {
-      ExpSum part = sh.part[0];
-      float top = sh.top[0];
-      for (uint32_t c = 1; c < split; ++c) {
-        part.add(sh.part[c].s, sh.part[c].rho);
-        top = fmaxf(top, sh.top[c]);
+    if (warp == kTopWarps - 1) {
+      const bool on = lane < (int)split;
+      ExpSum part = {0.0, kNegInf64};
+      if (on) part = sh.part[lane];
+      const double to = warp_max64(part.rho);
+      part.s = warp_sum64(scaled_to(part, to));
+      const float top = warp_max_ordered(on ? sh.top[lane] : kNegInf);
+      const int got = (int)__reduce_add_sync(kFull, on ? (unsigned)sh.parts_got[lane] : 0u);
+      if (lane == 0) {
+        part.rho = to;
+        sh.part[0] = part;
+        sh.top[0] = top;
+        sh.got = got < K ? got : K;
       }
-      sh.part[0] = part;
-      sh.top[0] = top;
-      sh.count = 0;
     }
-    __syncthreads();
+    // a key's place in the row: its place in its own list, and the number of
+    // larger keys in each of the others, all searched at once
+    int half = 1;
+    while (half * 2 <= K) half *= 2;
     for (int i = tid; i < K * (int)split; i += kTopThreads) {
       const int c = i / K;
-      if (i - c * K < sh.parts_got[c]) {
-        const uint64_t key = keys[i];
-        if (key >= least) sh.buf[atomicAdd(&sh.count, 1)] = key;
-      }
+      int place = i - c * K;
+      if (place >= sh.parts_got[c]) continue;
+      const uint64_t key = keys[i];
+      int at[kTopSplit] = {};
+      for (int step = half; step > 0; step >>= 1)
+#pragma unroll
+        for (int d = 0; d < kTopSplit; ++d) {
+          const int to = at[d] + step;
+          if (d < (int)split && to <= sh.parts_got[d] && keys[d * K + to - 1] > key) at[d] = to;
+        }
+#pragma unroll
+      for (int d = 0; d < kTopSplit; ++d) place += d != c ? at[d] : 0;
+      if (place < K) sh.best[place] = key;
     }
     __syncthreads();
-    const int all = sh.count;
-    __syncthreads();
-    top_cut(sh, all, K);
   }
 
   const ExpSum sum = sh.part[0];

@@ -28,9 +28,15 @@ constexpr float kWildExponent = 1048576.0f;
 
 __device__ __forceinline__ double nan64() { return __longlong_as_double(0x7ff8000000000000ll); }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// Maxima that are NaN where an operand is.
+__device__ __forceinline__ float max_nan(float a, float b) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -42,8 +48,9 @@ template <> struct RowVec<float> {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
   }
   static __device__ __forceinline__ float get(const float* p) { return *p; }
+  // NaN if the vector holds one
   static __device__ __forceinline__ float largest(uint4 r) {
-    return max3(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), __uint_as_float(r.z), __uint_as_float(r.w));
+    return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)), __uint_as_float(r.z), __uint_as_float(r.w));
   }
   // the vector with -inf where bit e of `bits` is clear
   static __device__ __forceinline__ uint4 select(uint4 r, uint32_t bits) {
@@ -66,8 +73,8 @@ template <> struct RowVec<__nv_bfloat16> {
   static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
   static __device__ __forceinline__ float largest(uint4 r) {
-    const __nv_bfloat162 m = __hmax2(__hmax2(pair(r.x), pair(r.y)), __hmax2(pair(r.z), pair(r.w)));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(pair(r.x), pair(r.y)), __hmax2_nan(pair(r.z), pair(r.w)));
+    return max_nan(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ uint32_t keep(uint32_t w, uint32_t bits) {
     // one byte per half word: 0xff where the bit is set
@@ -121,12 +128,14 @@ __device__ __forceinline__ uint4 load_raw(const T* row, int off, int i, int V) {
   return r;
 }
 
-// 2^d for d <= 0: exact for whole numbers.
+static __device__ __noinline__ double exp2_apart(double d) { return exp2(d); }
+
+// 2^d for d <= 0: exact for whole numbers, which all but wild rows have.
 __device__ __forceinline__ double pow2_down(double d) {
   if (d < -1000.0) return 0.0;
-  const double w = rint(d);
-  if (w == d) return __hiloint2double((1023 + (int)d) << 20, 0);
-  return exp2(d);
+  const int w = (int)d;
+  if ((double)w == d) return __hiloint2double((1023 + w) << 20, 0);
+  return exp2_apart(d);
 }
 
 // A running sum s 2^rho.
@@ -146,19 +155,29 @@ struct ExpSum {
   }
 };
 
-__device__ __forceinline__ ExpSum warp_join(ExpSum a) {
+// Largest of the warp's values, none of them NaN.
+__device__ __forceinline__ double warp_max64(double v) {
+  const long long b = __double_as_longlong(v);
+  const uint64_t key = b < 0 ? ~(uint64_t)b : (uint64_t)b | 0x8000000000000000ull;
+  const uint32_t hi = __reduce_max_sync(kFull, (uint32_t)(key >> 32));
+  const uint32_t lo = __reduce_max_sync(kFull, hi == (uint32_t)(key >> 32) ? (uint32_t)key : 0u);
+  const uint64_t most = (uint64_t)hi << 32 | lo;
+  return __longlong_as_double((long long)(most >> 63 ? most & 0x7fffffffffffffffull : ~most));
+}
+
+// s 2^rho as a multiple of 2^to, to >= rho: 0 for nothing, or the NaN it holds.
+__device__ __forceinline__ double scaled_to(const ExpSum& a, double to) {
+  return a.rho > kNegInf64 ? a.s * pow2_down(a.rho - to) : a.s;
+}
+
+__device__ __forceinline__ float warp_max_ordered(float v) {
+  return key_value((uint64_t)__reduce_max_sync(kFull, ordkey(v)) << 32);
+}
+
+__device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double t = __shfl_xor_sync(kFull, a.s, o), r = __shfl_xor_sync(kFull, a.rho, o);
-    // the same two numbers in the same order on both lanes
-    ExpSum b;
-    const bool low = (threadIdx.x & o) == 0;
-    b.s = low ? a.s : t;
-    b.rho = low ? a.rho : r;
-    b.add(low ? t : a.s, low ? r : a.rho);
-    a = b;
-  }
-  return a;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
 }
 
 // Constants of a row's exponentials.
@@ -173,12 +192,24 @@ struct ExpScale {
   }
 };
 
-// Adds the 2^(x c) of U vectors whose largest element is tm > -inf.
+template <typename T>
+__device__ __noinline__ float wild_exps(uint4 raw, float tm, float c) {
+  float v[RowVec<T>::n], sum = 0.0f;
+  RowVec<T>::unpack(raw, v);
+#pragma unroll
+  for (int e = 0; e < RowVec<T>::n; ++e) sum += ex2_approx((v[e] - tm) * c);
+  return sum;
+}
+
+// Adds the 2^(x c) of U vectors whose largest element is tm (NaN: one of
+// them holds a NaN).
 template <typename T, int U>
 __device__ __forceinline__ void add_exps(ExpSum& acc, const uint4 (&raw)[U], float tm, const ExpScale& k) {
   constexpr int n = RowVec<T>::n;
   const float top = tm * k.c;
-  if (fabsf(top) < kWildExponent) {
+  if (!(tm > kNegInf)) {
+    acc.add(tm == kNegInf ? 0.0 : nan64(), kNegInf64);
+  } else if (fabsf(top) < kWildExponent) {
     const float R = rintf(top);
     const uint64_t c2 = pk(k.c, k.c), r2 = pk(-R, -R);
     uint64_t sum0 = 0, sum1 = 0;
@@ -198,30 +229,9 @@ __device__ __forceinline__ void add_exps(ExpSum& acc, const uint4 (&raw)[U], flo
   } else {
     float sum = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[n];
-      RowVec<T>::unpack(raw[u], v);
-#pragma unroll
-      for (int e = 0; e < n; ++e) sum += ex2_approx((v[e] - tm) * k.c);
-    }
+    for (int u = 0; u < U; ++u) sum += wild_exps<T>(raw[u], tm, k.c);
     acc.add((double)sum, (double)tm * k.exact);
   }
-}
-
-// NaN if one of the vectors holds a NaN, else 0 (for vectors without a
-// largest element).
-template <typename T, int U>
-__device__ __forceinline__ double nan_of(const uint4 (&raw)[U]) {
-  float s = 0.0f;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float v[RowVec<T>::n];
-    RowVec<T>::unpack(raw[u], v);
-#pragma unroll
-    for (int e = 0; e < RowVec<T>::n; ++e)
-      if (v[e] != v[e]) s = v[e];
-  }
-  return (double)s;
 }
 
 }  // namespace pm
