@@ -2,23 +2,27 @@
 // beam search over them.
 //
 // k_top_rows: a row is streamed once, by one CTA or, where there are few
-// rows, by a cluster of up to eight that take consecutive parts of it.  Tiles
-// of 256 threads x four 16-byte vectors are loaded one ahead of the one in
-// work.  The loop only adds exponentials and takes maxima: a thread keeps the
-// largest element of its even and of its odd tiles, and the upper 16 bits of
-// each tile's largest go to shared memory.  There is no barrier in it.
+// rows, by a cluster of up to eight that take consecutive parts of it.  Every
+// warp streams its own chunks (32 lanes x U 16-byte vectors) through a ring in
+// shared memory that its first lane keeps full with bulk copies; there is no
+// barrier in the loop.  It only adds exponentials and takes maxima: a thread
+// keeps the largest element of its even and of its odd tiles, and the upper
+// 16 bits of each tile's largest go to shared memory.
 //
-// The k largest are looked for afterwards.  Each warp sorts its lanes' 64
-// maxima; the least of the eight warps' ceil(k/8)-th largest is a bound that
-// at least k elements reach.  Only the threads' tiles whose maximum reaches
-// it are read once more, about 1.2 k to 2 k of them, and only elements that
+// The k largest are looked for afterwards.  From each warp's 64 maxima the
+// ceil(k/8)-th largest is taken; the least of the eight is a bound that at
+// least k elements reach.  Only the threads' tiles whose maximum reaches it
+// are read once more, about 1.2 k to 2 k of them, and only elements that
 // reach it become keys, (ordered logit bits, ~id): larger logits first, then
 // lower ids, all keys different.  Up to 256 keys are ranked by counting, one
-// a thread; more are sorted.  A part with more keys than the
-// buffer holds (long ties, as in a constant row) takes the plain way: one
-// vector of every thread at a time against a running threshold.
+// a thread; more are sorted.  A part with more keys than the buffer holds
+// (long ties, as in a constant row) takes the plain way: one vector of every
+// thread at a time against a running threshold.
 // The cluster's CTAs put their lists and sums into the first one's shared
 // memory, which ranks them once more.
+//
+// Every wait on a copy is bounded; a row whose copy does not arrive gives
+// NaN and ids -1.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -29,13 +33,12 @@
 #include "pm_host.h"
 #include "pm_rowvec.cuh"
 #include "pm_select.cuh"
+#include "pm_tma.cuh"
 
 namespace pm {
 
 constexpr int kTopThreads = 256;
 constexpr int kTopWarps = kTopThreads / 32;
-constexpr int kTopU = 4;          // vectors of a thread in a tile
-constexpr int kTopResident = 4;   // CTAs of an SM
 constexpr int kTopMax = 256;      // largest k
 constexpr int kTopSplit = 8;      // most CTAs of a row (a portable cluster)
 constexpr int kTopBuf = 2560;     // keys: 2 x the largest k, and one vector of every thread
@@ -61,8 +64,16 @@ struct TopArgs {
   double* lse64;     // [rows] or NULL; NaN: the row offers nothing
 };
 
+// A step is four vectors of every lane, 2 KB of a warp's chunk and one stage
+// of its ring; a tile is 8,192 elements in either type, two steps of fp32 or
+// one of bf16.
+constexpr int kTopTile = 8192;
+constexpr int kTopStep = 4;
+constexpr int kTopStages = 2;
+constexpr int kTopStageBytes = kTopStep * 512 + 16;  // 16 more for rows off a 16-byte boundary
+
 struct TopShared {
-  alignas(16) uint64_t buf[kTopBuf];
+  uint64_t bar[kTopWarps][kTopStages];
   uint64_t best[kTopMax];
   double wrho[kTopWarps], wsum[kTopWarps];
   ExpSum part[kTopSplit];
@@ -75,10 +86,19 @@ struct TopShared {
   int listed;
   float thr;
   float wmax[kTopWarps], wbound[kTopWarps];
-  uint16_t list[kTopList];  // (tile of the part) * 256 + thread
-  // then [tiles of the part][256] upper halves of the tiles' ordered maxima,
-  // and, where a row is split, [parts][k] keys of the parts' lists
+  // Then, in dynamic shared memory,
+  //   the rings, and in their place once they are drained
+  //     buf[kTopBuf] keys and list[kTopList], (tile of the part) * 256 + thread;
+  //   [tiles of the part][256] upper halves of the tiles' ordered maxima;
+  //   where a row is split, [parts][k] keys of the parts' lists.
+  __device__ __forceinline__ unsigned char* rings() { return reinterpret_cast<unsigned char*>(this + 1); }
+  __device__ __forceinline__ uint64_t* buf() { return reinterpret_cast<uint64_t*>(this + 1); }
+  __device__ __forceinline__ uint16_t* list() { return reinterpret_cast<uint16_t*>(buf() + kTopBuf); }
 };
+static_assert(sizeof(TopShared) % 16 == 0, "the rings are 16-byte aligned");
+
+constexpr int kTopRingBytes = kTopWarps * kTopStages * kTopStageBytes;
+static_assert(kTopRingBytes >= kTopBuf * 8 + kTopList * 2 && kTopRingBytes % 16 == 0, "the keys fit in the rings' place");
 
 // The float before x, for x > -inf.
 __device__ __forceinline__ float float_below(float x) {
@@ -114,20 +134,20 @@ __device__ __forceinline__ void top_cut(TopShared& sh, int cnt, int K) {
   const int tid = threadIdx.x;
   if (cnt <= kTopFew) {
     // one key a thread: its rank is the number of larger keys
-    const uint64_t key = tid < cnt ? sh.buf[tid] : 0ull;
+    const uint64_t key = tid < cnt ? sh.buf()[tid] : 0ull;
     int rank = 0;
     if (tid < cnt) {
       int j = 0;
 #pragma unroll 8
       for (; j + 1 < cnt; j += 2) {
-        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.buf[j]);
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.buf()[j]);
         rank += (o.x > key) + (o.y > key);
       }
-      if (j < cnt) rank += sh.buf[j] > key;
+      if (j < cnt) rank += sh.buf()[j] > key;
     }
     __syncthreads();
     if (tid < cnt && rank < K) {
-      sh.buf[rank] = key;
+      sh.buf()[rank] = key;
       sh.best[rank] = key;
       if (rank == K - 1) sh.thr = key_value(key);
     }
@@ -136,16 +156,16 @@ __device__ __forceinline__ void top_cut(TopShared& sh, int cnt, int K) {
       if (cnt < K) sh.thr = kNegInf;
     }
   } else if (cnt <= kTopSort) {
-    top_sort(sh.buf, cnt);
+    top_sort(sh.buf(), cnt);
     const int got = cnt < K ? cnt : K;
-    if (tid < got) sh.best[tid] = sh.buf[tid];
+    if (tid < got) sh.best[tid] = sh.buf()[tid];
     if (tid == 0) {
       sh.count = sh.got = got;
-      sh.thr = got == K ? key_value(sh.buf[K - 1]) : kNegInf;
+      sh.thr = got == K ? key_value(sh.buf()[K - 1]) : kNegInf;
     }
   } else {
-    const int got = block_topk_sorted(sh.buf, cnt, K, sh.best, kTopMax, sh.hist, sh.scal);
-    for (int i = tid; i < got; i += kTopThreads) sh.buf[i] = sh.best[i];
+    const int got = block_topk_sorted(sh.buf(), cnt, K, sh.best, kTopMax, sh.hist, sh.scal);
+    for (int i = tid; i < got; i += kTopThreads) sh.buf()[i] = sh.best[i];
     if (tid == 0) {
       sh.count = sh.got = got;
       sh.thr = got == K ? key_value(sh.best[K - 1]) : kNegInf;
@@ -167,7 +187,7 @@ __device__ __forceinline__ void top_offer(TopShared& sh, uint4 raw, uint32_t fir
 #pragma unroll
   for (int e = 0; e < RowVec<T>::n; ++e)
     if ((hits >> e) & 1) {
-      if (pos < kTopBuf) sh.buf[pos] = rankkey(v[e], first + e);
+      if (pos < kTopBuf) sh.buf()[pos] = rankkey(v[e], first + e);
       ++pos;
     }
 }
@@ -226,17 +246,58 @@ __device__ __forceinline__ V* of_rank(V* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// The place-th largest of the warp's 64 values a, b; -inf if place > 64.
+__device__ __forceinline__ float warp_place(float a, float b, int place) {
+  const int lane = threadIdx.x & 31;
+  if (place > 64) return kNegInf;
+  const float first = fmaxf(a, b), second = fminf(a, b);
+  if (place <= 8 || place > 32) {
+    // taken one by one, the first of equal lanes
+    uint32_t mine = ordkey(first), later = ordkey(second), most = 0;
+    for (int i = 0; i < place; ++i) {
+      most = __reduce_max_sync(kFull, mine);
+      if (lane == __ffs(__ballot_sync(kFull, mine == most)) - 1) {
+        mine = later;
+        later = 0;
+      }
+    }
+    return key_value((uint64_t)most << 32);
+  }
+  // the 32 largest in descending order
+  auto sorted = [&](float v) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        const float p = __shfl_xor_sync(kFull, v, j);
+        v = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(v, p) : fminf(v, p);
+      }
+    return v;
+  };
+  const float hi = sorted(first), lo = sorted(second);
+  float o = fmaxf(hi, __shfl_sync(kFull, lo, 31 - lane));
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) {
+    const float p = __shfl_xor_sync(kFull, o, j);
+    o = (lane & j) == 0 ? fmaxf(o, p) : fminf(o, p);
+  }
+  return __shfl_sync(kFull, o, place - 1);
+}
+
 template <typename T, bool MASKED, bool ALIGNED>
-__global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs a) {
+__global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   TopShared& sh = *reinterpret_cast<TopShared*>(shared_bytes);
   constexpr int n = RowVec<T>::n;
-  constexpr int kTile = kTopThreads * kTopU * n;
+  constexpr int kChunk = kTopTile / kTopWarps;   // a warp's elements of a tile
+  constexpr int kStepElems = 32 * kTopStep * n;
+  constexpr int kSteps = kChunk / kStepElems;    // of a tile
+  constexpr int U = kSteps * kTopStep, S = kTopStages;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank(), split = cluster_size();
   const int64_t r = blockIdx.x / split;
   const int K = a.k, V = (int)a.vocab;
-  uint16_t* tops = reinterpret_cast<uint16_t*>(&sh + 1);
+  uint16_t* tops = reinterpret_cast<uint16_t*>(sh.rings() + kTopRingBytes);
   // the whole cluster leaves here or none of it
   if (a.scores && (!(a.scores[r] > kNegInf) || (a.done && a.done[r]))) {
     if (tid == 0 && rank == 0) a.lse64[r] = nan64();
@@ -248,111 +309,127 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
   const uint8_t* mask = MASKED ? reinterpret_cast<const uint8_t*>(a.mask + r * a.mask_stride) : nullptr;
   const ExpScale scale(a.inv_t);
 
-  const int tiles = (V + kTile - 1) / kTile;
+  const int tiles = (V + kTopTile - 1) / kTopTile;
   const int per = (tiles + (int)split - 1) / (int)split;
   const int t0 = (int)rank * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  // element u of thread g in tile t
+  auto at = [&](int t, int u, int g) { return t * kTopTile + (g >> 5) * kChunk + (u * 32 + (g & 31)) * n; };
 
-  auto at = [&](int t, int u) { return t * kTile + (u * kTopThreads + tid) * n; };
-  auto load_bits = [&](int t, uint32_t (&bits)[kTopU]) {
-#pragma unroll
-    for (int u = 0; u < kTopU; ++u) bits[u] = t < t1 ? top_bits<T>(mask, at(t, u), V) : 0u;
+  // the warp's ring
+  unsigned char* ring = sh.rings() + warp * S * kTopStageBytes;
+  uint64_t* bar = sh.bar[warp];
+  const uint64_t policy = policy_evict_first();
+  auto issue = [&](int q, int st) {  // step q counts from t0
+    const int first = (t0 + q / kSteps) * kTopTile + warp * kChunk + q % kSteps * kStepElems;
+    if (q >= (t1 - t0) * kSteps || first >= V) return;
+    const char* src = reinterpret_cast<const char*>(row + first) - off;
+    // up to the 16-byte boundary at or behind the row's end
+    const int64_t left = (reinterpret_cast<const char*>(row + V) - src + 15) & ~(int64_t)15;
+    constexpr int most = ALIGNED ? kTopStep * 512 : kTopStep * 512 + 16;
+    const uint32_t bytes = left < most ? (uint32_t)left : (uint32_t)most;
+    mbar_arrive_expect_tx(&bar[st], bytes);
+    bulk_copy_g2s(ring + st * kTopStageBytes, src, bytes, &bar[st], policy);
   };
-  auto load_tile = [&](int t, const uint32_t (&bits)[kTopU], uint4 (&raw)[kTopU]) {
-    constexpr uint32_t fill = RowVec<T>::kFill;
+  if (lane == 0) {
 #pragma unroll
-    for (int u = 0; u < kTopU; ++u)
-      raw[u] = t < t1 && (!MASKED || bits[u]) ? load_raw<T, ALIGNED>(row, off, at(t, u), V)
-                                              : make_uint4(fill, fill, fill, fill);
+    for (int st = 0; st < S; ++st) mbar_init(&bar[st], 1);
+    fence_proxy_async_smem();
+#pragma unroll
+    for (int st = 0; st < S; ++st) issue(st, st);
+  }
+  if (tid == 0) { sh.count = 0; sh.got = 0; sh.listed = 0; sh.thr = kNegInf; }
+  // the allowed bits of the thread's U vectors, 32 in all
+  auto load_bits = [&](int t) {
+    uint32_t b = 0;
+    if (MASKED && t < t1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) b |= top_bits<T>(mask, at(t, u, tid), V) << (u * n);
+    }
+    return b;
   };
+  uint32_t bits = load_bits(t0);
+  __syncwarp();
+
   ExpSum acc;
   acc.clear();
-  auto work = [&](int t, uint4 (&raw)[kTopU], const uint32_t (&bits)[kTopU], float& m) {
-    float vm[kTopU];
+  float m0 = kNegInf, m1 = kNegInf;  // of every second tile each
+  int st = 0, q = 0;
+  uint32_t parity = 0;
+  bool arrived = true;
+  for (int t = t0; t < t1 && arrived; ++t) {
+    const uint32_t next_bits = load_bits(t + 1);
+    float tile_max = kNegInf;
 #pragma unroll
-    for (int u = 0; u < kTopU; ++u) {
-      if (MASKED) raw[u] = RowVec<T>::select(raw[u], bits[u]);
-      vm[u] = RowVec<T>::largest(raw[u]);
-    }
-    const float tm = max_nan(max_nan(vm[0], vm[1]), vm[2], vm[3]);
-    tops[(t - t0) * kTopThreads + tid] = (uint16_t)(ordkey(tm) >> 16);
-    m = fmaxf(m, tm);
-    add_exps<T, kTopU>(acc, raw, tm, scale);
-  };
-
-  if (tid == 0) { sh.count = 0; sh.got = 0; sh.listed = 0; sh.thr = kNegInf; }
-  float m0 = kNegInf, m1 = kNegInf;  // of the even and the odd tiles
-  {
-    uint4 even[kTopU], odd[kTopU];
-    uint32_t be[kTopU] = {}, bo[kTopU] = {};
-    if (MASKED) { load_bits(t0, be); load_bits(t0 + 1, bo); }
-    load_tile(t0, be, even);
-    for (int t = t0; t < t1; t += 2) {
-      uint32_t bn[kTopU] = {};
-      load_tile(t + 1, bo, odd);
-      if (MASKED) load_bits(t + 2, bn);
-      work(t, even, be, m0);
-      load_tile(t + 2, bn, even);
-      if (MASKED) {
+    for (int h = 0; h < kSteps; ++h, ++q) {
+      const int first = t * kTopTile + warp * kChunk + h * kStepElems;
+      if (first < V && arrived) {
+        arrived = __all_sync(kFull, mbar_wait(&bar[st], parity));
+        const unsigned char* from = ring + st * kTopStageBytes + lane * 16;
+        uint4 raw[kTopStep];
 #pragma unroll
-        for (int u = 0; u < kTopU; ++u) be[u] = bn[u];
-        load_bits(t + 3, bn);
+        for (int u = 0; u < kTopStep; ++u) {
+          raw[u] = *reinterpret_cast<const uint4*>(from + u * 512);
+          if (!ALIGNED) raw[u] = shift_raw<T>(raw[u], *reinterpret_cast<const uint4*>(from + u * 512 + 16), off);
+        }
+        __syncwarp();
+        if (lane == 0 && arrived) {
+          fence_proxy_async_smem();
+          issue(q + S, st);
+        }
+        if (first + kStepElems > V) {
+#pragma unroll
+          for (int u = 0; u < kTopStep; ++u) {
+            const int left = V - (first + (u * 32 + lane) * n);
+            if (left < n) raw[u] = RowVec<T>::select(raw[u], left <= 0 ? 0u : (1u << left) - 1u);
+          }
+        }
+        float vm[kTopStep];
+#pragma unroll
+        for (int u = 0; u < kTopStep; ++u) {
+          if (MASKED) raw[u] = RowVec<T>::select(raw[u], bits >> ((h * kTopStep + u) * n));
+          vm[u] = RowVec<T>::largest(raw[u]);
+        }
+        const float tm = max_nan(max_nan(vm[0], vm[1]), vm[2], vm[3]);
+        add_exps<T, kTopStep>(acc, raw, tm, scale);
+        tile_max = max_nan(tile_max, tm);
+        if (++st == S) { st = 0; parity ^= 1; }
       }
-      if (t + 1 < t1) work(t + 1, odd, bo, m1);
-      if (MASKED) {
-#pragma unroll
-        for (int u = 0; u < kTopU; ++u) bo[u] = bn[u];
-      }
     }
+    tops[(t - t0) * kTopThreads + tid] = (uint16_t)(ordkey(tile_max) >> 16);
+    const float mx = fmaxf(m0, tile_max);
+    m0 = m1;
+    m1 = mx;
+    bits = next_bits;
+  }
+  if (!arrived) {
+    // give the copies in flight their time before their memory is used again
+    for (int j = 1; j < S; ++j) {
+      mbar_wait(&bar[st], parity);
+      if (++st == S) { st = 0; parity ^= 1; }
+    }
+    acc.add(nan64(), kNegInf64);
+    m0 = m1 = kNegInf;
   }
 
   // the bound: the warp's `place`-th largest of its lanes' 64 maxima
   const float m = fmaxf(m0, m1);
-  const int place = (K + kTopWarps - 1) / kTopWarps;
-  float o;
-  if (place <= 8) {
-    // taken one by one, the first of equal lanes
-    uint32_t mine = ordkey(m);
-    const uint32_t second = ordkey(fminf(m0, m1));
-    bool first = true;
-    uint32_t most = 0;
-    for (int i = 0; i < place; ++i) {
-      most = __reduce_max_sync(kFull, mine);
-      const unsigned at_most = __ballot_sync(kFull, mine == most);
-      if (lane == __ffs(at_most) - 1) {
-        mine = first ? second : 0u;
-        first = false;
-      }
-    }
-    o = key_value((uint64_t)most << 32);
-  } else {
-    // the 32 largest in descending order
-    auto sorted = [&](float v) {
-#pragma unroll
-      for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-        for (int j = k >> 1; j > 0; j >>= 1) {
-          const float p = __shfl_xor_sync(kFull, v, j);
-          v = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(v, p) : fminf(v, p);
-        }
-      return v;
-    };
-    const float hi = sorted(m), lo = sorted(fminf(m0, m1));
-    o = fmaxf(hi, __shfl_sync(kFull, lo, 31 - lane));
-#pragma unroll
-    for (int j = 16; j > 0; j >>= 1) {
-      const float p = __shfl_xor_sync(kFull, o, j);
-      o = (lane & j) == 0 ? fmaxf(o, p) : fminf(o, p);
-    }
-    o = __shfl_sync(kFull, o, place - 1);
-  }
+  float o = warp_place(m0, m1, (K + kTopWarps - 1) / kTopWarps);
   // and the largest exponent and element
   const double wrho = warp_max64(acc.rho);
   const float wm = warp_max_ordered(m);
   if (lane == 0) { sh.wbound[warp] = o; sh.wrho[warp] = wrho; sh.wmax[warp] = wm; }
   __syncthreads();
-  float bound = sh.wbound[0];
-#pragma unroll
-  for (int w = 1; w < kTopWarps; ++w) bound = fminf(bound, sh.wbound[w]);
+  float bound = -warp_max_ordered(-sh.wbound[lane % kTopWarps]);
+  // warps that hold nothing (behind the row's end, nothing allowed): the
+  // others' share is larger
+  const int holding = __popc(__ballot_sync(kFull, sh.wmax[lane % kTopWarps] > kNegInf)) / (32 / kTopWarps);
+  if (holding > 0 && holding < kTopWarps) {
+    o = warp_place(m0, m1, (K + holding - 1) / holding);
+    __syncthreads();
+    if (lane == 0) sh.wbound[warp] = wm > kNegInf ? o : -kNegInf;
+    __syncthreads();
+    bound = -warp_max_ordered(-sh.wbound[lane % kTopWarps]);
+  }
   const float below = bound > kNegInf ? float_below(bound) : kNegInf;
   if (m > below) {
     // without a bound every tile that holds anything
@@ -360,15 +437,15 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
     for (int t = t0; t < t1; ++t)
       if (tops[(t - t0) * kTopThreads + tid] >= least) {
         const int pos = atomicAdd(&sh.listed, 1);
-        if (pos < kTopList) sh.list[pos] = (uint16_t)((t - t0) * kTopThreads + tid);
+        if (pos < kTopList) sh.list()[pos] = (uint16_t)((t - t0) * kTopThreads + tid);
       }
   }
   __syncthreads();
   const int listed = sh.listed;
   if (listed <= kTopList) {
-    for (int j = tid; j < listed * kTopU; j += kTopThreads) {
-      const int g = sh.list[j / kTopU], u = j % kTopU;
-      const int i = (t0 + g / kTopThreads) * kTile + (u * kTopThreads + g % kTopThreads) * n;
+    for (int j = tid; j < listed * U; j += kTopThreads) {
+      const int g = sh.list()[j / U];
+      const int i = at(t0 + g / kTopThreads, j % U, g % kTopThreads);
       top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), (uint32_t)i, below);
     }
   }
@@ -377,29 +454,24 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
   if (lane == 0) sh.wsum[warp] = s;
   __syncthreads();
   if (listed > kTopList || sh.count > kTopBuf)
-    top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTile, t1 * kTile, V, K);
+    top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTopTile, t1 * kTopTile, V, K);
 
   // the part's list, maximum and sum
-  if (tid == 0) {
-    ExpSum part = {sh.wsum[0], rho};
-    float top = sh.wmax[0];
-#pragma unroll
-    for (int w = 1; w < kTopWarps; ++w) {
-      part.s += sh.wsum[w];
-      top = fmaxf(top, sh.wmax[w]);
+  if (warp == kTopWarps - 1) {
+    ExpSum part = {warp_sum64(lane < kTopWarps ? sh.wsum[lane] : 0.0), rho};
+    const float top = warp_max_ordered(sh.wmax[lane % kTopWarps]);
+    if (lane == 0) {
+      sh.part[0] = part;
+      sh.top[0] = top;
     }
-    sh.part[0] = part;
-    sh.top[0] = top;
   }
-  const int cnt = sh.count;
-  __syncthreads();
-  top_cut(sh, cnt, K);
+  top_cut(sh, sh.count, K);
 
   if (split > 1) {
-    uint64_t* keys = reinterpret_cast<uint64_t*>(tops + per * kTopThreads);
+    uint64_t* keys = reinterpret_cast<uint64_t*>(tops + per * kTopThreads);  // 16-byte aligned
     cluster_wait();  // every CTA of the cluster runs
     const int mine = sh.got;
-    for (int i = tid; i < mine; i += kTopThreads) *of_rank(&keys[rank * K + i], 0) = sh.best[i];
+    for (int i = tid; i < K; i += kTopThreads) *of_rank(&keys[rank * K + i], 0) = i < mine ? sh.best[i] : 0ull;
     if (tid == 0) {
       if (rank > 0) {
         *of_rank(&sh.part[rank], 0) = sh.part[0];
@@ -426,25 +498,41 @@ __global__ void __launch_bounds__(kTopThreads, kTopResident) k_top_rows(TopArgs 
         sh.got = got < K ? got : K;
       }
     }
-    // a key's place in the row: its place in its own list, and the number of
-    // larger keys in each of the others, all searched at once
-    int half = 1;
-    while (half * 2 <= K) half *= 2;
-    for (int i = tid; i < K * (int)split; i += kTopThreads) {
-      const int c = i / K;
-      int place = i - c * K;
-      if (place >= sh.parts_got[c]) continue;
-      const uint64_t key = keys[i];
-      int at[kTopSplit] = {};
-      for (int step = half; step > 0; step >>= 1)
-#pragma unroll
-        for (int d = 0; d < kTopSplit; ++d) {
-          const int to = at[d] + step;
-          if (d < (int)split && to <= sh.parts_got[d] && keys[d * K + to - 1] > key) at[d] = to;
+    // a key's place in the row is the number of larger keys
+    const int all = K * (int)split;
+    if (all <= kTopFew) {
+      const uint64_t key = tid < all ? keys[tid] : 0ull;
+      if (key) {
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < all; j += 2) {  // split is even
+          const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&keys[j]);
+          place += (o.x > key) + (o.y > key);
         }
+        if (place < K) sh.best[place] = key;
+      }
+    } else {
+      // searched for in all the lists at once
+      int half = 1;
+      while (half * 2 <= K) half *= 2;
+      for (int i = tid; i < all; i += kTopThreads) {
+        const uint64_t key = keys[i];
+        if (!key) continue;
+        int found[kTopSplit] = {};
+        for (int step = half; step > 0; step >>= 1) {
 #pragma unroll
-      for (int d = 0; d < kTopSplit; ++d) place += d != c ? at[d] : 0;
-      if (place < K) sh.best[place] = key;
+          for (int d = 0; d < kTopSplit; ++d) {
+            const int to = found[d] + step;
+            // lists that the row does not have hold nothing larger
+            const uint64_t there = keys[(d < (int)split ? d : 0) * K + (to < K ? to : K) - 1];
+            if (to <= K && d < (int)split && there > key) found[d] = to;
+          }
+        }
+        int place = 0;
+#pragma unroll
+        for (int d = 0; d < kTopSplit; ++d) place += found[d];
+        if (place < K) sh.best[place] = key;
+      }
     }
     __syncthreads();
   }
@@ -644,12 +732,22 @@ int check_logits(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
   return PM_OK;
 }
 
-// CTAs of a row: enough to fill the resident CTAs of every SM, no more
-// than it has tiles.
-int top_split(int64_t rows, int64_t tiles) {
-  const int64_t slots = (int64_t)pmh::num_sms() * pm::kTopResident;
+// Shared memory of a CTA: the rings, a part's maxima, and the parts' lists of
+// a row that is split.
+size_t top_bytes(int64_t tiles, int split, int k) {
+  return sizeof(pm::TopShared) + pm::kTopRingBytes + (size_t)((tiles + split - 1) / split) * pm::kTopThreads * 2 +
+         (split > 1 ? (size_t)split * k * 8 : 0);
+}
+
+// CTAs of a row: enough to fill every SM with resident CTAs, no more than it
+// has tiles.
+int top_split(int64_t rows, int64_t tiles, int k) {
   int c = 1;
-  while (c < pm::kTopSplit && 2 * c <= tiles && rows * 2 * c <= slots) c *= 2;
+  while (c < pm::kTopSplit && 2 * c <= tiles) {
+    const int64_t resident = 232448 / (int64_t)(top_bytes(tiles, 2 * c, k) + 1024);
+    if (rows * 2 * c > (int64_t)pmh::num_sms() * resident) break;
+    c *= 2;
+  }
   return c;
 }
 
@@ -658,22 +756,18 @@ cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
   auto* kernel = pm::k_top_rows<T, MASKED, ALIGNED>;
   static pmh::DeviceOnce once;
   cudaError_t e = cudaSuccess;
-  constexpr int64_t kTile = (int64_t)pm::kTopThreads * pm::kTopU * pm::RowVec<T>::n;
-  // a part's maxima, and the parts' lists of a row that is split
-  auto bytes = [](int64_t tiles, int split, int k) {
-    return sizeof(pm::TopShared) + (size_t)tiles * pm::kTopThreads * 2 + (split > 1 ? (size_t)split * k * 8 : 0);
-  };
   once([&] {
+    constexpr int64_t most = kMaxVocab / pm::kTopTile;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)bytes(kMaxVocab / kTile, pm::kTopSplit, pm::kTopMax));
+                             (int)(top_bytes(most, 1, pm::kTopMax) + (size_t)pm::kTopSplit * pm::kTopMax * 8));
   });
   if (e != cudaSuccess) return e;
-  const int64_t tiles = (a.vocab + kTile - 1) / kTile;
-  const int split = top_split(a.rows, tiles);
+  const int64_t tiles = (a.vocab + pm::kTopTile - 1) / pm::kTopTile;
+  const int split = top_split(a.rows, tiles, a.k);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * split));
   cfg.blockDim = dim3(pm::kTopThreads);
-  cfg.dynamicSmemBytes = bytes((tiles + split - 1) / split, split, a.k);
+  cfg.dynamicSmemBytes = top_bytes(tiles, split, a.k);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

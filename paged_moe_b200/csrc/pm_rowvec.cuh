@@ -86,6 +86,21 @@ template <> struct RowVec<__nv_bfloat16> {
   }
 };
 
+// The 16 bytes that start `off` bytes (a multiple of the element size) into
+// the aligned vector a, b being the one behind it.
+template <typename T>
+__device__ __forceinline__ uint4 shift_raw(uint4 a, uint4 b, int off) {
+  uint32_t w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x, w5 = b.y, w6 = b.z, w7 = b.w;
+  if (off & 8) { w0 = w2; w1 = w3; w2 = w4; w3 = w5; w4 = w6; w5 = w7; }
+  if (off & 4) { w0 = w1; w1 = w2; w2 = w3; w3 = w4; w4 = w5; }
+  if (sizeof(T) == 2) {
+    const int s = (off & 2) * 8;
+    w0 = __funnelshift_r(w0, w1, s); w1 = __funnelshift_r(w1, w2, s);
+    w2 = __funnelshift_r(w2, w3, s); w3 = __funnelshift_r(w3, w4, s);
+  }
+  return make_uint4(w0, w1, w2, w3);
+}
+
 // Elements [i, i + n) of a row, -inf behind its end.  A vector that lies
 // across the end is read element by element.  Rows that do not start on a
 // 16-byte boundary (off: bytes past one) are read as the two aligned vectors
@@ -99,15 +114,7 @@ __device__ __forceinline__ uint4 load_raw(const T* row, int off, int i, int V) {
     const uint4 a = __ldg(reinterpret_cast<const uint4*>(at));
     if (off == 0) return a;
     const uint4 b = __ldg(reinterpret_cast<const uint4*>(at + 16));
-    uint32_t w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x, w5 = b.y, w6 = b.z, w7 = b.w;
-    if (off & 8) { w0 = w2; w1 = w3; w2 = w4; w3 = w5; w4 = w6; w5 = w7; }
-    if (off & 4) { w0 = w1; w1 = w2; w2 = w3; w3 = w4; w4 = w5; }
-    if (sizeof(T) == 2) {
-      const int s = (off & 2) * 8;
-      w0 = __funnelshift_r(w0, w1, s); w1 = __funnelshift_r(w1, w2, s);
-      w2 = __funnelshift_r(w2, w3, s); w3 = __funnelshift_r(w3, w4, s);
-    }
-    return make_uint4(w0, w1, w2, w3);
+    return shift_raw<T>(a, b, off);
   }
   constexpr uint32_t fill = RowVec<T>::kFill;
   uint4 r = make_uint4(fill, fill, fill, fill);
