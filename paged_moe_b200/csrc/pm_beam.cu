@@ -246,6 +246,17 @@ __device__ __forceinline__ V* of_rank(V* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// The thread's share of the sum over elements [i0, i1) of a wild row.
+template <typename T, bool MASKED, bool ALIGNED>
+__device__ __noinline__ ExpSum top_wild(const T* row, int off, const uint8_t* mask, int i0, int i1, int V,
+                                        ExpScale scale) {
+  ExpSum acc;
+  acc.clear();
+  for (int i = i0 + (int)threadIdx.x * RowVec<T>::n; i < i1; i += kTopThreads * RowVec<T>::n)
+    add_wild<T>(acc, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), scale);
+  return acc;
+}
+
 // The place-th largest of the warp's 64 values a, b; -inf if place > 64.
 __device__ __forceinline__ float warp_place(float a, float b, int place) {
   const int lane = threadIdx.x & 31;
@@ -350,7 +361,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   uint32_t bits = load_bits(t0);
   __syncwarp();
 
-  ExpSum acc;
+  StepSum acc;
   acc.clear();
   float m0 = kNegInf, m1 = kNegInf;  // of every second tile each
   int st = 0, q = 0;
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
           vm[u] = RowVec<T>::largest(raw[u]);
         }
         const float tm = max_nan(max_nan(vm[0], vm[1]), vm[2], vm[3]);
-        add_exps<T, kTopStep>(acc, raw, tm, scale);
+        add_exps<T, kTopStep>(acc, raw, tm, scale.c);
         tile_max = max_nan(tile_max, tm);
         if (++st == S) { st = 0; parity ^= 1; }
       }
@@ -407,7 +418,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
       mbar_wait(&bar[st], parity);
       if (++st == S) { st = 0; parity ^= 1; }
     }
-    acc.add(nan64(), kNegInf64);
+    acc.s = nan64();
     m0 = m1 = kNegInf;
   }
 
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   const float m = fmaxf(m0, m1);
   float o = warp_place(m0, m1, (K + kTopWarps - 1) / kTopWarps);
   // and the largest exponent and element
-  const double wrho = warp_max64(acc.rho);
+  const double wrho = warp_max64(acc.sum().rho);
   const float wm = warp_max_ordered(m);
   if (lane == 0) { sh.wbound[warp] = o; sh.wrho[warp] = wrho; sh.wmax[warp] = wm; }
   __syncthreads();
@@ -449,8 +460,16 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
       top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), (uint32_t)i, below);
     }
   }
-  const double rho = warp_max64(sh.wrho[lane % kTopWarps]);
-  const double s = warp_sum64(scaled_to(acc, rho));
+  double rho = warp_max64(sh.wrho[lane % kTopWarps]);
+  ExpSum mine = acc.sum();
+  if (__syncthreads_or(acc.wild(warp_max_ordered(sh.wmax[lane % kTopWarps]), scale.c) && acc.s == acc.s)) {
+    mine = top_wild<T, MASKED, ALIGNED>(row, off, mask, t0 * kTopTile, t1 * kTopTile, V, scale);
+    const double r = warp_max64(mine.rho);
+    if (lane == 0) sh.wrho[warp] = r;
+    __syncthreads();
+    rho = warp_max64(sh.wrho[lane % kTopWarps]);
+  }
+  const double s = warp_sum64(scaled_to(mine, rho));
   if (lane == 0) sh.wsum[warp] = s;
   __syncthreads();
   if (listed > kTopList || sh.count > kTopBuf)

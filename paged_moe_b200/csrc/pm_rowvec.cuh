@@ -1,14 +1,20 @@
 // pm_rowvec.cuh -- rows of fp32 or bf16 logits read as 16-byte vectors, and
 // sums of their exponentials.
 //
-// Sums of e^(x / T) are kept as s 2^rho with s and rho in 64 bits.  A thread
-// sums a tile's vectors in fp32 as 2^(x c - R), c = fl32(log2(e) / T) and R
-// the integer nearest to the tile's largest x c: x c - R is one fused
-// multiply-add, R is exact, and tiles of different R are added with exact
-// powers of two.  So neither the order of the tiles nor how a row is split
+// Sums of e^(x / T) are kept as s 2^rho with s in 64 bits.  A thread sums a
+// step's vectors in fp32 as 2^(x c - R), c = fl32(log2(e) / T) and R the
+// integer nearest to the step's largest x c: x c - R is one fused
+// multiply-add, R is exact, and steps of different R are added with exact
+// powers of two.  So neither the order of the steps nor how a row is split
 // over CTAs changes more than the last bits of a 64-bit sum: a row's
 // log-sum-exp does not depend on the batch around it.  What c lacks of
 // log2(e) / T is put back once per row, for the row's maximum.
+//
+// Where |x c| passes 2^20 it no longer has the bits for this.  Steps far below
+// (masks of the type's lowest value) are left out: they add nothing to a row
+// that holds anything else.  A row, or part of one, that reaches far above,
+// or holds nothing but such values, is wild: it is summed once more, as
+// 2^((x - m) c) with rho = m log2(e) / T.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -145,20 +151,48 @@ __device__ __forceinline__ double pow2_down(double d) {
   return exp2_apart(d);
 }
 
-// A running sum s 2^rho.
+// A sum s 2^rho; rho = -inf: nothing, but s may be a NaN.
 struct ExpSum {
   double s, rho;
   __device__ __forceinline__ void clear() { s = 0.0; rho = kNegInf64; }
-  // += t 2^r; r = -inf stands for nothing but may carry a NaN in t
   __device__ __forceinline__ void add(double t, double r) {
     if (r > rho) {
-      s = s * pow2_down(rho - r) + t;  // from nothing: s is 0, or a NaN that stays
+      s = s * pow2_down(rho - r) + t;
       rho = r;
     } else if (r == rho) {
       s += t;
     } else {
       s += r > kNegInf64 ? t * pow2_down(r - rho) : t;
     }
+  }
+};
+
+// A thread's running sum, of steps with whole exponents.
+struct StepSum {
+  static constexpr int kNothing = -(1 << 28);
+  double s;
+  int rho;
+  bool high, low;  // a step far above, or far below, was left out
+  __device__ __forceinline__ void clear() { s = 0.0; rho = kNothing; high = low = false; }
+  // whether what was left out may count in a sum of maximum m
+  __device__ __forceinline__ bool wild(float m, float c) const {
+    return high || (low && !(m * c > -kWildExponent + 4096.0f));
+  }
+  // += t 2^r for a normal t > 0: integer operations and one fused multiply-add
+  __device__ __forceinline__ void add(float t, int r) {
+    const uint32_t b = __float_as_uint(t);
+    const double t64 = __hiloint2double((int)((b >> 3) + (896u << 20)), (int)(b << 29));
+    const bool up = r > rho;
+    const int apart = up ? r - rho : rho - r;
+    const double shift = __hiloint2double((1023 - (apart < 1000 ? apart : 1000)) << 20, 0);
+    s = dfma(up ? s : t64, shift, up ? t64 : s);
+    rho = up ? r : rho;
+  }
+  __device__ __forceinline__ ExpSum sum() const {
+    ExpSum e;
+    e.s = s;
+    e.rho = rho > kNothing ? (double)rho : kNegInf64;
+    return e;
   }
 };
 
@@ -199,26 +233,16 @@ struct ExpScale {
   }
 };
 
-template <typename T>
-__device__ __noinline__ float wild_exps(uint4 raw, float tm, float c) {
-  float v[RowVec<T>::n], sum = 0.0f;
-  RowVec<T>::unpack(raw, v);
-#pragma unroll
-  for (int e = 0; e < RowVec<T>::n; ++e) sum += ex2_approx((v[e] - tm) * c);
-  return sum;
-}
-
 // Adds the 2^(x c) of U vectors whose largest element is tm (NaN: one of
-// them holds a NaN).
+// them holds a NaN, and so does the sum from here on).
 template <typename T, int U>
-__device__ __forceinline__ void add_exps(ExpSum& acc, const uint4 (&raw)[U], float tm, const ExpScale& k) {
+__device__ __forceinline__ void add_exps(StepSum& acc, const uint4 (&raw)[U], float tm, float c) {
   constexpr int n = RowVec<T>::n;
-  const float top = tm * k.c;
-  if (!(tm > kNegInf)) {
-    acc.add(tm == kNegInf ? 0.0 : nan64(), kNegInf64);
-  } else if (fabsf(top) < kWildExponent) {
-    const float R = rintf(top);
-    const uint64_t c2 = pk(k.c, k.c), r2 = pk(-R, -R);
+  const float top = tm * c;
+  if (fabsf(top) < kWildExponent) {
+    const float magic = top + 12582912.0f;  // 1.5 2^23 + R
+    const float R = magic - 12582912.0f;
+    const uint64_t c2 = pk(c, c), r2 = pk(-R, -R);
     uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -232,13 +256,25 @@ __device__ __forceinline__ void add_exps(ExpSum& acc, const uint4 (&raw)[U], flo
       }
     }
     const uint64_t sum = add2(sum0, sum1);
-    acc.add((double)lo_f(sum) + (double)hi_f(sum), (double)R);
+    acc.add(lo_f(sum) + hi_f(sum), (int)(__float_as_uint(magic) - 0x4B400000u));
+  } else if (tm < 0.0f) {
+    acc.low = acc.low || tm > kNegInf;
   } else {
-    float sum = 0.0f;
-#pragma unroll
-    for (int u = 0; u < U; ++u) sum += wild_exps<T>(raw[u], tm, k.c);
-    acc.add((double)sum, (double)tm * k.exact);
+    acc.high = true;
+    if (tm != tm) acc.s = nan64();
   }
+}
+
+// A wild row's elements of one vector.
+template <typename T>
+__device__ __forceinline__ void add_wild(ExpSum& acc, uint4 raw, const ExpScale& k) {
+  const float tm = RowVec<T>::largest(raw);
+  if (tm == kNegInf) return;
+  float v[RowVec<T>::n], sum = 0.0f;
+  RowVec<T>::unpack(raw, v);
+#pragma unroll
+  for (int e = 0; e < RowVec<T>::n; ++e) sum += ex2_approx((v[e] - tm) * k.c);
+  acc.add((double)sum, tm == tm ? (double)tm * k.exact : kNegInf64);
 }
 
 }  // namespace pm
