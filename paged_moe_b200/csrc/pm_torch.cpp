@@ -510,7 +510,7 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
 }
 
 // pm_distill_loss over logits [..., V] viewed as rows: [loss or empty, grad or
-// empty].  The gradient is [N, V], dense.
+// empty].  The gradient is [N, V], dense where the logits are.
 std::vector<torch::Tensor> distill(torch::Tensor logits, torch::Tensor ids, torch::Tensor logprobs, double temp,
                                    int64_t tail, OptT weights, int64_t reduction, bool want_loss, bool want_grad,
                                    OptT grad_loss) {
@@ -565,8 +565,19 @@ std::vector<torch::Tensor> distill(torch::Tensor logits, torch::Tensor ids, torc
   if (want_loss)
     loss = torch::empty(reduction == PM_REDUCE_NONE ? std::vector<int64_t>{N} : std::vector<int64_t>{},
                         x.options().dtype(torch::kFloat32));
-  if (want_grad) grad = torch::empty({N, V}, x.options());
-  check(pm_distill_loss(&d, want_loss ? loss.data_ptr<float>() : nullptr, want_grad ? grad.data_ptr() : nullptr, V,
+  if (want_grad) {
+    // rows as far from a 16-byte boundary as the logits', so that the kernel
+    // reads and writes whole vectors; dense where the logits are
+    const int64_t unit = 16 / x.element_size();
+    const int64_t first = (int64_t)(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16) / x.element_size();
+    const int64_t step = N > 1 ? V + ((x.stride(0) - V) % unit + unit) % unit : V;
+    if (first == 0 && step == V)
+      grad = torch::empty({N, V}, x.options());
+    else
+      grad = torch::empty({first + N * step}, x.options()).as_strided({N, V}, {step, 1}, first);
+  }
+  check(pm_distill_loss(&d, want_loss ? loss.data_ptr<float>() : nullptr, want_grad ? grad.data_ptr() : nullptr,
+                        want_grad && N > 1 ? grad.stride(0) : V,
                         reinterpret_cast<const float*>(ptr(grad_loss)), ws.data_ptr(), need, stream_of(dev)),
         "pm_distill_loss");
   return {loss, grad};
@@ -576,7 +587,7 @@ std::vector<torch::Tensor> distill(torch::Tensor logits, torch::Tensor ids, torc
 void distill_scale(torch::Tensor grad, torch::Tensor factor) {
   const c10::cuda::CUDAGuard guard(grad.device());
   factor = factor.detach().to(torch::kFloat32).contiguous();
-  check(pm_distill_scale(grad.data_ptr(), logits_code(grad), grad.size(0), grad.size(1), grad.stride(0),
+  check(pm_distill_scale(grad.data_ptr(), logits_code(grad), grad.size(0), grad.size(1), row_stride(grad),
                          factor.data_ptr<float>(), stream_of(grad.device())),
         "pm_distill_scale");
 }
