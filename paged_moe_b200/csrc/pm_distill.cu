@@ -1,22 +1,20 @@
 // pm_distill.cu -- distillation loss from a teacher's top log-probabilities,
-// and its gradient.  Three kernels:
+// and its gradient.  Two kernels:
 //
 // k_distill_prep, a warp per row: the row's entries become probabilities in
 //   64 bits (the mass they leave is a difference of nearly equal numbers),
 //   sorted by id, the entries of one id added up.
-// k_distill_rows, a cluster of CTAs per row, each a slice of it that stays in
-//   its shared memory: bulk copies bring it in once, the pass that sums the
-//   exponentials and the pass that writes the gradient both read it there, so
-//   that a training step moves each logit in and each gradient out and
-//   nothing else.  Slices are at most about 45 KB, so that several CTAs share
-//   an SM and one's copies run under another's arithmetic.  The first pass
-//   keeps two sums of e^(x / T), over all tokens and over those that are no
-//   entries (again no difference of nearly equal numbers); the cluster's CTAs
-//   put theirs into one another's shared memory.  The gradient is e^(x / T)
-//   times one factor per row, and on entries q - p.
-// k_distill_finish, a warp per row: the loss from the row's sums and the
-//   entries' logits; the last CTA adds the rows up in a fixed order.  A wild
-//   row (pm_rowvec.cuh) is done here from its start.
+// k_distill_rows, a CTA per row, or a cluster where there are few rows.  Every
+//   warp streams its chunks through a ring in shared memory that its first
+//   lane keeps full with bulk copies: once forward for two sums of e^(x / T),
+//   over all tokens and over those that are no entries (again no difference
+//   of nearly equal numbers), and once more, backward, for the gradient,
+//   e^(x / T) times one factor per row, and on entries q - p.  The second
+//   time the logits come from L2: two rows an SM are in work, 95 MB at 320 KB
+//   a row, of which half is still wanted on average; what was read last is
+//   read first, and the gradients are stored as data that nobody reads soon.
+//   So device memory sees each logit once and each gradient once.  The last
+//   CTA to end adds the rows' losses up in a fixed order.
 //
 // Memory is cut at 16-byte boundaries: granule j of a row holds the elements
 // whose bytes share the j-th aligned 16 bytes.  The gradient's rows start as
@@ -36,17 +34,17 @@
 
 namespace pm {
 
-constexpr int kDistThreads = 128;
+constexpr int kDistThreads = 512;
 constexpr int kDistWarps = kDistThreads / 32;
-constexpr int kDistResident = 5;               // CTAs of an SM
+constexpr int kDistResident = 2;               // CTAs of an SM
 constexpr int kDistMax = 256;                  // largest k
 constexpr int kDistHeld = kDistMax / 32;       // entries of a lane
 constexpr int64_t kDistVocab = 262144;
-constexpr int kDistSplit = 16;                 // most CTAs of a row
-constexpr int kDistChunks = 4;                 // copies of a slice
-constexpr int kDistStep = 4;                   // vectors of a thread that are summed together
-constexpr int kDistStride = kDistThreads * kDistStep;  // granules of a step
-constexpr int kDistSlice = 45056;              // bytes of a slice that more CTAs are taken for
+constexpr int kDistSplit = 8;                  // most CTAs of a row
+constexpr int kDistStep = 4;                   // vectors of a lane in a chunk
+constexpr int kDistChunk = 32 * kDistStep;     // granules of a warp's chunk, a stage of its ring
+constexpr int kDistTile = kDistWarps * kDistChunk;
+constexpr int kDistStages = 2;
 constexpr int kRowThreads = 256;               // of the two kernels with a warp per row
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr double kTailFloor = 0x1p-100;        // smallest tail mass of the student that is told apart
@@ -55,10 +53,7 @@ constexpr double kTailFloor = 0x1p-100;        // smallest tail mass of the stud
 struct DistillRow {
   double mass;     // of its entries, 1 for PM_TAIL_DROP, 0 where they have none
   double shift;    // sum of p log p over the entries as they were given
-  double all, rest, rho;  // the student's sums, as multiples of 2^rho
-  float top;       // its largest logit
   int held;        // ids
-  int wild;
   int pad;
 };
 
@@ -189,7 +184,6 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
     row.mass = total;
     row.shift = entropy;
     row.held = held;
-    row.wild = 0;
   }
 }
 
@@ -223,15 +217,12 @@ struct DistillSum {
 };
 
 struct alignas(16) DistillShared {
-  uint64_t bar[kDistChunks];
+  uint64_t bar[kDistWarps][kDistStages];
   DistillPart warps[kDistWarps];
-  DistillPart parts[kDistSplit];
-  double p[kDistMax];        // the slice's entries
-  int at[kDistMax];          // their places, counted in elements from the slice's first granule
-  double on, by;             // factors of a marked element's q and p
-  float off, rho;            // of any other element's q, a multiple of 2^rho
-  int held, skip;
-  // then the slice, and a word of marks per thread and step: bit u n + e is
+  DistillPart parts[2][kDistSplit];  // of the first join, and of a wild row's
+  double loss[kDistWarps];
+  int last;
+  // then the rings, and a word of marks per tile and thread: bit u n + e is
   // element e of the thread's vector u
 };
 
@@ -266,7 +257,7 @@ __device__ __forceinline__ V* dist_of(V* p, uint32_t rank) {
 }
 
 // The warp's parts as one.
-__device__ __noinline__ DistillPart dist_reduce(DistillPart p) {
+__device__ __forceinline__ DistillPart dist_reduce(DistillPart p) {
   const double to = warp_max64(p.rho);
   const double f = p.rho > kNegInf64 ? pow2_down(p.rho - to) : 1.0;  // nothing: 0, or a NaN that stays
   p.all = warp_sum64(p.all * f);
@@ -275,6 +266,29 @@ __device__ __noinline__ DistillPart dist_reduce(DistillPart p) {
   p.top = warp_max_ordered(p.top);
   p.flags = (int)__reduce_or_sync(kFull, (unsigned)p.flags);
   return p;
+}
+
+// The row's part from its warps', through the cluster; every thread gets it.
+__device__ __noinline__ DistillPart dist_join(DistillShared& sh, DistillPart part, int again, uint32_t rank,
+                                              uint32_t split) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const DistillPart none = {0.0, 0.0, kNegInf64, kNegInf, 0};
+  part = dist_reduce(part);
+  if (lane == 0) sh.warps[warp] = part;
+  __syncthreads();
+  if (split == 1) {
+    part = dist_reduce(lane < kDistWarps ? sh.warps[lane] : none);
+    __syncthreads();
+    return part;
+  }
+  if (again == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
+  if (warp == 0) {
+    part = dist_reduce(lane < kDistWarps ? sh.warps[lane] : none);
+    if (lane < (int)split) *dist_of(&sh.parts[again][rank], lane) = part;
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  return dist_reduce(lane < (int)split ? sh.parts[again][lane] : none);
 }
 
 // What multiplies a row's gradient: weight, temperature, reduction and the
@@ -303,6 +317,30 @@ __device__ __forceinline__ double dist_factor(const DistillArgs& a, const Distil
   return 1.0 - left / dist_tail(rest, all);
 }
 
+// Of a wild row's part, elements [i0, i1): the sums of 2^((x - top) c), and
+// once they are known (S > 0) the gradient.
+template <typename T>
+__device__ __noinline__ void dist_wild(const DistillArgs& a, int64_t r, int i0, int i1, float top, double on, double off,
+                                       double by, bool store, double* all, double* rest) {
+  const int K = a.k, held = a.row[r].held;
+  const T* x = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
+  T* g = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
+  const float c = (float)(kLog2e64 * a.inv_t);
+  const int32_t* at = a.at + r * K;
+  for (int i = i0 + (int)threadIdx.x; i < i1; i += kDistThreads) {
+    const double e = (double)ex2_approx((RowVec<T>::get(x + i) - top) * c);
+    int lo = 0, hi = held;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (at[mid] < i) lo = mid + 1; else hi = mid;
+    }
+    const bool entry = lo < held && at[lo] == i;
+    *all += e;
+    *rest += entry ? 0.0 : e;
+    if (store) put_grad(g + i, entry ? (float)(e * on - a.p[r * K + lo] * by) : (float)(e * off));
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(DistillArgs a) {
   extern __shared__ __align__(16) unsigned char shared_bytes[];
@@ -312,96 +350,118 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = dist_rank(), split = dist_split();
   const int64_t r = blockIdx.x / split;
-  const int V = (int)a.vocab;
+  const int V = (int)a.vocab, K = a.k;
   const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
   T* grow = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
   const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);  // elements before the row in granule 0
   const bool vectors = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
-  // the slice: granules [g0, g0 + count) of the row's
+  // the part: granules [g0, g0 + count) of the row's, whole tiles but the last
   const int granules = (off + V + n - 1) / n;
-  const int per = (granules + (int)split - 1) / (int)split;
+  const int per = ((granules + kDistTile - 1) / kDistTile + (int)split - 1) / (int)split * kDistTile;
   const int g0 = (int)rank * per < granules ? (int)rank * per : granules;
   const int count = granules - g0 < per ? granules - g0 : per;
-  const int first = g0 * n - off;  // the slice's first element
+  const int first = g0 * n - off;  // the part's first element
   // granules wholly inside the row; one at each end may not be
   const int whole0 = first < 0 ? 1 : 0, whole1 = first + count * n > V ? count - 1 : count;
-
-  unsigned char* slice = reinterpret_cast<unsigned char*>(&sh + 1);
-  uint32_t* marks = reinterpret_cast<uint32_t*>(slice + (size_t)per * 16);
-  const int steps = (count + kDistStride - 1) / kDistStride;
-  const int chunk = ((per + kDistChunks - 1) / kDistChunks + kDistStride - 1) / kDistStride * kDistStride;
+  uint4* out = reinterpret_cast<uint4*>(grow + first);
+  auto singly = [&](int j, const float (&v)[n]) {
+    for (int e = 0; e < n; ++e) {
+      const int i = first + j * n + e;
+      if (i >= 0 && i < V) put_grad(grow + i, v[e]);
+    }
+  };
+  auto zeros = [&]() {
+    const float zero[n] = {};
+    for (int j = tid; j < count; j += kDistThreads) {
+      if (vectors && j >= whole0 && j < whole1) __stcs(out + j, make_uint4(0, 0, 0, 0));
+      else singly(j, zero);
+    }
+  };
+  double l = 0.0;  // of the thread's entry, then the row's
   // a row of weight 0 is not read; the whole cluster knows
   const bool skip = a.weights && a.weights[r] == 0.0f;
-  if (tid == 0 && !skip) {
-    const char* src = reinterpret_cast<const char*>(row - off) + (int64_t)g0 * 16;
-    const uint64_t policy = policy_evict_first();
-    for (int c = 0; c < kDistChunks; ++c) mbar_init(&sh.bar[c], 1);
-    fence_proxy_async_smem();
-    for (int g = 0, c = 0; g < count; g += chunk, ++c) {
-      const uint32_t have = (uint32_t)(count - g < chunk ? count - g : chunk) * 16;
-      mbar_arrive_expect_tx(&sh.bar[c], have);
-      bulk_copy_g2s(slice + (size_t)g * 16, src + (int64_t)g * 16, have, &sh.bar[c], policy);
+  if (skip) {
+    if (a.grad) zeros();
+    cudaGridDependencySynchronize();
+  } else {
+    // the warp's chunks: forward, and for the gradient back again
+    unsigned char* ring = reinterpret_cast<unsigned char*>(&sh + 1) + warp * kDistStages * kDistChunk * 16;
+    uint32_t* marks = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned char*>(&sh + 1) +
+                                                  kDistWarps * kDistStages * kDistChunk * 16);
+    uint64_t* bar = sh.bar[warp];
+    const int chunks = (count - warp * kDistChunk + kDistTile - 1) / kDistTile > 0
+                           ? (count - warp * kDistChunk + kDistTile - 1) / kDistTile : 0;
+    const int copies = a.grad ? 2 * chunks : chunks;
+    const char* src = reinterpret_cast<const char*>(row - off) + ((int64_t)g0 + warp * kDistChunk) * 16;
+    auto issue = [&](int q, int st) {
+      if (q >= copies) return;
+      const int t = q < chunks ? q : 2 * chunks - 1 - q;
+      const int left = count - warp * kDistChunk - t * kDistTile;
+      const uint32_t bytes = (uint32_t)(left < kDistChunk ? left : kDistChunk) * 16;
+      mbar_arrive_expect_tx(&bar[st], bytes);
+      bulk_copy_g2s_plain(ring + st * kDistChunk * 16, src + (int64_t)t * kDistTile * 16, bytes, &bar[st]);
+    };
+    if (lane == 0) {
+#pragma unroll
+      for (int st = 0; st < kDistStages; ++st) mbar_init(&bar[st], 1);
+      fence_proxy_async_smem();
+#pragma unroll
+      for (int st = 0; st < kDistStages; ++st) issue(st, st);
     }
-  }
-  if (!skip) {
     // waited for before the first store into another CTA
     if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    for (int i = tid; i < steps * kDistThreads; i += kDistThreads) marks[i] = 0;
-    if (tid == 0) sh.held = 0;
+    const int tiles = (count + kDistTile - 1) / kDistTile;
+    for (int i = tid; i < tiles * kDistThreads; i += kDistThreads) marks[i] = 0;
+    const int id = tid < K ? a.ids[r * K + tid] : -1;
     __syncthreads();
-    cudaGridDependencySynchronize();  // the entries
-    const int have = a.row[r].held;
-    for (int k = tid; k < have; k += kDistThreads) {
-      const int j = a.at[r * a.k + k] - first;
-      if (j >= 0 && j < count * n) {
-        const int v = j / n, u = v / kDistThreads;
-        atomicOr(&marks[u / kDistStep * kDistThreads + v % kDistThreads], 1u << (u % kDistStep * n + j % n));
-        const int i = atomicAdd(&sh.held, 1);  // all different: their order does not matter
-        sh.at[i] = j;
-        sh.p[i] = a.p[r * a.k + k];
-      }
+    if (id >= 0 && id < V && id >= first && id < first + count * n) {
+      const int j = (id - first) / n, e = (id - first) % n, u = j % kDistChunk / 32;
+      atomicOr(&marks[j / kDistTile * kDistThreads + j % kDistTile / kDistChunk * 32 + j % 32], 1u << (u * n + e));
     }
     __syncthreads();
 
-    // The granules at the row's ends: -inf outside of it.  The thread that
-    // does this is the only one that reads them.
-    auto close = [&](int j) {
-      for (int c = 0; c <= j / chunk; ++c) mbar_wait(&sh.bar[c], 0);
-      uint4* at = reinterpret_cast<uint4*>(slice + (size_t)j * 16);
-      uint32_t in = 0;
-      for (int e = 0; e < n; ++e) in |= first + j * n + e >= 0 && first + j * n + e < V ? 1u << e : 0u;
-      *at = RowVec<T>::select(*at, in);
+    // a copy's vectors, -inf in the granules' parts outside the row
+    int st = 0, q = 0;
+    uint32_t parity = 0;
+    bool lost = false;
+    auto take = [&](uint4 (&raw)[kDistStep], int j0) {
+      lost = !__all_sync(kFull, mbar_wait(&bar[st], parity)) || lost;
+      const uint4* from = reinterpret_cast<const uint4*>(ring + st * kDistChunk * 16) + lane;
+#pragma unroll
+      for (int u = 0; u < kDistStep; ++u) raw[u] = from[u * 32];
+      __syncwarp();
+      if (lane == 0) {
+        fence_proxy_async_smem();
+        issue(q + kDistStages, st);
+      }
+      ++q;
+      if (++st == kDistStages) { st = 0; parity ^= 1; }
+      if (j0 < whole0 || j0 + kDistChunk > whole1) {
+#pragma unroll
+        for (int u = 0; u < kDistStep; ++u) {
+          uint32_t in = 0;
+#pragma unroll
+          for (int e = 0; e < n; ++e) {
+            const int i = first + (j0 + u * 32 + lane) * n + e;
+            in |= i >= 0 && i < V ? 1u << e : 0u;
+          }
+          raw[u] = RowVec<T>::select(raw[u], in);
+        }
+      }
     };
-    if (whole0 > 0 && tid == 0) close(0);
-    if (whole1 < count && whole1 >= whole0 && tid == whole1 % kDistThreads) close(whole1);
-    __syncwarp();
 
-    // first pass: sums over all tokens and over the unmarked ones
+    // forward: sums over all tokens and over the unmarked ones
     const float c = (float)(kLog2e64 * a.inv_t);
     const uint64_t c2 = pk(c, c);
     DistillSum sums = {0.0, 0.0, StepSum::kNothing};
     float m = kNegInf;
     int flags = 0;
-    bool lost = false;
-    int ready = 0, next = 0;  // granules that have arrived, and the copy to wait for
-    for (int st = 0; st < steps; ++st) {
-      if (st * kDistStride >= ready) {
-        lost = !__all_sync(kFull, mbar_wait(&sh.bar[next++], 0)) || lost;
-        ready += chunk;
-      }
-      const int j0 = st * kDistStride + tid;
-      const uint32_t marked = marks[st * kDistThreads + tid];
+    for (int t = 0; t < chunks; ++t) {
+      const uint32_t marked = marks[t * kDistThreads + tid];
       uint4 raw[kDistStep];
-      float tm = kNegInf;
-#pragma unroll
-      for (int u = 0; u < kDistStep; ++u) {
-        constexpr uint32_t fill = RowVec<T>::kFill;
-        raw[u] = make_uint4(fill, fill, fill, fill);
-        if (j0 + u * kDistThreads < count) {
-          raw[u] = *reinterpret_cast<const uint4*>(slice + (size_t)(j0 + u * kDistThreads) * 16);
-          tm = max_nan(tm, RowVec<T>::largest(raw[u]));
-        }
-      }
+      take(raw, t * kDistTile + warp * kDistChunk);
+      const float tm = max_nan(max_nan(RowVec<T>::largest(raw[0]), RowVec<T>::largest(raw[1])),
+                               RowVec<T>::largest(raw[2]), RowVec<T>::largest(raw[3]));
       m = fmaxf(m, tm);
       const float top = tm * c;
       if (fabsf(top) < kWildExponent) {
@@ -412,7 +472,6 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
         float with = 0.0f, kept = 0.0f;  // of those with one: all elements, and the unmarked
 #pragma unroll
         for (int u = 0; u < kDistStep; ++u) {
-          if (st * kDistStride + u * kDistThreads >= count) break;  // the same for every thread
           float v[n];
           RowVec<T>::unpack(raw[u], v);
 #pragma unroll
@@ -443,192 +502,130 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       }
     }
     if (lost) sums.all = sums.rest = nan64();
-
-    // the warps' parts, the CTA's, the row's
     DistillPart part = {sums.all, sums.rest, sums.rho > StepSum::kNothing ? (double)sums.rho : kNegInf64, m, flags};
-    const DistillPart none = {0.0, 0.0, kNegInf64, kNegInf, 0};
-    part = dist_reduce(part);
-    if (lane == 0) sh.warps[warp] = part;
-    __syncthreads();
-    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
-    if (warp == 0) {
-      part = dist_reduce(lane < kDistWarps ? sh.warps[lane] : none);
-      if (split > 1 && lane < (int)split) *dist_of(&sh.parts[rank], lane) = part;
+    part = dist_join(sh, part, 0, rank, split);
+    cudaGridDependencySynchronize();  // the entries, and the sum of the weights
+    const DistillRow known = a.row[r];
+    const float top = part.top;
+    const bool wild = ((part.flags & kPartHigh) || ((part.flags & kPartLow) && !(top * c > -kWildExponent + 4096.0f))) &&
+                      part.all == part.all;
+    const int i0 = first > 0 ? first : 0, i1 = first + count * n < V ? first + count * n : V;
+    if (wild) {
+      double all = 0.0, rest = 0.0;
+      dist_wild<T>(a, r, i0, i1, top, 0.0, 0.0, 0.0, false, &all, &rest);
+      part = {all, rest, 0.0, top, 0};
+      part = dist_join(sh, part, 1, rank, split);
     }
-    if (split > 1) {
-      __syncwarp();
-      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
-    if (warp == 0) {
-      if (split > 1) part = dist_reduce(lane < (int)split ? sh.parts[lane] : none);
-      if (lane == 0) {
-        DistillRow& known = a.row[r];
-        const bool wild =
-            ((part.flags & kPartHigh) || ((part.flags & kPartLow) && !(part.top * c > -kWildExponent + 4096.0f))) &&
-            part.all == part.all;
-        // no finite logit: no distribution
-        const double all = part.top == kNegInf ? nan64() : part.all;
-        const double by = dist_by(a, r);
-        const bool empty = a.tail == PM_TAIL_DROP && known.mass == 0.0;
-        sh.on = by / all;
-        sh.by = by;
-        sh.off = (float)(sh.on * dist_factor(a, known, part.rest, all));
-        sh.rho = (float)part.rho;
-        sh.skip = empty || wild;  // a wild row's gradient is the last kernel's
-        if (rank == 0) {
-          known.all = all;
-          known.rest = part.rest;
-          known.rho = part.rho;
-          known.top = part.top;
-          known.wild = wild;
+    // no finite logit: no distribution
+    const double all = top == kNegInf ? nan64() : part.all;
+    const bool empty = a.tail == PM_TAIL_DROP && known.mass == 0.0;
+
+    // the loss: this thread's entry
+    if (rank == 0 && a.loss) {
+      // log of the sum of e^((x - top) / T)
+      const double exact = kLog2e64 * a.inv_t;
+      const double logS = wild ? log(all) : log(all) + (part.rho + (double)top * (exact - (double)c)) * kLn264 - (double)top * a.inv_t;
+      if (tid < known.held && !empty) {
+        const double p = a.p[r * K + tid];
+        const double logq = ((double)RowVec<T>::get(row + a.at[r * K + tid]) - (double)top) * a.inv_t - logS;
+        if (p != 0.0) l = -p * logq;
+      }
+      if (tid == 0 && !empty) {
+        l += known.shift;
+        if (a.tail == PM_TAIL_BUCKET && known.held < a.vocab) {
+          const double left = known.mass != known.mass ? known.mass : fmax(0.0, 1.0 - known.mass);
+          if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(part.rest, all)));
         }
       }
+      if (a.weights) l *= (double)a.weights[r];
     }
-    if (!a.grad) return;
-    __syncthreads();
-  } else {
-    cudaGridDependencySynchronize();  // so that this grid's end is the end of the one before it too
-    if (!a.grad) return;
-  }
 
-  // second pass: the gradient
-  auto singly = [&](int j, const float (&v)[n]) {
-    for (int e = 0; e < n; ++e) {
-      const int i = first + j * n + e;
-      if (i >= 0 && i < V) put_grad(grow + i, v[e]);
-    }
-  };
-  uint4* out = reinterpret_cast<uint4*>(grow + first);
-  if (skip || sh.skip) {
-    const float zero[n] = {};
-    for (int j = tid; j < count; j += kDistThreads) {
-      if (vectors && j >= whole0 && j < whole1) out[j] = make_uint4(0, 0, 0, 0);
-      else singly(j, zero);
-    }
-    return;
-  }
-  const float c = (float)(kLog2e64 * a.inv_t);
-  const float R = sh.rho, by_off = sh.off;
-  const uint64_t c2 = pk(c, c), r2 = pk(-R, -R), by2 = pk(by_off, by_off);
-  for (int st = 0; st < steps; ++st) {
-    uint32_t marked = marks[st * kDistThreads + tid];
-    int j = st * kDistStride + tid;
-#pragma unroll 2
-    for (int u = 0; u < kDistStep; ++u, j += kDistThreads, marked >>= n) {
-      if (j >= count) break;
-      float v[n], g[n];
-      RowVec<T>::unpack(*reinterpret_cast<const uint4*>(slice + (size_t)j * 16), v);
+    if (a.grad) {
+      const double by = dist_by(a, r), on = by / all, factor = on * dist_factor(a, known, part.rest, all);
+      if (wild || empty) {
+        // the copies that were on their way are not wanted
+        for (; q < copies && q < chunks + kDistStages; ++q) {
+          mbar_wait(&bar[st], parity);
+          if (++st == kDistStages) { st = 0; parity ^= 1; }
+        }
+        if (empty) {
+          zeros();
+        } else {
+          double s0 = 0.0, s1 = 0.0;
+          dist_wild<T>(a, r, i0, i1, top, on, factor, by, true, &s0, &s1);
+        }
+      } else {
+        const float R = (float)part.rho, f = (float)factor;
+        const uint64_t r2 = pk(-R, -R), f2 = pk(f, f);
+        for (int t = chunks - 1; t >= 0; --t) {
+          uint32_t marked = marks[t * kDistThreads + tid];
+          const int j0 = t * kDistTile + warp * kDistChunk;
+          uint4 raw[kDistStep];
+          take(raw, j0);
 #pragma unroll
-      for (int e = 0; e < n; e += 2) {
-        const uint64_t x = fma2(pk(v[e], v[e + 1]), c2, r2);
-        v[e] = ex2_approx(lo_f(x));
-        v[e + 1] = ex2_approx(hi_f(x));
-        const uint64_t y = mul2(pk(v[e], v[e + 1]), by2);
-        g[e] = lo_f(y);
-        g[e + 1] = hi_f(y);
-      }
-      if (marked & kBits) {
-        for (int i = 0; i < sh.held; ++i) {
-          const int e = sh.at[i] - j * n;
-          if (e >= 0 && e < n) {
-            const double y = sh.on, z = sh.p[i] * sh.by;
+          for (int u = 0; u < kDistStep; ++u) {
+            float v[n], g[n];
+            RowVec<T>::unpack(raw[u], v);
 #pragma unroll
-            for (int d = 0; d < n; ++d)
-              if (d == e) g[d] = (float)((double)v[d] * y - z);  // one rounding of the difference
+            for (int e = 0; e < n; e += 2) {
+              const uint64_t x = fma2(pk(v[e], v[e + 1]), c2, r2);
+              v[e] = ex2_approx(lo_f(x));
+              v[e + 1] = ex2_approx(hi_f(x));
+              const uint64_t y = mul2(pk(v[e], v[e + 1]), f2);
+              g[e] = lo_f(y);
+              g[e + 1] = hi_f(y);
+            }
+            const int j = j0 + u * 32 + lane;
+            if ((marked >> (u * n)) & kBits) {
+              // the entries from this vector's first element on
+              const int i = first + j * n;
+              int lo = 0, hi = known.held;
+              while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (a.at[r * K + mid] < i) lo = mid + 1; else hi = mid;
+              }
+              for (; lo < known.held && a.at[r * K + lo] < i + n; ++lo) {
+                const int e = a.at[r * K + lo] - i;
+                const double z = a.p[r * K + lo] * by;
+#pragma unroll
+                for (int d = 0; d < n; ++d)
+                  if (d == e) g[d] = (float)((double)v[d] * on - z);  // one rounding of the difference
+              }
+            }
+            if (vectors && j >= whole0 && j < whole1) __stcs(out + j, pack_grad(g));
+            else if (j < count) singly(j, g);
           }
         }
       }
-      if (vectors && j >= whole0 && j < whole1) out[j] = pack_grad(g);
-      else singly(j, g);
     }
   }
-}
 
-// ---------------------------------------------------------------------------
-// The loss
-// ---------------------------------------------------------------------------
-// A wild row by one warp: sums of 2^((x - top) c), and the gradient.
-template <typename T>
-__device__ __noinline__ void dist_wild(const DistillArgs& a, int64_t r, DistillRow& row) {
-  const int lane = threadIdx.x & 31, V = (int)a.vocab, K = a.k;
-  const T* x = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
-  const float c = (float)(kLog2e64 * a.inv_t);
-  const int32_t* at = a.at + r * K;
-  // the place of id i among the row's, or -1
-  auto find = [&](int i) {
-    int lo = 0, hi = row.held;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (at[mid] < i) lo = mid + 1; else hi = mid;
-    }
-    return lo < row.held && at[lo] == i ? lo : -1;
-  };
-  double all = 0.0, rest = 0.0;
-  for (int i = lane; i < V; i += 32) {
-    const double e = (double)ex2_approx((RowVec<T>::get(x + i) - row.top) * c);
-    all += e;
-    rest += find(i) < 0 ? e : 0.0;
-  }
-  row.all = warp_sum64(all);
-  row.rest = warp_sum64(rest);
-  row.rho = 0.0;
-  if (!a.grad || (a.tail == PM_TAIL_DROP && row.mass == 0.0)) return;  // an empty row's gradient is 0 already
-  T* g = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
-  const double by = dist_by(a, r), on = by / row.all, off = on * dist_factor(a, row, row.rest, row.all);
-  for (int i = lane; i < V; i += 32) {
-    const double e = (double)ex2_approx((RowVec<T>::get(x + i) - row.top) * c);
-    const int k = find(i);
-    put_grad(g + i, k < 0 ? (float)(e * off) : (float)(e * on - a.p[r * K + k] * by));
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_distill_finish(DistillArgs a) {
-  __shared__ double scratch[kRowWarps];
-  __shared__ bool last;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.k;
-  const int64_t r = (int64_t)blockIdx.x * kRowWarps + warp;
-  cudaGridDependencySynchronize();
-  double l = 0.0;
-  if (r < a.rows && !(a.weights && a.weights[r] == 0.0f)) {
-    DistillRow row = a.row[r];
-    if (row.wild) dist_wild<T>(a, r, row);
-    const T* x = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
-    const ExpScale scale(a.inv_t);
-    const double top = (double)row.top;
-    // log of the sum of e^((x - top) / T)
-    const double logS = row.wild ? log(row.all)
-                                 : log(row.all) + (row.rho + top * (scale.exact - (double)scale.c)) * kLn264 - top * a.inv_t;
-    for (int k = lane; k < row.held; k += 32) {
-      const double p = a.p[r * K + k];
-      const double logq = ((double)RowVec<T>::get(x + a.at[r * K + k]) - top) * a.inv_t - logS;
-      if (p != 0.0) l -= p * logq;
-    }
-    l = warp_sum64(l) + row.shift;
-    if (a.tail == PM_TAIL_BUCKET && row.held < a.vocab) {
-      const double left = row.mass != row.mass ? row.mass : fmax(0.0, 1.0 - row.mass);
-      if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(row.rest, row.all)));
-    }
-    if (a.tail == PM_TAIL_DROP && row.mass == 0.0) l = 0.0;
-    if (a.weights) l *= (double)a.weights[r];
-  }
-  if (!a.loss) return;
-  if (a.each) {
-    if (r < a.rows && lane == 0) a.loss[r] = (float)l;
-    return;
-  }
-  if (r < a.rows && lane == 0) a.row_loss[r] = l;
-  // the last CTA adds the rows up, in an order of its own
-  __threadfence();
+  // the row's loss, and the last CTA's sum of all
+  if (rank != 0 || !a.loss) return;
+  l = warp_sum64(l);
+  if (lane == 0) sh.loss[warp] = l;
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+  if (tid == 0) {
+    for (int i = 1; i < kDistWarps; ++i) l += sh.loss[i];
+    if (a.each) {
+      a.loss[r] = (float)l;
+    } else {
+      a.row_loss[r] = l;
+      __threadfence();
+      sh.last = atomicAdd(a.ticket, 1u) == (unsigned)a.rows - 1u;
+    }
+  }
+  if (a.each) return;
   __syncthreads();
-  if (!last) return;
+  if (!sh.last) return;
   __threadfence();
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < a.rows; i += kRowThreads) s += __ldcg(a.row_loss + i);
-  s = block_add(s, scratch);
-  if (threadIdx.x == 0) {
+  for (int64_t i = tid; i < a.rows; i += kDistThreads) s += __ldcg(a.row_loss + i);
+  s = warp_sum64(s);
+  if (lane == 0) sh.loss[warp] = s;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < kDistWarps; ++i) s += sh.loss[i];
     if (a.mean) {
       const double by = a.weights ? *a.weight_sum : (double)a.rows;
       s = by != 0.0 ? s / by : 0.0;
@@ -691,28 +688,25 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
   pm::k_distill_prep<<<(unsigned)row_grid, pm::kRowThreads, 0, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // CTAs of a row: slices of at most kDistSlice bytes, or sixteen of them (a
-  // cluster beyond the portable eight, which sm_100 allows)
+  // CTAs of a row: as many as keep every SM's two, no more than it has tiles
   auto* kernel = pm::k_distill_rows<T>;
   constexpr int n = pm::RowVec<T>::n;
   const int64_t granules = (a.vocab + n - 1) / n + 1;  // one more where a row starts off a boundary
+  const int64_t tiles = (granules + pm::kDistTile - 1) / pm::kDistTile;
   int split = 1;
-  while (split < pm::kDistSplit && (granules + split - 1) / split * 16 > pm::kDistSlice) split *= 2;
-  auto bytes = [](int64_t per) {
-    const int64_t steps = (per + pm::kDistStride - 1) / pm::kDistStride;
-    return sizeof(pm::DistillShared) + (size_t)per * 16 + (size_t)steps * pm::kDistThreads * 4;
+  while (split < pm::kDistSplit && 2 * split <= tiles && a.rows * 2 * split <= (int64_t)pmh::num_sms() * pm::kDistResident)
+    split *= 2;
+  auto bytes = [](int64_t tiles) {
+    return sizeof(pm::DistillShared) + (size_t)pm::kDistWarps * pm::kDistStages * pm::kDistChunk * 16 +
+           (size_t)tiles * pm::kDistThreads * 4;
   };
   static pmh::DeviceOnce once;
   once([&] {
-    const int64_t widest = (pm::kDistVocab / n + 1) / pm::kDistSplit + 1, wanted = pm::kDistSlice / 16;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)bytes(widest > wanted ? widest : wanted));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+                             (int)bytes(pm::kDistVocab / n / pm::kDistTile + 1));
   });
   if (e != cudaSuccess) return e;
-  e = launch_after(kernel, a.rows * split, pm::kDistThreads, bytes((granules + split - 1) / split), split, st, a);
-  if (e != cudaSuccess) return e;
-  return launch_after(pm::k_distill_finish<T>, row_grid, pm::kRowThreads, 0, 1, st, a);
+  return launch_after(kernel, a.rows * split, pm::kDistThreads, bytes((tiles + split - 1) / split), split, st, a);
 }
 
 }  // namespace
