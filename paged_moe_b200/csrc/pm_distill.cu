@@ -69,10 +69,12 @@ struct DistillArgs {
   void* grad;                // or NULL
   int64_t grad_stride;
   const float* grad_loss;
+  bool vectors;              // row 0 of the gradient lies as the logits' does
+  int mark_tiles;            // tiles that there are marks for
   // workspace
   double* weight_sum;
   unsigned* ticket;
-  double* row_loss;          // [rows]
+  double* row_loss;          // [CTAs or clusters]
   DistillRow* row;           // [rows]
   double* p;                 // [rows, k] probabilities by id
   int32_t* at;               // [rows, k] the ids, ascending
@@ -219,7 +221,7 @@ struct DistillSum {
 struct alignas(16) DistillShared {
   uint64_t bar[kDistWarps][kDistStages];
   DistillPart warps[kDistWarps];
-  DistillPart parts[2][kDistSplit];  // of the first join, and of a wild row's
+  DistillPart parts[2][kDistSplit];  // of one join and of the next
   double loss[kDistWarps];
   int last;
   // then the rings, and a word of marks per tile and thread: bit u n + e is
@@ -269,7 +271,7 @@ __device__ __forceinline__ DistillPart dist_reduce(DistillPart p) {
 }
 
 // The row's part from its warps', through the cluster; every thread gets it.
-__device__ __noinline__ DistillPart dist_join(DistillShared& sh, DistillPart part, int again, uint32_t rank,
+__device__ __noinline__ DistillPart dist_join(DistillShared& sh, DistillPart part, int joins, uint32_t rank,
                                               uint32_t split) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const DistillPart none = {0.0, 0.0, kNegInf64, kNegInf, 0};
@@ -281,14 +283,14 @@ __device__ __noinline__ DistillPart dist_join(DistillShared& sh, DistillPart par
     __syncthreads();
     return part;
   }
-  if (again == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
+  if (joins == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
   if (warp == 0) {
     part = dist_reduce(lane < kDistWarps ? sh.warps[lane] : none);
-    if (lane < (int)split) *dist_of(&sh.parts[again][rank], lane) = part;
+    if (lane < (int)split) *dist_of(&sh.parts[joins & 1][rank], lane) = part;
   }
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  return dist_reduce(lane < (int)split ? sh.parts[again][lane] : none);
+  return dist_reduce(lane < (int)split ? sh.parts[joins & 1][lane] : none);
 }
 
 // What multiplies a row's gradient: weight, temperature, reduction and the
@@ -349,81 +351,109 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   constexpr uint32_t kBits = (1u << n) - 1u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = dist_rank(), split = dist_split();
-  const int64_t r = blockIdx.x / split;
   const int V = (int)a.vocab, K = a.k;
-  const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
-  T* grow = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
-  const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);  // elements before the row in granule 0
-  const bool vectors = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
-  // the part: granules [g0, g0 + count) of the row's, whole tiles but the last
-  const int granules = (off + V + n - 1) / n;
-  const int per = ((granules + kDistTile - 1) / kDistTile + (int)split - 1) / (int)split * kDistTile;
-  const int g0 = (int)rank * per < granules ? (int)rank * per : granules;
-  const int count = granules - g0 < per ? granules - g0 : per;
-  const int first = g0 * n - off;  // the part's first element
-  // granules wholly inside the row; one at each end may not be
-  const int whole0 = first < 0 ? 1 : 0, whole1 = first + count * n > V ? count - 1 : count;
-  uint4* out = reinterpret_cast<uint4*>(grow + first);
-  auto singly = [&](int j, const float (&v)[n]) {
-    for (int e = 0; e < n; ++e) {
-      const int i = first + j * n + e;
-      if (i >= 0 && i < V) put_grad(grow + i, v[e]);
-    }
-  };
-  auto zeros = [&]() {
-    const float zero[n] = {};
-    for (int j = tid; j < count; j += kDistThreads) {
-      if (vectors && j >= whole0 && j < whole1) __stcs(out + j, make_uint4(0, 0, 0, 0));
-      else singly(j, zero);
-    }
-  };
-  double l = 0.0;  // of the thread's entry, then the row's
-  // a row of weight 0 is not read; the whole cluster knows
-  const bool skip = a.weights && a.weights[r] == 0.0f;
-  if (skip) {
-    if (a.grad) zeros();
-    cudaGridDependencySynchronize();
-  } else {
-    // the warp's chunks: forward, and for the gradient back again
-    unsigned char* ring = reinterpret_cast<unsigned char*>(&sh + 1) + warp * kDistStages * kDistChunk * 16;
-    uint32_t* marks = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned char*>(&sh + 1) +
-                                                  kDistWarps * kDistStages * kDistChunk * 16);
-    uint64_t* bar = sh.bar[warp];
-    const int chunks = (count - warp * kDistChunk + kDistTile - 1) / kDistTile > 0
-                           ? (count - warp * kDistChunk + kDistTile - 1) / kDistTile : 0;
-    const int copies = a.grad ? 2 * chunks : chunks;
-    const char* src = reinterpret_cast<const char*>(row - off) + ((int64_t)g0 + warp * kDistChunk) * 16;
-    auto issue = [&](int q, int st) {
-      if (q >= copies) return;
-      const int t = q < chunks ? q : 2 * chunks - 1 - q;
-      const int left = count - warp * kDistChunk - t * kDistTile;
-      const uint32_t bytes = (uint32_t)(left < kDistChunk ? left : kDistChunk) * 16;
-      mbar_arrive_expect_tx(&bar[st], bytes);
-      bulk_copy_g2s_plain(ring + st * kDistChunk * 16, src + (int64_t)t * kDistTile * 16, bytes, &bar[st]);
-    };
-    if (lane == 0) {
-#pragma unroll
-      for (int st = 0; st < kDistStages; ++st) mbar_init(&bar[st], 1);
-      fence_proxy_async_smem();
-#pragma unroll
-      for (int st = 0; st < kDistStages; ++st) issue(st, st);
-    }
-    // waited for before the first store into another CTA
-    if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    const int tiles = (count + kDistTile - 1) / kDistTile;
-    for (int i = tid; i < tiles * kDistThreads; i += kDistThreads) marks[i] = 0;
-    const int id = tid < K ? a.ids[r * K + tid] : -1;
-    __syncthreads();
-    if (id >= 0 && id < V && id >= first && id < first + count * n) {
-      const int j = (id - first) / n, e = (id - first) % n, u = j % kDistChunk / 32;
-      atomicOr(&marks[j / kDistTile * kDistThreads + j % kDistTile / kDistChunk * 32 + j % 32], 1u << (u * n + e));
-    }
-    __syncthreads();
+  const int rows = (int)a.rows, row0 = (int)(blockIdx.x / split), row_step = (int)(gridDim.x / split);
+  const bool bucket = a.tail == PM_TAIL_BUCKET;
+  const float c = (float)(kLog2e64 * a.inv_t);
+  const uint64_t c2 = pk(c, c);
+  unsigned char* ring = reinterpret_cast<unsigned char*>(&sh + 1) + warp * kDistStages * kDistChunk * 16;
+  uint32_t* marks = reinterpret_cast<uint32_t*>(reinterpret_cast<unsigned char*>(&sh + 1) +
+                                                kDistWarps * kDistStages * kDistChunk * 16);
+  uint64_t* bar = sh.bar[warp];
 
+  // The part of a row: granules [g0, g0 + count) of its own, whole tiles but
+  // the last; the first may hold elements before the row, the last behind it.
+  struct Part {
+    int off, count, first, whole0, whole1, chunks;
+  };
+  auto part_of = [&](int r) {
+    Part p;
+    const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
+    p.off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);
+    const int granules = (p.off + V + n - 1) / n;
+    int per = granules, g0 = 0;
+    if (split > 1) {
+      per = ((granules + kDistTile - 1) / kDistTile + (int)split - 1) / (int)split * kDistTile;
+      g0 = (int)rank * per < granules ? (int)rank * per : granules;
+    }
+    p.count = granules - g0 < per ? granules - g0 : per;
+    p.first = g0 * n - p.off;
+    p.whole0 = p.first < 0 ? 1 : 0;
+    p.whole1 = p.first + p.count * n > V ? p.count - 1 : p.count;
+    const int left = p.count - warp * kDistChunk + kDistTile - 1;
+    p.chunks = left > 0 ? left / kDistTile : 0;
+    return p;
+  };
+  // a row of weight 0 is not read; the whole cluster knows
+  auto skipped = [&](int r) { return a.weights && a.weights[r] == 0.0f; };
+  auto next_of = [&](int r) {
+    r += row_step;
+    while (r < rows && skipped(r)) r += row_step;
+    return r;
+  };
+  auto zeros = [&](int r, const Part& p) {
+    T* grow = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
+    const bool vectors = (a.row_stride - a.grad_stride) * (int64_t)sizeof(T) * r % 16 == 0 && a.vectors;
+    for (int j = tid; j < p.count; j += kDistThreads) {
+      if (vectors && j >= p.whole0 && j < p.whole1) {
+        __stcs(reinterpret_cast<uint4*>(grow + p.first) + j, make_uint4(0, 0, 0, 0));
+      } else {
+        for (int i = p.first + j * n; i < p.first + j * n + n; ++i)
+          if (i >= 0 && i < V) put_grad(grow + i, 0.0f);
+      }
+    }
+  };
+
+  // The warp's copies, first lane only: the chunks of a row forward, for the
+  // gradient back again, then those of the next row.
+  int ir = row0 - row_step;  // the row that copies are issued for
+  int iq = 0, icopies = 0, ichunks = 0;
+  const char* isrc = nullptr;
+  int ileft = 0;
+  auto issue = [&](int st) {
+    while (iq == icopies) {
+      ir = next_of(ir);
+      if (ir >= rows) { ir = rows; iq = icopies = 0; return; }
+      const Part p = part_of(ir);
+      ichunks = p.chunks;
+      icopies = a.grad ? 2 * p.chunks : p.chunks;
+      isrc = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.logits) + ir * a.row_stride + p.first) +
+             warp * kDistChunk * 16;
+      ileft = p.count - warp * kDistChunk;
+      iq = 0;
+    }
+    const int t = iq < ichunks ? iq : 2 * ichunks - 1 - iq;
+    ++iq;
+    const int left = ileft - t * kDistTile;
+    const uint32_t bytes = (uint32_t)(left < kDistChunk ? left : kDistChunk) * 16;
+    mbar_arrive_expect_tx(&bar[st], bytes);
+    bulk_copy_g2s_plain(ring + st * kDistChunk * 16, isrc + (int64_t)t * kDistTile * 16, bytes, &bar[st]);
+  };
+  if (lane == 0) {
+#pragma unroll
+    for (int st = 0; st < kDistStages; ++st) mbar_init(&bar[st], 1);
+    fence_proxy_async_smem();
+#pragma unroll
+    for (int st = 0; st < kDistStages; ++st) issue(st);
+  }
+  // waited for before the first store into another CTA
+  if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (bucket) {
+    for (int i = tid; i < a.mark_tiles * kDistThreads; i += kDistThreads) marks[i] = 0;
+  }
+  if (a.grad && a.weights)
+    for (int r = row0; r < rows; r += row_step)
+      if (skipped(r)) zeros(r, part_of(r));
+  __syncthreads();
+
+  int st = 0, joins = 0;
+  uint32_t parity = 0;
+  bool lost = false;
+  double loss = 0.0;  // of this thread's entries of all the CTA's rows
+  for (int r = next_of(row0 - row_step); r < rows; r = next_of(r)) {
+    const Part p = part_of(r);
+    const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
     // a copy's vectors, -inf in the granules' parts outside the row
-    int st = 0, q = 0;
-    uint32_t parity = 0;
-    bool lost = false;
     auto take = [&](uint4 (&raw)[kDistStep], int j0) {
       lost = !__all_sync(kFull, mbar_wait(&bar[st], parity)) || lost;
       const uint4* from = reinterpret_cast<const uint4*>(ring + st * kDistChunk * 16) + lane;
@@ -432,34 +462,46 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       __syncwarp();
       if (lane == 0) {
         fence_proxy_async_smem();
-        issue(q + kDistStages, st);
+        issue(st);
       }
-      ++q;
       if (++st == kDistStages) { st = 0; parity ^= 1; }
-      if (j0 < whole0 || j0 + kDistChunk > whole1) {
+    };
+
+    if (bucket) {
+      const int id = tid < K ? a.ids[(int64_t)r * K + tid] : -1;
+      const int i = id - p.first;
+      if (id >= 0 && id < V && i >= 0 && i < p.count * n) {
+        const int j = i / n, u = j % kDistChunk / 32;
+        atomicOr(&marks[j / kDistTile * kDistThreads + j % kDistTile / kDistChunk * 32 + j % 32], 1u << (u * n + i % n));
+      }
+      __syncthreads();
+    }
+
+    // forward: sums over all tokens and over the unmarked ones
+    DistillSum sums = {0.0, 0.0, StepSum::kNothing};
+    float m = kNegInf;
+    int flags = 0;
+    for (int t = 0; t < p.chunks; ++t) {
+      uint32_t marked = 0;
+      if (bucket) {
+        marked = marks[t * kDistThreads + tid];
+        if (marked) marks[t * kDistThreads + tid] = 0;  // for the next row
+      }
+      const int j0 = t * kDistTile + warp * kDistChunk;
+      uint4 raw[kDistStep];
+      take(raw, j0);
+      if (j0 < p.whole0 || j0 + kDistChunk > p.whole1) {
 #pragma unroll
         for (int u = 0; u < kDistStep; ++u) {
           uint32_t in = 0;
 #pragma unroll
           for (int e = 0; e < n; ++e) {
-            const int i = first + (j0 + u * 32 + lane) * n + e;
+            const int i = p.first + (j0 + u * 32 + lane) * n + e;
             in |= i >= 0 && i < V ? 1u << e : 0u;
           }
           raw[u] = RowVec<T>::select(raw[u], in);
         }
       }
-    };
-
-    // forward: sums over all tokens and over the unmarked ones
-    const float c = (float)(kLog2e64 * a.inv_t);
-    const uint64_t c2 = pk(c, c);
-    DistillSum sums = {0.0, 0.0, StepSum::kNothing};
-    float m = kNegInf;
-    int flags = 0;
-    for (int t = 0; t < chunks; ++t) {
-      const uint32_t marked = marks[t * kDistThreads + tid];
-      uint4 raw[kDistStep];
-      take(raw, t * kDistTile + warp * kDistChunk);
       const float tm = max_nan(max_nan(RowVec<T>::largest(raw[0]), RowVec<T>::largest(raw[1])),
                                RowVec<T>::largest(raw[2]), RowVec<T>::largest(raw[3]));
       m = fmaxf(m, tm);
@@ -502,133 +544,159 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       }
     }
     if (lost) sums.all = sums.rest = nan64();
-    DistillPart part = {sums.all, sums.rest, sums.rho > StepSum::kNothing ? (double)sums.rho : kNegInf64, m, flags};
-    part = dist_join(sh, part, 0, rank, split);
-    cudaGridDependencySynchronize();  // the entries, and the sum of the weights
+    if (joins == 0) cudaGridDependencySynchronize();  // the entries, and the sum of the weights
+    // this thread's entry and the row's factors, on their way during the join
     const DistillRow known = a.row[r];
+    int id = -1;
+    double prob = 0.0;
+    float x_id = 0.0f;
+    if (tid < known.held) {
+      id = a.at[(int64_t)r * K + tid];
+      prob = a.p[(int64_t)r * K + tid];
+      x_id = RowVec<T>::get(row + id);
+    }
+    const double by = dist_by(a, r);
+    DistillPart part = {sums.all, sums.rest, sums.rho > StepSum::kNothing ? (double)sums.rho : kNegInf64, m, flags};
+    part = dist_join(sh, part, joins, rank, split);
+    ++joins;
     const float top = part.top;
     const bool wild = ((part.flags & kPartHigh) || ((part.flags & kPartLow) && !(top * c > -kWildExponent + 4096.0f))) &&
                       part.all == part.all;
-    const int i0 = first > 0 ? first : 0, i1 = first + count * n < V ? first + count * n : V;
+    const int i0 = p.first > 0 ? p.first : 0, i1 = p.first + p.count * n < V ? p.first + p.count * n : V;
     if (wild) {
       double all = 0.0, rest = 0.0;
       dist_wild<T>(a, r, i0, i1, top, 0.0, 0.0, 0.0, false, &all, &rest);
       part = {all, rest, 0.0, top, 0};
-      part = dist_join(sh, part, 1, rank, split);
+      part = dist_join(sh, part, joins, rank, split);
+      ++joins;
     }
     // no finite logit: no distribution
     const double all = top == kNegInf ? nan64() : part.all;
-    const bool empty = a.tail == PM_TAIL_DROP && known.mass == 0.0;
-
-    // the loss: this thread's entry
-    if (rank == 0 && a.loss) {
-      // log of the sum of e^((x - top) / T)
-      const double exact = kLog2e64 * a.inv_t;
-      const double logS = wild ? log(all) : log(all) + (part.rho + (double)top * (exact - (double)c)) * kLn264 - (double)top * a.inv_t;
-      if (tid < known.held && !empty) {
-        const double p = a.p[r * K + tid];
-        const double logq = ((double)RowVec<T>::get(row + a.at[r * K + tid]) - (double)top) * a.inv_t - logS;
-        if (p != 0.0) l = -p * logq;
-      }
-      if (tid == 0 && !empty) {
-        l += known.shift;
-        if (a.tail == PM_TAIL_BUCKET && known.held < a.vocab) {
-          const double left = known.mass != known.mass ? known.mass : fmax(0.0, 1.0 - known.mass);
-          if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(part.rest, all)));
-        }
-      }
-      if (a.weights) l *= (double)a.weights[r];
-    }
+    const bool empty = !bucket && known.mass == 0.0;
 
     if (a.grad) {
-      const double by = dist_by(a, r), on = by / all, factor = on * dist_factor(a, known, part.rest, all);
+      T* grow = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
+      const bool vectors = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
+      uint4* out = reinterpret_cast<uint4*>(grow + p.first);
+      const double on = by / all, factor = on * dist_factor(a, known, part.rest, all);
       if (wild || empty) {
-        // the copies that were on their way are not wanted
-        for (; q < copies && q < chunks + kDistStages; ++q) {
-          mbar_wait(&bar[st], parity);
-          if (++st == kDistStages) { st = 0; parity ^= 1; }
-        }
+        // the copies are not wanted, but others follow them
+        uint4 raw[kDistStep];
+        for (int t = 0; t < p.chunks; ++t) take(raw, 0);
         if (empty) {
-          zeros();
+          zeros(r, p);
         } else {
           double s0 = 0.0, s1 = 0.0;
           dist_wild<T>(a, r, i0, i1, top, on, factor, by, true, &s0, &s1);
         }
       } else {
-        const float R = (float)part.rho, f = (float)factor;
-        const uint64_t r2 = pk(-R, -R), f2 = pk(f, f);
-        for (int t = chunks - 1; t >= 0; --t) {
-          uint32_t marked = marks[t * kDistThreads + tid];
+        const float f = (float)factor;
+        const uint64_t r2 = pk(-(float)part.rho, -(float)part.rho), f2 = pk(f, f);
+        for (int t = p.chunks - 1; t >= 0; --t) {
           const int j0 = t * kDistTile + warp * kDistChunk;
+          const bool whole = vectors && j0 >= p.whole0 && j0 + kDistChunk <= p.whole1;
           uint4 raw[kDistStep];
           take(raw, j0);
 #pragma unroll
           for (int u = 0; u < kDistStep; ++u) {
-            float v[n], g[n];
+            float v[n];
             RowVec<T>::unpack(raw[u], v);
 #pragma unroll
             for (int e = 0; e < n; e += 2) {
               const uint64_t x = fma2(pk(v[e], v[e + 1]), c2, r2);
-              v[e] = ex2_approx(lo_f(x));
-              v[e + 1] = ex2_approx(hi_f(x));
-              const uint64_t y = mul2(pk(v[e], v[e + 1]), f2);
-              g[e] = lo_f(y);
-              g[e + 1] = hi_f(y);
+              const uint64_t y = mul2(pk(ex2_approx(lo_f(x)), ex2_approx(hi_f(x))), f2);
+              v[e] = lo_f(y);
+              v[e + 1] = hi_f(y);
             }
             const int j = j0 + u * 32 + lane;
-            if ((marked >> (u * n)) & kBits) {
-              // the entries from this vector's first element on
-              const int i = first + j * n;
-              int lo = 0, hi = known.held;
-              while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (a.at[r * K + mid] < i) lo = mid + 1; else hi = mid;
-              }
-              for (; lo < known.held && a.at[r * K + lo] < i + n; ++lo) {
-                const int e = a.at[r * K + lo] - i;
-                const double z = a.p[r * K + lo] * by;
+            if (whole || (vectors && j >= p.whole0 && j < p.whole1)) {
+              __stcs(out + j, pack_grad(v));
+            } else if (j < p.count) {
 #pragma unroll
-                for (int d = 0; d < n; ++d)
-                  if (d == e) g[d] = (float)((double)v[d] * on - z);  // one rounding of the difference
+              for (int e = 0; e < n; ++e) {
+                const int i = p.first + j * n + e;
+                if (i >= 0 && i < V) put_grad(grow + i, v[e]);
               }
             }
-            if (vectors && j >= whole0 && j < whole1) __stcs(out + j, pack_grad(g));
-            else if (j < count) singly(j, g);
           }
+        }
+        // the entries' elements once more, q - p, behind the CTA's own stores
+        __syncthreads();
+        if (id >= 0 && id >= i0 && id < i1) {
+          const double q = (double)ex2_approx(fmaf(x_id, c, -(float)part.rho));
+          put_grad(grow + id, (float)(q * on - prob * by));
         }
       }
     }
+
+    // the loss: this thread's entry
+    if (rank == 0 && a.loss) {
+      double l = 0.0;
+      if (!empty) {
+        if (prob != 0.0 || tid == 0) {
+          // log of the sum of e^((x - top) / T)
+          const double logS = wild ? log(all)
+                                   : log(all) + (part.rho + (double)top * (kLog2e64 * a.inv_t - (double)c)) * kLn264 -
+                                         (double)top * a.inv_t;
+          if (prob != 0.0) l = -prob * (((double)x_id - (double)top) * a.inv_t - logS);
+        }
+        if (tid == 0) {
+          l += known.shift;
+          if (bucket && known.held < V) {
+            const double left = known.mass != known.mass ? known.mass : fmax(0.0, 1.0 - known.mass);
+            if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(part.rest, all)));
+          }
+        }
+        if (a.weights) l *= (double)a.weights[r];
+      }
+      loss += l;
+      if (a.each) {
+        l = warp_sum64(l);
+        if (lane == 0) sh.loss[warp] = l;
+        __syncthreads();
+        if (tid == 0) {
+          for (int i = 1; i < kDistWarps; ++i) l += sh.loss[i];
+          a.loss[r] = (float)l;
+        }
+      }
+    }
+    if (bucket) __syncthreads();  // the marks are clear
+  }
+  if (joins == 0) {
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cudaGridDependencySynchronize();
+  }
+  if (rank != 0 || !a.loss) return;
+  if (a.each) {
+    for (int r = row0 + tid * row_step; r < rows; r += kDistThreads * row_step)
+      if (skipped(r)) a.loss[r] = 0.0f;
+    return;
   }
 
-  // the row's loss, and the last CTA's sum of all
-  if (rank != 0 || !a.loss) return;
-  l = warp_sum64(l);
-  if (lane == 0) sh.loss[warp] = l;
+  // the CTA's loss, and the last CTA's sum of all
+  loss = warp_sum64(loss);
+  __syncthreads();
+  if (lane == 0) sh.loss[warp] = loss;
   __syncthreads();
   if (tid == 0) {
-    for (int i = 1; i < kDistWarps; ++i) l += sh.loss[i];
-    if (a.each) {
-      a.loss[r] = (float)l;
-    } else {
-      a.row_loss[r] = l;
-      __threadfence();
-      sh.last = atomicAdd(a.ticket, 1u) == (unsigned)a.rows - 1u;
-    }
+    for (int i = 1; i < kDistWarps; ++i) loss += sh.loss[i];
+    a.row_loss[row0] = loss;
+    __threadfence();
+    sh.last = atomicAdd(a.ticket, 1u) == (unsigned)row_step - 1u;
   }
-  if (a.each) return;
   __syncthreads();
   if (!sh.last) return;
   __threadfence();
   double s = 0.0;
-  for (int64_t i = tid; i < a.rows; i += kDistThreads) s += __ldcg(a.row_loss + i);
+  for (int i = tid; i < row_step; i += kDistThreads) s += __ldcg(a.row_loss + i);
   s = warp_sum64(s);
   if (lane == 0) sh.loss[warp] = s;
   __syncthreads();
   if (tid == 0) {
     for (int i = 1; i < kDistWarps; ++i) s += sh.loss[i];
     if (a.mean) {
-      const double by = a.weights ? *a.weight_sum : (double)a.rows;
-      s = by != 0.0 ? s / by : 0.0;
+      const double weights = a.weights ? *a.weight_sum : (double)a.rows;
+      s = weights != 0.0 ? s / weights : 0.0;
     }
     *a.loss = (float)s;
   }
@@ -693,9 +761,10 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
   constexpr int n = pm::RowVec<T>::n;
   const int64_t granules = (a.vocab + n - 1) / n + 1;  // one more where a row starts off a boundary
   const int64_t tiles = (granules + pm::kDistTile - 1) / pm::kDistTile;
+  const int64_t slots = (int64_t)pmh::num_sms() * pm::kDistResident;
   int split = 1;
-  while (split < pm::kDistSplit && 2 * split <= tiles && a.rows * 2 * split <= (int64_t)pmh::num_sms() * pm::kDistResident)
-    split *= 2;
+  while (split < pm::kDistSplit && 2 * split <= tiles && a.rows * 2 * split <= slots) split *= 2;
+  const int64_t mark_tiles = (tiles + split - 1) / split;
   auto bytes = [](int64_t tiles) {
     return sizeof(pm::DistillShared) + (size_t)pm::kDistWarps * pm::kDistStages * pm::kDistChunk * 16 +
            (size_t)tiles * pm::kDistThreads * 4;
@@ -706,7 +775,12 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
                              (int)bytes(pm::kDistVocab / n / pm::kDistTile + 1));
   });
   if (e != cudaSuccess) return e;
-  return launch_after(kernel, a.rows * split, pm::kDistThreads, bytes((tiles + split - 1) / split), split, st, a);
+  pm::DistillArgs b = a;
+  b.vectors = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
+  b.mark_tiles = (int)mark_tiles;
+  const int64_t clusters = a.rows < slots / split ? a.rows : slots / split;
+  return launch_after(kernel, clusters * split, pm::kDistThreads, bytes(a.tail == PM_TAIL_BUCKET ? mark_tiles : 0), split,
+                      st, b);
 }
 
 }  // namespace
