@@ -2,19 +2,20 @@
 // and its gradient.  Two kernels:
 //
 // k_distill_prep, a warp per row: the row's entries become probabilities in
-//   64 bits (the mass they leave is a difference of nearly equal numbers),
-//   sorted by id, the entries of one id added up.
-// k_distill_rows, a CTA per row, or a cluster where there are few rows.  Every
-//   warp streams its chunks through a ring in shared memory that its first
-//   lane keeps full with bulk copies: once forward for two sums of e^(x / T),
-//   over all tokens and over those that are no entries (again no difference
-//   of nearly equal numbers), and once more, backward, for the gradient,
-//   e^(x / T) times one factor per row, and on entries q - p.  The second
-//   time the logits come from L2: two rows an SM are in work, 95 MB at 320 KB
-//   a row, of which half is still wanted on average; what was read last is
-//   read first, and the gradients are stored as data that nobody reads soon.
-//   So device memory sees each logit once and each gradient once.  The last
-//   CTA to end adds the rows' losses up in a fixed order.
+//   64 bits (the mass they leave is a difference of nearly equal numbers), the
+//   entries of one id added up, next to their logits.
+// k_distill_rows, two CTAs per SM that take row after row, or a cluster per
+//   row where there are few.  Every warp streams its chunks through a ring in
+//   shared memory that its first lane keeps full with bulk copies: once forward
+//   for two sums of e^(x / T), over all tokens and over those that are no
+//   entries (again no difference of nearly equal numbers), and once more,
+//   backward, for the gradient, e^(x / T) times one factor per row.  The
+//   entries' elements are written once more behind it, q - p.  The second time
+//   the logits come from L2: 95 MB are in work at 320 KB a row, of which half
+//   is still wanted on average; what was read last is read first, the first
+//   reading asks L2 to keep the data and the second and the stores to let go of
+//   it.  The last CTA to end computes the rows' losses from their sums and adds
+//   them up in a fixed order.
 //
 // Memory is cut at 16-byte boundaries: granule j of a row holds the elements
 // whose bytes share the j-th aligned 16 bytes.  The gradient's rows start as
@@ -34,7 +35,7 @@
 
 namespace pm {
 
-constexpr int kDistThreads = 512;
+constexpr int kDistThreads = 384;
 constexpr int kDistWarps = kDistThreads / 32;
 constexpr int kDistResident = 2;               // CTAs of an SM
 constexpr int kDistMax = 256;                  // largest k
@@ -44,17 +45,22 @@ constexpr int kDistSplit = 8;                  // most CTAs of a row
 constexpr int kDistStep = 4;                   // vectors of a lane in a chunk
 constexpr int kDistChunk = 32 * kDistStep;     // granules of a warp's chunk, a stage of its ring
 constexpr int kDistTile = kDistWarps * kDistChunk;
-constexpr int kDistStages = 2;
+constexpr int kDistStages = 3;
 constexpr int kRowThreads = 256;               // of the two kernels with a warp per row
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr double kTailFloor = 0x1p-100;        // smallest tail mass of the student that is told apart
 
-// What the kernels know of a row.
+// What the kernels know of a row.  The teacher's:
 struct DistillRow {
   double mass;     // of its entries, 1 for PM_TAIL_DROP, 0 where they have none
-  double shift;    // sum of p log p over the entries as they were given
-  int held;        // ids
-  int pad;
+  double entropy;  // sum of p log p over the entries as they were given
+  double lean;     // sum of p (x - ref) over their logits
+  float ref;       // the largest of these
+  int held;        // distinct ids
+  // the student's, from k_distill_rows
+  double all, rest, rho;  // sums, as multiples of 2^rho
+  float top;       // the largest logit
+  int wild;        // the sums are multiples of 2^(top c), not of 2^rho
 };
 
 struct DistillArgs {
@@ -74,20 +80,13 @@ struct DistillArgs {
   // workspace
   double* weight_sum;
   unsigned* ticket;
-  double* row_loss;          // [CTAs or clusters]
   DistillRow* row;           // [rows]
-  double* p;                 // [rows, k] probabilities by id
-  int32_t* at;               // [rows, k] the ids, ascending
+  double* p;                 // [rows, k] probabilities, at an id's first entry those of all
+  int32_t* at;               // [rows, k] ids; -1: no entry, or not an id's first
+  float* x;                  // [rows, k] their logits
 };
 
-__device__ __forceinline__ double block_add(double v, double* scratch) {
-  v = warp_sum64(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return warp_sum64((threadIdx.x & 31) < kRowWarps ? scratch[threadIdx.x & 31] : 0.0);
-}
-
+template <typename T>
 __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
   __shared__ int s_id[kRowWarps][kDistMax];
   __shared__ double s_p[kRowWarps][kDistMax];
@@ -99,33 +98,41 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
     if (a.mean && a.weights) {
       double s = 0.0;
       for (int64_t i = threadIdx.x; i < a.rows; i += kRowThreads) s += (double)a.weights[i];
-      s = block_add(s, scratch);
-      if (threadIdx.x == 0) *a.weight_sum = s;
+      s = warp_sum64(s);
+      if (lane == 0) scratch[warp] = s;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int i = 1; i < kRowWarps; ++i) s += scratch[i];
+        *a.weight_sum = s;
+      }
     }
   }
   const int64_t r = (int64_t)blockIdx.x * kRowWarps + warp;
   if (r >= a.rows || (a.weights && a.weights[r] == 0.0f)) return;
+  const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
   int id[kDistHeld];
-  double lp[kDistHeld], p[kDistHeld];
+  float lp[kDistHeld], x[kDistHeld];
   float top = kNegInf;
 #pragma unroll
   for (int i = 0; i < kDistHeld; ++i) {
-    const int k = i * 32 + lane;
     id[i] = -1;
-    lp[i] = kNegInf64;
-    if (k < K) {
-      id[i] = a.ids[r * K + k];
-      lp[i] = (double)a.logprobs[r * K + k];
+    lp[i] = kNegInf;
+    if (i * 32 + lane < K) {
+      id[i] = a.ids[r * K + i * 32 + lane];
+      lp[i] = a.logprobs[r * K + i * 32 + lane];
     }
     if (id[i] < 0 || id[i] >= V) id[i] = -1;
-    else top = fmaxf(top, lp[i] == lp[i] ? (float)lp[i] : -kNegInf);
+    else top = fmaxf(top, lp[i] == lp[i] ? lp[i] : -kNegInf);
   }
+#pragma unroll
+  for (int i = 0; i < kDistHeld; ++i) x[i] = id[i] >= 0 ? RowVec<T>::get(row + id[i]) : kNegInf;
   // raw logits are as good as log-probabilities for PM_TAIL_DROP: the largest first
   const double most = a.tail == PM_TAIL_DROP ? (double)warp_max_ordered(top) : 0.0;
-  double total = 0.0;
+  double p[kDistHeld], total = 0.0;
 #pragma unroll
   for (int i = 0; i < kDistHeld; ++i) {
-    p[i] = id[i] >= 0 && most > kNegInf64 ? exp(lp[i] - most) : 0.0;
+    p[i] = 0.0;
+    if (i * 32 < K) p[i] = id[i] >= 0 && most > kNegInf64 ? exp((double)lp[i] - most) : 0.0;
     total += p[i];
   }
   total = warp_sum64(total);
@@ -136,56 +143,62 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
     shift = mass ? most + log(total) : 0.0;
     total = mass ? 1.0 : 0.0;
   }
-  double entropy = 0.0;
+  // the largest of the entries' logits that weigh anything
+  float ref = kNegInf;
 #pragma unroll
   for (int i = 0; i < kDistHeld; ++i) {
     p[i] *= by;
-    if (p[i] != 0.0) entropy += p[i] * (lp[i] - shift);
-    if (i * 32 + lane < K) {
-      s_id[warp][i * 32 + lane] = id[i];
-      s_p[warp][i * 32 + lane] = p[i];
+    if (p[i] != 0.0) ref = fmaxf(ref, x[i]);
+  }
+  ref = warp_max_ordered(ref);
+  if (ref == kNegInf) ref = 0.0f;
+  double entropy = 0.0, lean = 0.0;
+#pragma unroll
+  for (int i = 0; i < kDistHeld; ++i) {
+    if (i * 32 >= K) break;
+    if (p[i] != 0.0) {
+      entropy += p[i] * ((double)lp[i] - shift);
+      lean += p[i] * ((double)x[i] - (double)ref);
     }
+    s_id[warp][i * 32 + lane] = id[i];
+    s_p[warp][i * 32 + lane] = p[i];
   }
   entropy = warp_sum64(entropy);
+  lean = warp_sum64(lean);
   __syncwarp();
-  // an id's place is the number of distinct smaller ids; its first entry takes it, with the sum of all
+  // an id's first entry takes the sum of all
   int held = 0;
+#pragma unroll 4
+  for (int j = 0; j < K; ++j) {
+    const int other = s_id[warp][j];
+    const double more = s_p[warp][j];
 #pragma unroll
-  for (int i = 0; i < kDistHeld; ++i) {
-    if (i * 32 >= K) break;
-    const int k = i * 32 + lane;
-    bool first = id[i] >= 0;
-    for (int j = 0; j < k && j < K; ++j) first = first && s_id[warp][j] != id[i];
-    if (first) {
-      double all = p[i];
-      for (int j = k + 1; j < K; ++j)
-        if (s_id[warp][j] == id[i]) all += s_p[warp][j];
-      p[i] = all;
-    } else {
-      id[i] = -1;
+    for (int i = 0; i < kDistHeld; ++i) {
+      const int k = i * 32 + lane;
+      if (i * 32 >= K) break;
+      if (other == id[i] && other >= 0) {
+        if (j > k) p[i] += more;
+        else if (j < k) id[i] = -1;
+      }
     }
-    held += __popc(__ballot_sync(kFull, first));
   }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < kDistHeld; ++i)
-    if (i * 32 + lane < K) s_id[warp][i * 32 + lane] = id[i];
-  __syncwarp();
 #pragma unroll
   for (int i = 0; i < kDistHeld; ++i) {
     if (i * 32 >= K) break;
-    int place = 0;
-    for (int j = 0; j < K; ++j) place += s_id[warp][j] >= 0 && s_id[warp][j] < id[i];
-    if (id[i] >= 0) {
-      a.at[r * K + place] = id[i];
-      a.p[r * K + place] = p[i];
+    if (i * 32 + lane < K) {
+      a.at[r * K + i * 32 + lane] = id[i];
+      a.p[r * K + i * 32 + lane] = p[i];
+      a.x[r * K + i * 32 + lane] = x[i];
     }
+    held += __popc(__ballot_sync(kFull, id[i] >= 0));
   }
   if (lane == 0) {
-    DistillRow& row = a.row[r];
-    row.mass = total;
-    row.shift = entropy;
-    row.held = held;
+    DistillRow& out = a.row[r];
+    out.mass = total;
+    out.entropy = entropy;
+    out.lean = lean;
+    out.ref = ref;
+    out.held = held;
   }
 }
 
@@ -205,6 +218,7 @@ constexpr int kPartHigh = 1, kPartLow = 2;  // steps far above, or far below, we
 struct DistillSum {
   double all, rest;
   int rho;
+  template <bool BOTH>
   __device__ __forceinline__ void add(float a, float b, int r) {
     const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
     const double a64 = __hiloint2double((int)((x >> 3) + (896u << 20)), (int)(x << 29));
@@ -213,15 +227,15 @@ struct DistillSum {
     const int apart = up ? r - rho : rho - r;
     const double shift = __hiloint2double((1023 - (apart < 1000 ? apart : 1000)) << 20, 0);
     all = dfma(up ? all : a64, shift, up ? a64 : all);
-    rest = dfma(up ? rest : b64, shift, up ? b64 : rest);
+    if (BOTH) rest = dfma(up ? rest : b64, shift, up ? b64 : rest);
     rho = up ? r : rho;
   }
 };
 
 struct alignas(16) DistillShared {
   uint64_t bar[kDistWarps][kDistStages];
-  DistillPart warps[kDistWarps];
-  DistillPart parts[2][kDistSplit];  // of one join and of the next
+  DistillPart warps[2][kDistWarps];  // of one row and of the next
+  DistillPart parts[2][kDistSplit];
   double loss[kDistWarps];
   int last;
   // then the rings, and a word of marks per tile and thread: bit u n + e is
@@ -271,38 +285,23 @@ __device__ __forceinline__ DistillPart dist_reduce(DistillPart p) {
 }
 
 // The row's part from its warps', through the cluster; every thread gets it.
-__device__ __noinline__ DistillPart dist_join(DistillShared& sh, DistillPart part, int joins, uint32_t rank,
-                                              uint32_t split) {
+// Between one call and the next but one lies a barrier, so two places do.
+__device__ __forceinline__ DistillPart dist_join(DistillShared& sh, DistillPart part, int joins, uint32_t rank,
+                                                 uint32_t split) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const DistillPart none = {0.0, 0.0, kNegInf64, kNegInf, 0};
   part = dist_reduce(part);
-  if (lane == 0) sh.warps[warp] = part;
+  if (lane == 0) sh.warps[joins & 1][warp] = part;
   __syncthreads();
-  if (split == 1) {
-    part = dist_reduce(lane < kDistWarps ? sh.warps[lane] : none);
-    __syncthreads();
-    return part;
-  }
+  if (split == 1) return dist_reduce(lane < kDistWarps ? sh.warps[joins & 1][lane] : none);
   if (joins == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA of the cluster runs
   if (warp == 0) {
-    part = dist_reduce(lane < kDistWarps ? sh.warps[lane] : none);
+    part = dist_reduce(lane < kDistWarps ? sh.warps[joins & 1][lane] : none);
     if (lane < (int)split) *dist_of(&sh.parts[joins & 1][rank], lane) = part;
   }
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   return dist_reduce(lane < (int)split ? sh.parts[joins & 1][lane] : none);
-}
-
-// What multiplies a row's gradient: weight, temperature, reduction and the
-// loss's own gradient.
-__device__ __forceinline__ double dist_by(const DistillArgs& a, int64_t r) {
-  double by = (a.weights ? (double)a.weights[r] : 1.0) * a.inv_t;
-  if (a.mean) {
-    const double weights = a.weights ? *a.weight_sum : (double)a.rows;
-    by = weights != 0.0 ? by / weights : 0.0;
-  }
-  if (a.grad_loss) by *= (double)a.grad_loss[a.each ? r : 0];
-  return by;
 }
 
 // The student's mass outside the entries, for the bucket.
@@ -311,12 +310,18 @@ __device__ __forceinline__ double dist_tail(double rest, double all) {
   return q < kTailFloor ? kTailFloor : q;
 }
 
-// The bucket's factor of an element's q.
-__device__ __forceinline__ double dist_factor(const DistillArgs& a, const DistillRow& row, double rest, double all) {
-  // without a token outside the entries nothing is left for the bucket
-  if (a.tail != PM_TAIL_BUCKET || row.held >= a.vocab) return 1.0;
-  const double left = row.mass != row.mass ? row.mass : fmax(0.0, 1.0 - row.mass);
-  return 1.0 - left / dist_tail(rest, all);
+// 1 / x by Newton's iteration from an fp32 reciprocal: the gradient's factors
+// are wanted by every warp at once, and 64-bit divisions are slow.
+__device__ __forceinline__ double dist_inverse(double x) {
+  double y = (double)__frcp_rn((float)x);
+  y = dfma(y, dfma(-x, y, 1.0), y);
+  return dfma(y, dfma(-x, y, 1.0), y);
+}
+
+// The bucket's factor of an element's q; inverse = 1 / all.
+__device__ __forceinline__ double dist_factor(double mass, double rest, double all, double inverse) {
+  const double left = mass != mass ? mass : fmax(0.0, 1.0 - mass);
+  return rest * inverse < kTailFloor ? 1.0 - left / kTailFloor : 1.0 - left * all * dist_inverse(rest);
 }
 
 // Of a wild row's part, elements [i0, i1): the sums of 2^((x - top) c), and
@@ -324,26 +329,49 @@ __device__ __forceinline__ double dist_factor(const DistillArgs& a, const Distil
 template <typename T>
 __device__ __noinline__ void dist_wild(const DistillArgs& a, int64_t r, int i0, int i1, float top, double on, double off,
                                        double by, bool store, double* all, double* rest) {
-  const int K = a.k, held = a.row[r].held;
+  const int K = a.k;
   const T* x = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
   T* g = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
   const float c = (float)(kLog2e64 * a.inv_t);
   const int32_t* at = a.at + r * K;
   for (int i = i0 + (int)threadIdx.x; i < i1; i += kDistThreads) {
     const double e = (double)ex2_approx((RowVec<T>::get(x + i) - top) * c);
-    int lo = 0, hi = held;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (at[mid] < i) lo = mid + 1; else hi = mid;
-    }
-    const bool entry = lo < held && at[lo] == i;
+    int k = 0;
+    while (k < K && at[k] != i) ++k;
+    const bool entry = k < K;
     *all += e;
     *rest += entry ? 0.0 : e;
-    if (store) put_grad(g + i, entry ? (float)(e * on - a.p[r * K + lo] * by) : (float)(e * off));
+    if (store) put_grad(g + i, entry ? (float)(e * on - a.p[r * K + k] * by) : (float)(e * off));
   }
 }
 
+// A vector that begins at row element i0, with -inf outside the row.
 template <typename T>
+__device__ __noinline__ uint4 dist_clip(uint4 raw, int i0, int V) {
+  uint32_t in = 0;
+#pragma unroll
+  for (int e = 0; e < RowVec<T>::n; ++e) in |= i0 + e >= 0 && i0 + e < V ? 1u << e : 0u;
+  return RowVec<T>::select(raw, in);
+}
+
+// Stores a lane's packed gradients one by one, those that lie inside the row.
+template <typename T>
+__device__ __noinline__ void dist_edge(T* grow, uint4 r0, uint4 r1, uint4 r2, uint4 r3, int i0, int V) {
+  constexpr int n = RowVec<T>::n;
+  const uint4 raw[kDistStep] = {r0, r1, r2, r3};
+#pragma unroll
+  for (int u = 0; u < kDistStep; ++u) {
+    float v[n];
+    RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+      const int i = i0 + u * 32 * n + e;
+      if (i >= 0 && i < V) put_grad(grow + i, v[e]);
+    }
+  }
+}
+
+template <typename T, bool BUCKET>
 __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(DistillArgs a) {
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   DistillShared& sh = *reinterpret_cast<DistillShared*>(shared_bytes);
@@ -353,7 +381,6 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   const uint32_t rank = dist_rank(), split = dist_split();
   const int V = (int)a.vocab, K = a.k;
   const int rows = (int)a.rows, row0 = (int)(blockIdx.x / split), row_step = (int)(gridDim.x / split);
-  const bool bucket = a.tail == PM_TAIL_BUCKET;
   const float c = (float)(kLog2e64 * a.inv_t);
   const uint64_t c2 = pk(c, c);
   unsigned char* ring = reinterpret_cast<unsigned char*>(&sh + 1) + warp * kDistStages * kDistChunk * 16;
@@ -406,6 +433,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
 
   // The warp's copies, first lane only: the chunks of a row forward, for the
   // gradient back again, then those of the next row.
+  const uint64_t keep = policy_evict_last(), drop = policy_evict_first();
   int ir = row0 - row_step;  // the row that copies are issued for
   int iq = 0, icopies = 0, ichunks = 0;
   const char* isrc = nullptr;
@@ -427,7 +455,8 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
     const int left = ileft - t * kDistTile;
     const uint32_t bytes = (uint32_t)(left < kDistChunk ? left : kDistChunk) * 16;
     mbar_arrive_expect_tx(&bar[st], bytes);
-    bulk_copy_g2s_plain(ring + st * kDistChunk * 16, isrc + (int64_t)t * kDistTile * 16, bytes, &bar[st]);
+    bulk_copy_g2s(ring + st * kDistChunk * 16, isrc + (int64_t)t * kDistTile * 16, bytes, &bar[st],
+                  a.grad && iq <= ichunks ? keep : drop);
   };
   if (lane == 0) {
 #pragma unroll
@@ -438,7 +467,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   }
   // waited for before the first store into another CTA
   if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (bucket) {
+  if (BUCKET) {
     for (int i = tid; i < a.mark_tiles * kDistThreads; i += kDistThreads) marks[i] = 0;
   }
   if (a.grad && a.weights)
@@ -449,13 +478,58 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   int st = 0, joins = 0;
   uint32_t parity = 0;
   bool lost = false;
-  double loss = 0.0;  // of this thread's entries of all the CTA's rows
-  for (int r = next_of(row0 - row_step); r < rows; r = next_of(r)) {
+  // The row's entry of this thread and the row's mass, asked for while the
+  // row before is in work.
+  struct Row {
+    int id, held;
+    float x, w;
+    double p, mass;
+  };
+  auto ask = [&](int r) {
+    Row w = {-1, 0, 0.0f, 1.0f, 0.0, 0.0};
+    if (r < rows) {
+      if (tid < K) {
+        w.id = a.at[(int64_t)r * K + tid];
+        w.p = a.p[(int64_t)r * K + tid];
+        w.x = a.x[(int64_t)r * K + tid];
+      }
+      w.mass = a.row[r].mass;
+      w.held = a.row[r].held;
+      if (a.weights) w.w = a.weights[r];
+      if (a.grad_loss && a.each) w.w *= a.grad_loss[r];
+    }
+    return w;
+  };
+  // the entries of a row are marked, for the bucket
+  auto mark = [&](int r, int id) {
+    const Part p = part_of(r);
+    const int i = id - p.first;
+    if (id >= 0 && i >= 0 && i < p.count * n) {
+      const int j = i / n, u = j % kDistChunk / 32;
+      atomicOr(&marks[j / kDistTile * kDistThreads + j % kDistTile / kDistChunk * 32 + j % 32], 1u << (u * n + i % n));
+    }
+  };
+  cudaGridDependencySynchronize();  // the entries, and the sum of the weights
+  // what every row's gradient is multiplied by, but for its weight
+  double scale = a.inv_t;
+  if (a.mean) {
+    const double weights = a.weights ? *a.weight_sum : (double)a.rows;
+    scale = weights != 0.0 ? scale / weights : 0.0;
+  }
+  if (a.grad_loss && !a.each) scale *= (double)a.grad_loss[0];
+  int r = next_of(row0 - row_step);
+  Row now = ask(r);
+  if (BUCKET && r < rows) {
+    mark(r, now.id);
+    __syncthreads();
+  }
+  for (int after; r < rows; r = after) {
+    after = next_of(r);
     const Part p = part_of(r);
     const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
-    // a copy's vectors, -inf in the granules' parts outside the row
-    auto take = [&](uint4 (&raw)[kDistStep], int j0) {
-      lost = !__all_sync(kFull, mbar_wait(&bar[st], parity)) || lost;
+    // the warp's vectors of its next chunk
+    auto take = [&](uint4 (&raw)[kDistStep]) {
+      if (!lost) lost = !__all_sync(kFull, mbar_wait(&bar[st], parity));
       const uint4* from = reinterpret_cast<const uint4*>(ring + st * kDistChunk * 16) + lane;
 #pragma unroll
       for (int u = 0; u < kDistStep; ++u) raw[u] = from[u * 32];
@@ -467,40 +541,22 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       if (++st == kDistStages) { st = 0; parity ^= 1; }
     };
 
-    if (bucket) {
-      const int id = tid < K ? a.ids[(int64_t)r * K + tid] : -1;
-      const int i = id - p.first;
-      if (id >= 0 && id < V && i >= 0 && i < p.count * n) {
-        const int j = i / n, u = j % kDistChunk / 32;
-        atomicOr(&marks[j / kDistTile * kDistThreads + j % kDistTile / kDistChunk * 32 + j % 32], 1u << (u * n + i % n));
-      }
-      __syncthreads();
-    }
-
-    // forward: sums over all tokens and over the unmarked ones
+    // forward: sums over all tokens and, for the bucket, over the unmarked ones
     DistillSum sums = {0.0, 0.0, StepSum::kNothing};
     float m = kNegInf;
     int flags = 0;
     for (int t = 0; t < p.chunks; ++t) {
       uint32_t marked = 0;
-      if (bucket) {
+      if (BUCKET) {
         marked = marks[t * kDistThreads + tid];
         if (marked) marks[t * kDistThreads + tid] = 0;  // for the next row
       }
       const int j0 = t * kDistTile + warp * kDistChunk;
       uint4 raw[kDistStep];
-      take(raw, j0);
+      take(raw);
       if (j0 < p.whole0 || j0 + kDistChunk > p.whole1) {
 #pragma unroll
-        for (int u = 0; u < kDistStep; ++u) {
-          uint32_t in = 0;
-#pragma unroll
-          for (int e = 0; e < n; ++e) {
-            const int i = p.first + (j0 + u * 32 + lane) * n + e;
-            in |= i >= 0 && i < V ? 1u << e : 0u;
-          }
-          raw[u] = RowVec<T>::select(raw[u], in);
-        }
+        for (int u = 0; u < kDistStep; ++u) raw[u] = dist_clip<T>(raw[u], p.first + (j0 + u * 32 + lane) * n, V);
       }
       const float tm = max_nan(max_nan(RowVec<T>::largest(raw[0]), RowVec<T>::largest(raw[1])),
                                RowVec<T>::largest(raw[2]), RowVec<T>::largest(raw[3]));
@@ -510,7 +566,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
         const float magic = top + 12582912.0f;  // 1.5 2^23 + R
         const float R = magic - 12582912.0f;
         const uint64_t r2 = pk(-R, -R);
-        uint64_t sum = 0;                // of vectors without a mark
+        uint64_t sum0 = 0, sum1 = 0;     // of vectors without a mark
         float with = 0.0f, kept = 0.0f;  // of those with one: all elements, and the unmarked
 #pragma unroll
         for (int u = 0; u < kDistStep; ++u) {
@@ -522,10 +578,13 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
             v[e] = ex2_approx(lo_f(x));
             v[e + 1] = ex2_approx(hi_f(x));
           }
-          const uint32_t bits = (marked >> (u * n)) & kBits;
+          const uint32_t bits = BUCKET ? (marked >> (u * n)) & ((1u << n) - 1u) : 0u;
           if (bits == 0) {
 #pragma unroll
-            for (int e = 0; e < n; e += 2) sum = add2(sum, pk(v[e], v[e + 1]));
+            for (int e = 0; e < n; e += 4) {
+              sum0 = add2(sum0, pk(v[e], v[e + 1]));
+              sum1 = add2(sum1, pk(v[e + 2], v[e + 3]));
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < n; ++e) {
@@ -534,8 +593,9 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
             }
           }
         }
+        const uint64_t sum = add2(sum0, sum1);
         const float plain = lo_f(sum) + hi_f(sum);
-        sums.add(plain + with, plain + kept, (int)(__float_as_uint(magic) - 0x4B400000u));
+        sums.template add<BUCKET>(plain + with, plain + kept, (int)(__float_as_uint(magic) - 0x4B400000u));
       } else if (tm < 0.0f) {
         flags |= tm > kNegInf ? kPartLow : 0;
       } else {
@@ -544,59 +604,64 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       }
     }
     if (lost) sums.all = sums.rest = nan64();
-    if (joins == 0) cudaGridDependencySynchronize();  // the entries, and the sum of the weights
-    // this thread's entry and the row's factors, on their way during the join
-    const DistillRow known = a.row[r];
-    int id = -1;
-    double prob = 0.0;
-    float x_id = 0.0f;
-    if (tid < known.held) {
-      id = a.at[(int64_t)r * K + tid];
-      prob = a.p[(int64_t)r * K + tid];
-      x_id = RowVec<T>::get(row + id);
-    }
-    const double by = dist_by(a, r);
     DistillPart part = {sums.all, sums.rest, sums.rho > StepSum::kNothing ? (double)sums.rho : kNegInf64, m, flags};
     part = dist_join(sh, part, joins, rank, split);
     ++joins;
+    const Row next = ask(after);
     const float top = part.top;
     const bool wild = ((part.flags & kPartHigh) || ((part.flags & kPartLow) && !(top * c > -kWildExponent + 4096.0f))) &&
                       part.all == part.all;
     const int i0 = p.first > 0 ? p.first : 0, i1 = p.first + p.count * n < V ? p.first + p.count * n : V;
     if (wild) {
+      // every CTA sums the whole row
       double all = 0.0, rest = 0.0;
-      dist_wild<T>(a, r, i0, i1, top, 0.0, 0.0, 0.0, false, &all, &rest);
+      dist_wild<T>(a, r, 0, V, top, 0.0, 0.0, 0.0, false, &all, &rest);
       part = {all, rest, 0.0, top, 0};
-      part = dist_join(sh, part, joins, rank, split);
+      part = dist_join(sh, part, joins, 0, 1);
       ++joins;
     }
     // no finite logit: no distribution
     const double all = top == kNegInf ? nan64() : part.all;
-    const bool empty = !bucket && known.mass == 0.0;
+    const bool empty = !BUCKET && now.mass == 0.0;
+    if (rank == 0 && tid == 0) {
+      DistillRow& out = a.row[r];
+      out.all = all;
+      out.rest = part.rest;
+      out.rho = part.rho;
+      out.top = top;
+      out.wild = wild;
+    }
 
     if (a.grad) {
       T* grow = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
       const bool vectors = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
       uint4* out = reinterpret_cast<uint4*>(grow + p.first);
-      const double on = by / all, factor = on * dist_factor(a, known, part.rest, all);
+      const double by = scale * (double)now.w, inverse = dist_inverse(all), on = by * inverse;
+      // without a token outside the entries nothing is left for the bucket
+      const double factor = BUCKET && now.held < V ? on * dist_factor(now.mass, part.rest, all, inverse) : on;
       if (wild || empty) {
         // the copies are not wanted, but others follow them
         uint4 raw[kDistStep];
-        for (int t = 0; t < p.chunks; ++t) take(raw, 0);
+        for (int t = 0; t < p.chunks; ++t) take(raw);
         if (empty) {
           zeros(r, p);
         } else {
           double s0 = 0.0, s1 = 0.0;
           dist_wild<T>(a, r, i0, i1, top, on, factor, by, true, &s0, &s1);
         }
+        if (BUCKET) {
+          if (after < rows) mark(after, next.id);
+          __syncthreads();
+        }
       } else {
         const float f = (float)factor;
         const uint64_t r2 = pk(-(float)part.rho, -(float)part.rho), f2 = pk(f, f);
+        // chunks from lo to hi lie wholly inside the row
+        const int lo = vectors ? p.whole0 : 0x7fffffff, hi = p.whole1 - kDistChunk;
         for (int t = p.chunks - 1; t >= 0; --t) {
           const int j0 = t * kDistTile + warp * kDistChunk;
-          const bool whole = vectors && j0 >= p.whole0 && j0 + kDistChunk <= p.whole1;
           uint4 raw[kDistStep];
-          take(raw, j0);
+          take(raw);
 #pragma unroll
           for (int u = 0; u < kDistStep; ++u) {
             float v[n];
@@ -608,79 +673,40 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
               v[e] = lo_f(y);
               v[e + 1] = hi_f(y);
             }
-            const int j = j0 + u * 32 + lane;
-            if (whole || (vectors && j >= p.whole0 && j < p.whole1)) {
-              __stcs(out + j, pack_grad(v));
-            } else if (j < p.count) {
+            raw[u] = pack_grad(v);
+          }
+          if (j0 >= lo && j0 <= hi) {
+            uint4* to = out + j0 + lane;
 #pragma unroll
-              for (int e = 0; e < n; ++e) {
-                const int i = p.first + j * n + e;
-                if (i >= 0 && i < V) put_grad(grow + i, v[e]);
-              }
-            }
+            for (int u = 0; u < kDistStep; ++u) __stcs(to + u * 32, raw[u]);
+          } else {
+            dist_edge<T>(grow, raw[0], raw[1], raw[2], raw[3], p.first + (j0 + lane) * n, V);
           }
         }
+        if (BUCKET && after < rows) mark(after, next.id);
         // the entries' elements once more, q - p, behind the CTA's own stores
         __syncthreads();
-        if (id >= 0 && id >= i0 && id < i1) {
-          const double q = (double)ex2_approx(fmaf(x_id, c, -(float)part.rho));
-          put_grad(grow + id, (float)(q * on - prob * by));
+        if (now.id >= i0 && now.id < i1) {  // none is -1, i0 is at least 0
+          const double q = (double)ex2_approx(fmaf(now.x, c, -(float)part.rho));
+          put_grad(grow + now.id, (float)(q * on - now.p * by));
         }
       }
+    } else if (BUCKET) {
+      if (after < rows) mark(after, next.id);
+      __syncthreads();
     }
-
-    // the loss: this thread's entry
-    if (rank == 0 && a.loss) {
-      double l = 0.0;
-      if (!empty) {
-        if (prob != 0.0 || tid == 0) {
-          // log of the sum of e^((x - top) / T)
-          const double logS = wild ? log(all)
-                                   : log(all) + (part.rho + (double)top * (kLog2e64 * a.inv_t - (double)c)) * kLn264 -
-                                         (double)top * a.inv_t;
-          if (prob != 0.0) l = -prob * (((double)x_id - (double)top) * a.inv_t - logS);
-        }
-        if (tid == 0) {
-          l += known.shift;
-          if (bucket && known.held < V) {
-            const double left = known.mass != known.mass ? known.mass : fmax(0.0, 1.0 - known.mass);
-            if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(part.rest, all)));
-          }
-        }
-        if (a.weights) l *= (double)a.weights[r];
-      }
-      loss += l;
-      if (a.each) {
-        l = warp_sum64(l);
-        if (lane == 0) sh.loss[warp] = l;
-        __syncthreads();
-        if (tid == 0) {
-          for (int i = 1; i < kDistWarps; ++i) l += sh.loss[i];
-          a.loss[r] = (float)l;
-        }
-      }
+    now = next;
+  }
+  if (lost)  // what is still on its way gets its time before the memory goes
+    for (int i = 0; i < kDistStages; ++i) {
+      mbar_wait(&bar[st], parity);
+      if (++st == kDistStages) { st = 0; parity ^= 1; }
     }
-    if (bucket) __syncthreads();  // the marks are clear
-  }
-  if (joins == 0) {
-    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    cudaGridDependencySynchronize();
-  }
+  if (joins == 0 && split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (rank != 0 || !a.loss) return;
-  if (a.each) {
-    for (int r = row0 + tid * row_step; r < rows; r += kDistThreads * row_step)
-      if (skipped(r)) a.loss[r] = 0.0f;
-    return;
-  }
 
-  // the CTA's loss, and the last CTA's sum of all
-  loss = warp_sum64(loss);
-  __syncthreads();
-  if (lane == 0) sh.loss[warp] = loss;
-  __syncthreads();
+  // the last CTA computes the losses
   if (tid == 0) {
-    for (int i = 1; i < kDistWarps; ++i) loss += sh.loss[i];
-    a.row_loss[row0] = loss;
     __threadfence();
     sh.last = atomicAdd(a.ticket, 1u) == (unsigned)row_step - 1u;
   }
@@ -688,7 +714,29 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   if (!sh.last) return;
   __threadfence();
   double s = 0.0;
-  for (int i = tid; i < row_step; i += kDistThreads) s += __ldcg(a.row_loss + i);
+  for (int64_t i = tid; i < a.rows; i += kDistThreads) {
+    const double w = a.weights ? (double)a.weights[i] : 1.0;
+    double l = 0.0;
+    if (w != 0.0) {
+      const DistillRow* k = a.row + i;
+      const double mass = k->mass, all = __ldcg(&k->all), rest = __ldcg(&k->rest), rho = __ldcg(&k->rho);
+      const double top = (double)__ldcg(&k->top), ref = (double)k->ref;
+      if (BUCKET || mass != 0.0) {
+        // log of the sum of e^((x - top) / T)
+        double logS = log(all);
+        if (!__ldcg(&k->wild)) logS += (rho + top * (kLog2e64 * a.inv_t - (double)c)) * kLn264 - top * a.inv_t;
+        if (mass != 0.0) l = k->entropy - (k->lean + (ref - top) * mass) * a.inv_t + mass * logS;
+        if (BUCKET && k->held < V) {
+          const double left = mass != mass ? mass : fmax(0.0, 1.0 - mass);
+          if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(rest, all)));
+        }
+      }
+      l *= w;
+    }
+    if (a.each) a.loss[i] = (float)l;
+    s += l;
+  }
+  if (a.each) return;
   s = warp_sum64(s);
   if (lane == 0) sh.loss[warp] = s;
   __syncthreads();
@@ -750,14 +798,14 @@ cudaError_t launch_after(void (*kernel)(A...), int64_t grid, int threads, size_t
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename T>
+template <typename T, bool BUCKET>
 cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
   const int64_t row_grid = (a.rows + pm::kRowWarps - 1) / pm::kRowWarps;
-  pm::k_distill_prep<<<(unsigned)row_grid, pm::kRowThreads, 0, st>>>(a);
+  pm::k_distill_prep<T><<<(unsigned)row_grid, pm::kRowThreads, 0, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // CTAs of a row: as many as keep every SM's two, no more than it has tiles
-  auto* kernel = pm::k_distill_rows<T>;
+  auto* kernel = pm::k_distill_rows<T, BUCKET>;
   constexpr int n = pm::RowVec<T>::n;
   const int64_t granules = (a.vocab + n - 1) / n + 1;  // one more where a row starts off a boundary
   const int64_t tiles = (granules + pm::kDistTile - 1) / pm::kDistTile;
@@ -779,7 +827,7 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
   b.vectors = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
   b.mark_tiles = (int)mark_tiles;
   const int64_t clusters = a.rows < slots / split ? a.rows : slots / split;
-  return launch_after(kernel, clusters * split, pm::kDistThreads, bytes(a.tail == PM_TAIL_BUCKET ? mark_tiles : 0), split,
+  return launch_after(kernel, clusters * split, pm::kDistThreads, bytes(BUCKET ? mark_tiles : 0), split,
                       st, b);
 }
 
@@ -788,7 +836,7 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
 extern "C" size_t pm_distill_workspace_bytes(const pm_distill* d) {
   if (check_distill(d) != PM_OK) return 0;
   const size_t rows = (size_t)d->rows, entries = rows * d->k;
-  return 16 + round16(8 * rows) + round16(sizeof(pm::DistillRow) * rows) + round16(8 * entries) + round16(4 * entries);
+  return 16 + round16(sizeof(pm::DistillRow) * rows) + round16(8 * entries) + 2 * round16(4 * entries);
 }
 
 extern "C" int pm_distill_loss(const pm_distill* d, float* loss, void* grad, int64_t grad_stride,
@@ -828,14 +876,18 @@ extern "C" int pm_distill_loss(const pm_distill* d, float* loss, void* grad, int
   a.weight_sum = reinterpret_cast<double*>(ws);
   a.ticket = reinterpret_cast<unsigned*>(ws + 8);
   ws += 16;
-  a.row_loss = reinterpret_cast<double*>(ws);
-  ws += round16(8 * rows);
   a.row = reinterpret_cast<pm::DistillRow*>(ws);
   ws += round16(sizeof(pm::DistillRow) * rows);
   a.p = reinterpret_cast<double*>(ws);
   ws += round16(8 * entries);
   a.at = reinterpret_cast<int32_t*>(ws);
-  const cudaError_t e = d->dtype == PM_DTYPE_F32 ? launch_distill<float>(a, st) : launch_distill<__nv_bfloat16>(a, st);
+  ws += round16(4 * entries);
+  a.x = reinterpret_cast<float*>(ws);
+  const bool bucket = d->tail == PM_TAIL_BUCKET;
+  const cudaError_t e =
+      d->dtype == PM_DTYPE_F32
+          ? bucket ? launch_distill<float, true>(a, st) : launch_distill<float, false>(a, st)
+          : bucket ? launch_distill<__nv_bfloat16, true>(a, st) : launch_distill<__nv_bfloat16, false>(a, st);
   return e == cudaSuccess ? PM_OK : pmh::cuda_fail(e);
 }
 
