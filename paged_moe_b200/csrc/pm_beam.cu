@@ -205,10 +205,10 @@ __device__ __forceinline__ uint4 top_load(const T* row, int off, const uint8_t* 
   return raw;
 }
 
-// The plain way through elements [i0, i1): any order, any ties.  The buffer
-// never holds more than 2 K keys before a step offers at most one vector of
-// every thread, and elements come in ascending order of ids, so that one
-// which only equals the threshold is out.
+// The plain way through elements [i0, i1): any order, any ties.  A step offers
+// at most one vector of half the threads, so that the 2 K keys that stay and
+// the new ones can be sorted; elements come in ascending order of ids, so that
+// one which only equals the threshold is out.
 template <typename T, bool MASKED, bool ALIGNED>
 __device__ __noinline__ void top_plain(TopShared& sh, const T* row, int off, const uint8_t* mask, int i0, int i1,
                                        int V, int K) {
@@ -217,8 +217,11 @@ __device__ __noinline__ void top_plain(TopShared& sh, const T* row, int off, con
   __syncthreads();
   if (tid == 0) { sh.count = 0; sh.thr = kNegInf; }
   __syncthreads();
-  for (int i = i0; i < i1; i += kTopThreads * n) {
-    top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i + tid * n, V), (uint32_t)(i + tid * n), sh.thr);
+  constexpr int kHalf = kTopThreads / 2;
+  static_assert(2 * kTopMax + kHalf * RowVec<T>::n <= kTopSort, "a step's keys can be sorted");
+  for (int i = i0; i < i1; i += kHalf * n) {
+    if (tid < kHalf)
+      top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i + tid * n, V), (uint32_t)(i + tid * n), sh.thr);
     __syncthreads();
     const int cnt = sh.count;
     __syncthreads();
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
 
   const int tiles = (V + kTopTile - 1) / kTopTile;
   const int per = (tiles + (int)split - 1) / (int)split;
-  const int t0 = (int)rank * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  const int t0 = (int)rank * tiles / (int)split, t1 = ((int)rank + 1) * tiles / (int)split;
   // element u of thread g in tile t
   auto at = [&](int t, int u, int g) { return t * kTopTile + (g >> 5) * kChunk + (u * 32 + (g & 31)) * n; };
 
@@ -453,13 +456,14 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   }
   __syncthreads();
   const int listed = sh.listed;
-  if (listed <= kTopList) {
+  auto offer = [&](float above) {
     for (int j = tid; j < listed * U; j += kTopThreads) {
       const int g = sh.list()[j / U];
       const int i = at(t0 + g / kTopThreads, j % U, g % kTopThreads);
-      top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), (uint32_t)i, below);
+      top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), (uint32_t)i, above);
     }
-  }
+  };
+  if (listed <= kTopList) offer(below);
   double rho = warp_max64(sh.wrho[lane % kTopWarps]);
   ExpSum mine = acc.sum();
   if (__syncthreads_or(acc.wild(warp_max_ordered(sh.wmax[lane % kTopWarps]), scale.c) && acc.s == acc.s)) {
@@ -472,8 +476,22 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   const double s = warp_sum64(scaled_to(mine, rho));
   if (lane == 0) sh.wsum[warp] = s;
   __syncthreads();
-  if (listed > kTopList || sh.count > kTopBuf)
+  if (listed > kTopList) {
     top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTopTile, t1 * kTopTile, V, K);
+  } else if (sh.count > kTopBuf) {
+    // a part of few tiles at a large k: the k-th of some of its elements is a
+    // better bound, once
+    __syncthreads();
+    top_cut(sh, kTopSort, K);
+    const float better = float_below(sh.thr);
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (better > below) offer(better);
+    __syncthreads();
+    if (!(better > below) || sh.count > kTopBuf)
+      top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTopTile, t1 * kTopTile, V, K);
+  }
 
   // the part's list, maximum and sum
   if (warp == kTopWarps - 1) {

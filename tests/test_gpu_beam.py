@@ -298,3 +298,19 @@ def test_select_on_another_stream_and_captured():
     for got in (other, *outs):
         for k in want:
             assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V,k", [(2, 3000, 256), (3, 4096, 200), (64, 151936, 256), (5, 8192, 256), (1, 9000, 130),
+                                      (7, 20000, 256)])
+def test_top_large_k_of_short_parts(rows, V, k, dtype):
+    """Few maxima for many candidates: rows, or parts of split rows, of one or two tiles."""
+    _check_top(_logits(40, rows, V, dtype), k)
+
+
+def test_top_short_parts_with_ties():
+    x = torch.zeros((3, 6000), device=DEV)
+    x[1, ::3] = 1.0
+    x[2, 5000:] = 2.0
+    _check_top(x, 256)
+    _check_top(x.to(torch.bfloat16), 200)
