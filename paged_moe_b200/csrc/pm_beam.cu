@@ -18,8 +18,8 @@
 // a thread; more are sorted.  A part with more keys than the buffer holds
 // (long ties, as in a constant row) takes the plain way: one vector of every
 // thread at a time against a running threshold.
-// The cluster's CTAs put their lists and sums into the first one's shared
-// memory, which ranks them once more.
+// The cluster's CTAs put their lists and sums into one another's shared memory;
+// each finds its own keys' places in the row and writes those.
 //
 // Every wait on a copy is bounded; a row whose copy does not arrive gives
 // NaN and ids -1.
@@ -72,12 +72,12 @@ constexpr int kTopStep = 4;
 constexpr int kTopStages = 2;
 constexpr int kTopStageBytes = kTopStep * 512 + 16;  // 16 more for rows off a 16-byte boundary
 
-struct TopShared {
+struct alignas(16) TopShared {
   uint64_t bar[kTopWarps][kTopStages];
   uint64_t best[kTopMax];
   double wrho[kTopWarps], wsum[kTopWarps];
-  ExpSum part[kTopSplit];
-  float top[kTopSplit];   // the parts' maxima
+  ExpSum part[1], parts[kTopSplit];  // the CTA's, and those of the row's CTAs
+  float top[1], tops[kTopSplit];     // likewise the largest elements
   int parts_got[kTopSplit];
   unsigned hist[256];
   int scal[4];
@@ -504,91 +504,83 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   }
   top_cut(sh, sh.count, K);
 
+  // key j of rank i in the row, and what the row lacks of K by its first CTA
+  auto put = [&](int i, uint64_t key, bool have, double lse, bool bad) {
+    const float x = have ? key_value(key) : kNegInf;
+    a.ids[r * K + i] = have ? (int32_t)key_index(key) : -1;
+    if (a.vals) a.vals[r * K + i] = x;
+    if (a.logprobs) a.logprobs[r * K + i] = bad ? (float)lse : have ? (float)((double)x * a.inv_t - lse) : kNegInf;
+  };
+  uint64_t* keys = reinterpret_cast<uint64_t*>(tops + per * kTopThreads);
+  int total = sh.got;  // keys of the row
   if (split > 1) {
-    uint64_t* keys = reinterpret_cast<uint64_t*>(tops + per * kTopThreads);  // 16-byte aligned
+    // every CTA gets all the lists and places its own
     cluster_wait();  // every CTA of the cluster runs
     const int mine = sh.got;
-    for (int i = tid; i < K; i += kTopThreads) *of_rank(&keys[rank * K + i], 0) = i < mine ? sh.best[i] : 0ull;
-    if (tid == 0) {
-      if (rank > 0) {
-        *of_rank(&sh.part[rank], 0) = sh.part[0];
-        *of_rank(&sh.top[rank], 0) = sh.top[0];
-      }
-      *of_rank(&sh.parts_got[rank], 0) = mine;
+    for (int i = tid; i < K * (int)split; i += kTopThreads) {
+      const int c = i / K, j = i - c * K;
+      *of_rank(&keys[rank * K + j], c) = j < mine ? sh.best[j] : 0ull;
+    }
+    if (warp == 0 && lane < (int)split) {
+      *of_rank(&sh.parts[rank], lane) = sh.part[0];
+      *of_rank(&sh.tops[rank], lane) = sh.top[0];
+      *of_rank(&sh.parts_got[rank], lane) = mine;
     }
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    if (rank != 0) return;
+    total = 0;
+#pragma unroll
+    for (int d = 0; d < kTopSplit; ++d) total += d < (int)split ? sh.parts_got[d] : 0;
     if (warp == kTopWarps - 1) {
       const bool on = lane < (int)split;
       ExpSum part = {0.0, kNegInf64};
-      if (on) part = sh.part[lane];
+      if (on) part = sh.parts[lane];
       const double to = warp_max64(part.rho);
       part.s = warp_sum64(scaled_to(part, to));
-      const float top = warp_max_ordered(on ? sh.top[lane] : kNegInf);
-      const int got = (int)__reduce_add_sync(kFull, on ? (unsigned)sh.parts_got[lane] : 0u);
+      part.rho = to;
+      const float top = warp_max_ordered(on ? sh.tops[lane] : kNegInf);
       if (lane == 0) {
-        part.rho = to;
         sh.part[0] = part;
         sh.top[0] = top;
-        sh.got = got < K ? got : K;
-      }
-    }
-    // a key's place in the row is the number of larger keys
-    const int all = K * (int)split;
-    if (all <= kTopFew) {
-      const uint64_t key = tid < all ? keys[tid] : 0ull;
-      if (key) {
-        int place = 0;
-#pragma unroll 8
-        for (int j = 0; j < all; j += 2) {  // split is even
-          const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&keys[j]);
-          place += (o.x > key) + (o.y > key);
-        }
-        if (place < K) sh.best[place] = key;
-      }
-    } else {
-      // searched for in all the lists at once
-      int half = 1;
-      while (half * 2 <= K) half *= 2;
-      for (int i = tid; i < all; i += kTopThreads) {
-        const uint64_t key = keys[i];
-        if (!key) continue;
-        int found[kTopSplit] = {};
-        for (int step = half; step > 0; step >>= 1) {
-#pragma unroll
-          for (int d = 0; d < kTopSplit; ++d) {
-            const int to = found[d] + step;
-            // lists that the row does not have hold nothing larger
-            const uint64_t there = keys[(d < (int)split ? d : 0) * K + (to < K ? to : K) - 1];
-            if (to <= K && d < (int)split && there > key) found[d] = to;
-          }
-        }
-        int place = 0;
-#pragma unroll
-        for (int d = 0; d < kTopSplit; ++d) place += found[d];
-        if (place < K) sh.best[place] = key;
       }
     }
     __syncthreads();
   }
-
   const ExpSum sum = sh.part[0];
   const float M = sh.top[0];
   const bool bad = !(sum.s == sum.s) || M == -kNegInf;
   const double lse = bad ? nan64() : M > kNegInf ? scale.log_of(sum, M) : kNegInf64;
-  const int got = bad ? 0 : sh.got;
-  if (tid == 0) {
-    if (a.lse) a.lse[r] = (float)lse;
-    if (a.lse64) a.lse64[r] = M > kNegInf ? lse : nan64();
+  if (rank == 0) {
+    if (tid == 0) {
+      if (a.lse) a.lse[r] = (float)lse;
+      if (a.lse64) a.lse64[r] = M > kNegInf ? lse : nan64();
+    }
+    for (int i = (bad ? 0 : total) + tid; i < K; i += kTopThreads) put(i, 0ull, false, lse, bad);
   }
-  for (int i = tid; i < K; i += kTopThreads) {
-    const bool have = i < got;
-    const float x = have ? key_value(sh.best[i]) : kNegInf;
-    a.ids[r * K + i] = have ? (int32_t)key_index(sh.best[i]) : -1;
-    if (a.vals) a.vals[r * K + i] = x;
-    if (a.logprobs) a.logprobs[r * K + i] = bad ? (float)lse : have ? (float)((double)x * a.inv_t - lse) : kNegInf;
+  if (bad) return;
+  for (int i = tid; i < sh.got; i += kTopThreads) {
+    const uint64_t key = sh.best[i];
+    int place = i;
+    if (split > 1) {
+      // the number of larger keys, searched for in all the lists at once
+      int half = 1;
+      while (half * 2 <= K) half *= 2;
+      int found[kTopSplit] = {};
+      for (int step = half; step > 0; step >>= 1) {
+#pragma unroll
+        for (int d = 0; d < kTopSplit; ++d) {
+          const int to = found[d] + step;
+          // lists that the row does not have hold nothing larger
+          const uint64_t there = keys[(d < (int)split ? d : 0) * K + (to < K ? to : K) - 1];
+          if (to <= K && d < (int)split && there > key) found[d] = to;
+        }
+      }
+      place = 0;
+#pragma unroll
+      for (int d = 0; d < kTopSplit; ++d) place += found[d];
+    }
+    if (place < K) put(place, key, true, lse, false);
   }
 }
 
