@@ -8,6 +8,8 @@
 // happens here: every kernel is in libpm_sample.so.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -592,6 +594,84 @@ void distill_scale(torch::Tensor grad, torch::Tensor factor) {
         "pm_distill_scale");
 }
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A gradient that cannot be differentiated once more says so when it is.
+variable_list once(torch::Tensor grad, const torch::Tensor& grad_loss, size_t inputs) {
+  if (at::GradMode::is_enabled() && grad_loss.requires_grad())
+    grad = (*std::make_shared<torch::autograd::DelayedError>(
+        "distill_loss has no second derivative", 1))({grad})[0];
+  variable_list grads(inputs);
+  grads[0] = std::move(grad);
+  return grads;
+}
+
+// Sum and mean: the loss and its gradient in one pass over the logits, in the
+// forward; the backward multiplies by the loss's own gradient, in place, and
+// hands the buffer on.
+struct DistillWithGrad : torch::autograd::Function<DistillWithGrad> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& logits, const torch::Tensor& ids,
+                               const torch::Tensor& logprobs, double temp, int64_t tail, const OptT& weights,
+                               int64_t reduction) {
+    std::vector<torch::Tensor> r = distill(logits, ids, logprobs, temp, tail, weights, reduction, true, true, OptT());
+    ctx->saved_data["grad"] = r[1];
+    ctx->saved_data["shape"] = logits.sizes();
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto it = ctx->saved_data.find("grad");
+    TORCH_CHECK(it != ctx->saved_data.end(),
+                "distill_loss keeps its gradient for one backward pass; call it again for another");
+    torch::Tensor grad = it->second.toTensor();
+    ctx->saved_data.erase(it);
+    {
+      const at::NoGradGuard off;
+      distill_scale(grad, grads[0]);
+      grad = grad.view(ctx->saved_data["shape"].toIntVector());
+    }
+    return once(std::move(grad), grads[0], 7);
+  }
+};
+
+// No reduction: the gradient waits for the rows' own, so the backward reads
+// the logits again.
+struct DistillPerRow : torch::autograd::Function<DistillPerRow> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& logits, const torch::Tensor& ids,
+                               const torch::Tensor& logprobs, double temp, int64_t tail, const OptT& weights,
+                               int64_t reduction) {
+    torch::Tensor loss = distill(logits, ids, logprobs, temp, tail, weights, reduction, true, false, OptT())[0];
+    ctx->save_for_backward({logits, ids, logprobs, weights.has_value() ? *weights : torch::Tensor()});
+    ctx->saved_data["temp"] = temp;
+    ctx->saved_data["tail"] = tail;
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    torch::Tensor grad;
+    {
+      const at::NoGradGuard off;
+      grad = distill(saved[0], saved[1], saved[2], ctx->saved_data["temp"].toDouble(),
+                     ctx->saved_data["tail"].toInt(), saved[3].defined() ? OptT(saved[3]) : OptT(),
+                     ctx->saved_data["reduction"].toInt(), false, true, OptT(grads[0]))[1];
+      grad = grad.view(saved[0].sizes());
+    }
+    return once(std::move(grad), grads[0], 7);
+  }
+};
+
+// The loss of logits [..., V]: one value, or one per row [N] without a reduction.
+torch::Tensor distill_loss(torch::Tensor logits, torch::Tensor ids, torch::Tensor logprobs, double temp, int64_t tail,
+                           OptT weights, int64_t reduction) {
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    if (reduction == PM_REDUCE_NONE)
+      return DistillPerRow::apply(logits, ids, logprobs, temp, tail, weights, reduction);
+    return DistillWithGrad::apply(logits, ids, logprobs, temp, tail, weights, reduction);
+  }
+  return distill(logits, ids, logprobs, temp, tail, weights, reduction, true, false, OptT())[0];
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -603,7 +683,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("top_logprobs", &top_logprobs);
   m.def("beam_select", &beam_select);
   m.def("beam_reorder", &beam_reorder);
-  m.def("distill", &distill);
-  m.def("distill_scale", &distill_scale);
+  m.def("distill_loss", &distill_loss);
   m.def("version", [] { return std::string(pm_version()); });
 }

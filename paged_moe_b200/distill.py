@@ -19,47 +19,6 @@ _TAILS = {"drop": L.PM_TAIL_DROP, "bucket": L.PM_TAIL_BUCKET}
 _REDUCTIONS = {"none": L.PM_REDUCE_NONE, "sum": L.PM_REDUCE_SUM, "mean": L.PM_REDUCE_MEAN}
 
 
-class _WithGrad(torch.autograd.Function):
-    """Sum and mean: the loss and its gradient in one pass over the logits,
-    in the forward; the backward multiplies by the loss's own gradient, in
-    place, and hands the buffer on."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, logprobs, temp, tail, weights, reduction):
-        loss, grad = L.ext().distill(logits, ids, logprobs, temp, tail, weights, reduction, True, True, None)
-        ctx.grad, ctx.shape = grad, logits.shape
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_loss):
-        grad, ctx.grad = ctx.grad, None
-        if grad is None:
-            raise RuntimeError("distill_loss keeps its gradient for one backward pass; call it again for another")
-        L.ext().distill_scale(grad, grad_loss)
-        return grad.view(ctx.shape), None, None, None, None, None, None
-
-
-class _PerRow(torch.autograd.Function):
-    """No reduction: the gradient waits for the rows' own, so the backward
-    reads the logits again."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, logprobs, temp, tail, weights, reduction):
-        (loss, _) = L.ext().distill(logits, ids, logprobs, temp, tail, weights, reduction, True, False, None)
-        ctx.save_for_backward(logits, ids, logprobs, weights)
-        ctx.args = (temp, tail, reduction)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_loss):
-        logits, ids, logprobs, weights = ctx.saved_tensors
-        temp, tail, reduction = ctx.args
-        (_, grad) = L.ext().distill(logits, ids, logprobs, temp, tail, weights, reduction, False, True, grad_loss)
-        return grad.view(logits.shape), None, None, None, None, None, None
-
-
 def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logprobs: torch.Tensor, temp: float = 1.0,
                  tail: str = "drop", weights: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
     """KL divergence of the student's distribution from a teacher's top
@@ -96,9 +55,6 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
         raise ValueError(f"tail must be one of {sorted(_TAILS)}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
-    args = (logits, teacher_ids, teacher_logprobs, float(temp), _TAILS[tail], weights, _REDUCTIONS[reduction])
-    if torch.is_grad_enabled() and logits.requires_grad:
-        loss = (_PerRow if reduction == "none" else _WithGrad).apply(*args)
-    else:
-        loss = L.ext().distill(*args, True, False, None)[0]
+    loss = L.ext().distill_loss(logits, teacher_ids, teacher_logprobs, float(temp), _TAILS[tail], weights,
+                                _REDUCTIONS[reduction])
     return loss.view(logits.shape[:-1]) if reduction == "none" else loss
