@@ -750,13 +750,55 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   }
 }
 
+// The gradient times the loss's own, in place; nothing to do where that is 1.
+// An element of bf16 is rounded a second time (by half a step at most): the
+// loss's gradient is not known yet when the first pass writes it.  Bound by
+// memory, a read and a write of every element: a row is cut into parts of 4,096
+// granules so that few long rows fill the GPU, and four loads of a thread are
+// in flight.
+constexpr int kScaleThreads = 256;
+constexpr int kScaleLoads = 4;
+constexpr int kScalePart = 4096;
 template <typename T>
-__global__ void __launch_bounds__(256) k_distill_scale(T* g, int64_t rows, int64_t vocab, int64_t stride,
-                                                       const float* factor) {
+__global__ void __launch_bounds__(kScaleThreads) k_distill_scale(T* g, int64_t rows, int vocab, int64_t stride, int parts,
+                                                                 const float* factor) {
+  constexpr int n = RowVec<T>::n;
   const float f = *factor;
   if (f == 1.0f) return;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int64_t i = threadIdx.x; i < vocab; i += 256) put_grad(g + r * stride + i, RowVec<T>::get(g + r * stride + i) * f);
+  for (int64_t unit = blockIdx.x; unit < rows * parts; unit += gridDim.x) {
+    const int64_t r = unit / parts;
+    const int first = (int)(unit - r * parts) * kScalePart;
+    T* row = g + r * stride;
+    const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);
+    uint4* whole = reinterpret_cast<uint4*>(row - off);
+    const int end = min((off + vocab + n - 1) / n, first + kScalePart);
+    for (int j0 = first + threadIdx.x; j0 < end; j0 += kScaleThreads * kScaleLoads) {
+      uint4 raw[kScaleLoads];
+      bool in[kScaleLoads];
+#pragma unroll
+      for (int u = 0; u < kScaleLoads; ++u) {
+        const int j = j0 + u * kScaleThreads;
+        in[u] = j < end && j * n >= off && (j + 1) * n - off <= vocab;
+        if (in[u]) raw[u] = whole[j];
+      }
+#pragma unroll
+      for (int u = 0; u < kScaleLoads; ++u) {
+        const int j = j0 + u * kScaleThreads;
+        if (in[u]) {
+          float v[n];
+          RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+          for (int e = 0; e < n; ++e) v[e] *= f;
+          whole[j] = pack_grad(v);
+        } else if (j < end) {  // a granule that the row shares with what lies beside it
+          for (int e = 0; e < n; ++e) {
+            const int i = j * n + e - off;
+            if (i >= 0 && i < vocab) put_grad(row + i, RowVec<T>::get(row + i) * f);
+          }
+        }
+      }
+    }
+  }
 }
 
 }  // namespace pm
@@ -898,13 +940,17 @@ extern "C" int pm_distill_scale(void* grad, int32_t dtype, int64_t rows, int64_t
   if (rows == 0) return PM_OK;
   if (!grad || !factor) return PM_ERR_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t most = (int64_t)pmh::num_sms() * 8;
-  const unsigned grid = (unsigned)(rows < most ? rows : most);
+  if (vocab > pm::kDistVocab) return PM_ERR_UNSUPPORTED;
+  // a row covers up to two granules more than it fills
+  const int parts = (int)((vocab * (dtype == PM_DTYPE_F32 ? 4 : 2) / 16 + 1) / pm::kScalePart) + 1;
+  const int64_t most = (int64_t)pmh::num_sms() * 8, units = rows * parts;
+  const unsigned grid = (unsigned)(units < most ? units : most);
   if (dtype == PM_DTYPE_F32)
-    pm::k_distill_scale<float><<<grid, 256, 0, st>>>(reinterpret_cast<float*>(grad), rows, vocab, grad_stride, factor);
+    pm::k_distill_scale<float><<<grid, pm::kScaleThreads, 0, st>>>(reinterpret_cast<float*>(grad), rows, (int)vocab,
+                                                                   grad_stride, parts, factor);
   else
-    pm::k_distill_scale<__nv_bfloat16>
-        <<<grid, 256, 0, st>>>(reinterpret_cast<__nv_bfloat16*>(grad), rows, vocab, grad_stride, factor);
+    pm::k_distill_scale<__nv_bfloat16><<<grid, pm::kScaleThreads, 0, st>>>(
+        reinterpret_cast<__nv_bfloat16*>(grad), rows, (int)vocab, grad_stride, parts, factor);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PM_OK : pmh::cuda_fail(e);
 }

@@ -601,7 +601,7 @@ using torch::autograd::variable_list;
 variable_list once(torch::Tensor grad, const torch::Tensor& grad_loss, size_t inputs) {
   if (at::GradMode::is_enabled() && grad_loss.requires_grad())
     grad = (*std::make_shared<torch::autograd::DelayedError>(
-        "distill_loss has no second derivative", 1))({grad})[0];
+        "distill_loss has no second derivative", 1))({grad.detach().requires_grad_()})[0];
   variable_list grads(inputs);
   grads[0] = std::move(grad);
   return grads;

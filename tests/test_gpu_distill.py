@@ -309,3 +309,39 @@ def test_limits_raise():
         pm.distill_loss(x, ids, lps)
     with pytest.raises(ValueError):
         pm.distill_loss(x, ids[:, :3].cpu(), lps[:, :3])
+
+
+@pytest.mark.parametrize("dtype,N,V,pad,offset", [
+    (torch.float32, 3, 16383, 1, 3), (torch.float32, 2, 16384, 0, 0), (torch.bfloat16, 2, 32767, 9, 7),
+    (torch.bfloat16, 3, 100, 0, 1), (torch.float32, 1, 1, 0, 2), (torch.float32, 2, 40001, 2, 1)])
+def test_a_loss_with_a_factor(dtype, N, V, pad, offset):
+    """The factor multiplies the loss's gradient as it was stored, one
+    rounding more; nothing beside the rows is written."""
+    x, ids, lps = _case(40, N, V, 5, dtype, pad=pad, offset=offset)
+    x.requires_grad_()
+    plain = torch.autograd.grad(pm.distill_loss(x, ids, lps, reduction="sum"), x)[0]
+    scaled = torch.autograd.grad(pm.distill_loss(x, ids, lps, reduction="sum") * 0.7, x)[0]
+    # in fp32 here: a bf16 tensor times a tensor of no dimensions rounds 0.7 to bf16 first
+    assert torch.equal(scaled, (plain.float() * np.float32(0.7).item()).to(dtype))
+    grad = torch.full((N * (V + pad) + offset + 40,), 3.0, dtype=dtype, device=DEV)
+    rows = grad[offset:offset + N * (V + pad)].view(N, V + pad)
+    before = grad.clone()
+    from paged_moe_b200 import _lib as L
+    code = L.PM_DTYPE_F32 if dtype == torch.float32 else L.PM_DTYPE_BF16
+    factor = torch.tensor([-0.5], device=DEV)
+    L.check(L.load().pm_distill_scale(rows.data_ptr(), code, N, V, V + pad, factor.data_ptr(),
+                                      torch.cuda.current_stream().cuda_stream), "pm_distill_scale")
+    want = before.clone()
+    want[offset:offset + N * (V + pad)].view(N, V + pad)[:, :V] *= -0.5
+    assert torch.equal(grad, want)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_no_second_derivative(reduction):
+    x, ids, lps = _case(41, 3, 100, 4)
+    x.requires_grad_()
+    up = torch.ones((), device=DEV, requires_grad=True)
+    loss = (pm.distill_loss(x, ids, lps, reduction=reduction) * up).sum()
+    grad = torch.autograd.grad(loss, x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="second derivative"):
+        grad.sum().backward()
