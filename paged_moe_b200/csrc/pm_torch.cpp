@@ -283,6 +283,16 @@ Mask check_mask(const OptT& mask, int64_t rows, int64_t V) {
   return m;
 }
 
+// Bytes [at, ...) of a call's own output buffer as a tensor, without the time of
+// the dispatched narrow() and view().
+torch::Tensor piece(const torch::Tensor& buf, int64_t at, torch::ScalarType type, torch::IntArrayRef sizes) {
+  torch::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(),
+                                                             c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 // pm_top_logprobs: [ids [N, k], logprobs [N, k], lse [N] or empty]
 std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, double temp, OptT mask, bool want_lse) {
   pm_top_rows t;
@@ -307,9 +317,9 @@ std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, double 
   t.inv_temperature = 1.0 / temp;
   if (k > 256) check(PM_ERR_UNSUPPORTED, "pm_top_logprobs");  // before any allocation
   torch::Tensor buf = torch::empty({N * (2 * k + (want_lse ? 1 : 0))}, x.options().dtype(torch::kInt32));
-  torch::Tensor ids = buf.narrow(0, 0, N * k).view({N, k});
-  torch::Tensor lp = buf.narrow(0, N * k, N * k).view(torch::kFloat32).view({N, k});
-  torch::Tensor lse = want_lse ? buf.narrow(0, 2 * N * k, N).view(torch::kFloat32) : buf.narrow(0, 0, 0);
+  torch::Tensor ids = piece(buf, 0, torch::kInt32, {N, k});
+  torch::Tensor lp = piece(buf, 4 * N * k, torch::kFloat32, {N, k});
+  torch::Tensor lse = piece(buf, 8 * N * k, torch::kFloat32, {want_lse ? N : 0});
   check(pm_top_logprobs(&t, ids.data_ptr<int32_t>(), lp.data_ptr<float>(), want_lse ? lse.data_ptr<float>() : nullptr,
                         stream_of(x.device())),
         "pm_top_logprobs");
@@ -377,27 +387,27 @@ std::vector<torch::Tensor> beam_select(torch::Tensor logits, torch::Tensor score
   const int64_t E = B * n;
   torch::Tensor buf = torch::empty({E * 3 + (lengths.has_value() ? E : 0) + (eos >= 0 ? (E + 3) / 4 : 0)},
                                    x.options().dtype(torch::kInt32));
-  std::vector<torch::Tensor> res(5, buf.narrow(0, 0, 0));
+  std::vector<torch::Tensor> res(5);
   int64_t at = 0;
-  auto take = [&] {
-    torch::Tensor t = buf.narrow(0, at, E).view({B, n});
-    at += E;
+  auto take = [&](torch::ScalarType type) {
+    torch::Tensor t = piece(buf, at, type, {B, n});
+    at += E * 4;
     return t;
   };
   pm_beam_out o;
   std::memset(&o, 0, sizeof(o));
-  res[0] = take().view(torch::kFloat32);
-  res[1] = take();
-  res[2] = take();
+  res[0] = take(torch::kFloat32);
+  res[1] = take(torch::kInt32);
+  res[2] = take(torch::kInt32);
   o.scores = res[0].data_ptr<float>();
   o.parents = res[1].data_ptr<int32_t>();
   o.tokens = res[2].data_ptr<int32_t>();
   if (lengths.has_value()) {
-    res[3] = take();
+    res[3] = take(torch::kInt32);
     o.lengths = res[3].data_ptr<int32_t>();
   }
   if (eos >= 0) {
-    res[4] = buf.narrow(0, at, (E + 3) / 4).view(torch::kUInt8).narrow(0, 0, E).view(torch::kBool).view({B, n});
+    res[4] = take(torch::kBool);
     o.done = reinterpret_cast<uint8_t*>(res[4].data_ptr());
   }
   check(pm_beam_select(&b, &o, ws.data_ptr(), need, stream_of(x.device())), "pm_beam_select");
@@ -452,9 +462,20 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
   }
   std::vector<pm_state> s(states.size());
   std::vector<const void*> read, written;
+  struct Extent {  // of a tensor that fills it
+    const char *from, *to;
+    bool written;
+  };
+  std::vector<Extent> extents;
+  auto add_extent = [&](const torch::Tensor& t, bool write) {
+    const char* from = reinterpret_cast<const char*>(t.data_ptr());
+    if (t.is_non_overlapping_and_dense()) extents.push_back({from, from + t.nbytes(), write});
+  };
   for (size_t i = 0; i < states.size(); ++i) {
     const torch::Tensor& a = states[i];
     const std::string name = "state " + std::to_string(i);
+    if (at::GradMode::is_enabled() && (out.has_value() ? (*out)[i] : a).requires_grad())
+      bad_value(name + " requires a gradient, which the reorder does not carry; call it under torch.no_grad()");
     if (a.dim() < 1 || a.size(0) != B * W) bad_value(name + " must have items * beams rows");
     int64_t dim = dims[i];
     if (dim >= 0 && !lengths.has_value()) bad_value("seq_dim needs lengths");
@@ -486,6 +507,8 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
     if (a.numel() == 0) { s[i].run_bytes = 0; continue; }
     read.push_back(s[i].src);
     written.push_back(s[i].dst);
+    add_extent(a, !out.has_value());
+    if (out.has_value()) add_extent(b, true);
   }
   // the same memory twice would be moved twice, or read after it was written
   std::vector<const void*> seen = written;
@@ -494,6 +517,14 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
   if (out.has_value())
     for (const void* p : read)
       if (std::binary_search(seen.begin(), seen.end(), p)) bad_value("out shares its memory with a state");
+  std::sort(extents.begin(), extents.end(), [](const Extent& a, const Extent& b) { return a.from < b.from; });
+  const char *end = nullptr, *written_end = nullptr;  // of those that begin before
+  for (const Extent& e : extents) {
+    if (e.from < (e.written ? end : written_end))
+      bad_value(out.has_value() ? "out overlaps a state or another out" : "two states overlap");
+    end = std::max(end, e.to);
+    if (e.written) written_end = std::max(written_end, e.to);
+  }
   need_cuda(parents, "parents");
   const torch::Device dev = parents.device();
   if (lengths.has_value()) on_device(*lengths, dev, "lengths");
@@ -509,6 +540,8 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
                           reinterpret_cast<const int32_t*>(ptr(lengths)), B, (int32_t)std::min<int64_t>(W, 0x7fffffff),
                           stream_of(dev)),
           "pm_beam_reorder");
+  for (const torch::Tensor& t : out.has_value() ? *out : states)  // as an operation in place does
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // pm_distill_loss over logits [..., V] viewed as rows: [loss or empty, grad or

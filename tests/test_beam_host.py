@@ -192,3 +192,34 @@ def test_beam_reorder_c_nothing_to_do():
     assert lib.pm_beam_reorder(None, 0, None, 0, None, 2, 4, None) == L.PM_OK
     arr = (L.State * 1)(_state())
     assert lib.pm_beam_reorder(arr, 1, None, 0, None, 0, 4, None) == L.PM_OK
+
+
+def test_beam_reorder_refuses_memory_that_overlaps():
+    """Dense tensors that share a part of their memory; the parts of one
+    buffer that lie between one another do not."""
+    parents = torch.zeros(1, 3, dtype=torch.int32)
+    buf = torch.zeros(40)
+    a, shifted, behind = buf[:12].view(3, 4), buf[4:16].view(3, 4), buf[12:24].view(3, 4)
+    with pytest.raises(ValueError, match="overlap"):
+        pm.beam_reorder([a, shifted], parents)
+    with pytest.raises(ValueError, match="overlap"):
+        pm.beam_reorder([a], parents, out=[shifted])
+    with pytest.raises(ValueError, match="overlap"):
+        pm.beam_reorder([a, torch.zeros(3, 4)], parents, out=[behind, buf[20:32].view(3, 4)])
+    pair = torch.zeros(3, 2, 4)
+    for states in ([a, behind], [pair[:, 0], pair[:, 1]]):
+        with pytest.raises(ValueError, match="CUDA"):  # all that is left to refuse
+            pm.beam_reorder(states, parents)
+    with pytest.raises(ValueError, match="CUDA"):  # states that are only read may share
+        pm.beam_reorder([a, shifted], parents, out=[torch.zeros(3, 4), torch.zeros(3, 4)])
+
+
+def test_beam_reorder_refuses_a_state_with_a_gradient():
+    parents = torch.zeros(1, 3, dtype=torch.int32)
+    leaf = torch.zeros(3, 4, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        pm.beam_reorder([leaf], parents)
+    with pytest.raises(ValueError, match="gradient"):
+        pm.beam_reorder([torch.zeros(3, 4)], parents, out=[leaf])
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        pm.beam_reorder([leaf], parents)

@@ -171,3 +171,20 @@ def test_captured_and_other_stream():
     torch.cuda.synchronize()
     np.testing.assert_array_equal(out.double().cpu().numpy(),
                                   P.reorder(t.double().cpu().numpy(), par.cpu().numpy()))
+
+
+def test_a_write_counts_as_one_in_place():
+    """A tensor saved for a backward pass and reordered after it is refused by
+    that pass, as any other write in place is."""
+    state = torch.randn(4, 8, device=DEV)
+    leaf = torch.randn(4, 8, device=DEV, requires_grad=True)
+    parents = torch.tensor([[1, 0, 3, 2]], dtype=torch.int32, device=DEV)
+    y = (state * leaf).sum()
+    pm.beam_reorder([state], parents)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        inside = torch.randn(4, 8, device=DEV)
+    before = inside.clone()
+    pm.beam_reorder([inside], parents)
+    assert torch.equal(inside, before[[1, 0, 3, 2]])
