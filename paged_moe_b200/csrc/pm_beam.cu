@@ -81,6 +81,8 @@ struct alignas(16) TopShared {
   int parts_got[kTopSplit];
   unsigned hist[256];
   int scal[4];
+  double lse;             // of the row
+  int bad;                // the row has no distribution
   int count;              // keys in buf
   int got;                // keys in best
   int listed;
@@ -504,7 +506,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   }
   top_cut(sh, sh.count, K);
 
-  // key j of rank i in the row, and what the row lacks of K by its first CTA
+  // the row's key of rank i
   auto put = [&](int i, uint64_t key, bool have, double lse, bool bad) {
     const float x = have ? key_value(key) : kNegInf;
     a.ids[r * K + i] = have ? (int32_t)key_index(key) : -1;
@@ -532,56 +534,60 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
     total = 0;
 #pragma unroll
     for (int d = 0; d < kTopSplit; ++d) total += d < (int)split ? sh.parts_got[d] : 0;
-    if (warp == kTopWarps - 1) {
-      const bool on = lane < (int)split;
-      ExpSum part = {0.0, kNegInf64};
-      if (on) part = sh.parts[lane];
-      const double to = warp_max64(part.rho);
-      part.s = warp_sum64(scaled_to(part, to));
-      part.rho = to;
-      const float top = warp_max_ordered(on ? sh.tops[lane] : kNegInf);
-      if (lane == 0) {
-        sh.part[0] = part;
-        sh.top[0] = top;
-      }
-    }
-    __syncthreads();
   }
-  const ExpSum sum = sh.part[0];
-  const float M = sh.top[0];
-  const bool bad = !(sum.s == sum.s) || M == -kNegInf;
-  const double lse = bad ? nan64() : M > kNegInf ? scale.log_of(sum, M) : kNegInf64;
-  if (rank == 0) {
-    if (tid == 0) {
-      if (a.lse) a.lse[r] = (float)lse;
-      if (a.lse64) a.lse64[r] = M > kNegInf ? lse : nan64();
-    }
-    for (int i = (bad ? 0 : total) + tid; i < K; i += kTopThreads) put(i, 0ull, false, lse, bad);
-  }
-  if (bad) return;
-  for (int i = tid; i < sh.got; i += kTopThreads) {
-    const uint64_t key = sh.best[i];
-    int place = i;
+  // the last warp joins the sums and takes the logarithm, while the others
+  // look for their keys' places
+  if (warp == kTopWarps - 1) {
+    ExpSum sum = sh.part[0];
+    float M = sh.top[0];
     if (split > 1) {
-      // the number of larger keys, searched for in all the lists at once
-      int half = 1;
-      while (half * 2 <= K) half *= 2;
-      int found[kTopSplit] = {};
-      for (int step = half; step > 0; step >>= 1) {
-#pragma unroll
-        for (int d = 0; d < kTopSplit; ++d) {
-          const int to = found[d] + step;
-          // lists that the row does not have hold nothing larger
-          const uint64_t there = keys[(d < (int)split ? d : 0) * K + (to < K ? to : K) - 1];
-          if (to <= K && d < (int)split && there > key) found[d] = to;
-        }
-      }
-      place = 0;
-#pragma unroll
-      for (int d = 0; d < kTopSplit; ++d) place += found[d];
+      const bool on = lane < (int)split;
+      sum = {0.0, kNegInf64};
+      if (on) sum = sh.parts[lane];
+      const double to = warp_max64(sum.rho);
+      sum.s = warp_sum64(scaled_to(sum, to));
+      sum.rho = to;
+      M = warp_max_ordered(on ? sh.tops[lane] : kNegInf);
     }
-    if (place < K) put(place, key, true, lse, false);
+    const bool bad = !(sum.s == sum.s) || M == -kNegInf;
+    const double lse = bad ? nan64() : M > kNegInf ? scale.log_of(sum, M) : kNegInf64;
+    if (lane == 0) {
+      sh.lse = lse;
+      sh.bad = bad;
+      if (rank == 0) {
+        if (a.lse) a.lse[r] = (float)lse;
+        if (a.lse64) a.lse64[r] = M > kNegInf ? lse : nan64();
+      }
+    }
   }
+  static_assert(kTopMax <= kTopThreads, "a key a thread");
+  const uint64_t key = tid < sh.got ? sh.best[tid] : 0ull;
+  int place = tid < sh.got ? tid : K;
+  if (split > 1 && tid < sh.got) {
+    // the number of larger keys, searched for in all the lists at once
+    int half = 1;
+    while (half * 2 <= K) half *= 2;
+    int found[kTopSplit] = {};
+    for (int step = half; step > 0; step >>= 1) {
+#pragma unroll
+      for (int d = 0; d < kTopSplit; ++d) {
+        const int to = found[d] + step;
+        // lists that the row does not have hold nothing larger
+        const uint64_t there = keys[(d < (int)split ? d : 0) * K + (to < K ? to : K) - 1];
+        if (to <= K && d < (int)split && there > key) found[d] = to;
+      }
+    }
+    place = 0;
+#pragma unroll
+    for (int d = 0; d < kTopSplit; ++d) place += found[d];
+  }
+  __syncthreads();
+  const double lse = sh.lse;
+  const bool bad = sh.bad;
+  if (!bad && place < K) put(place, key, true, lse, false);
+  // what the row lacks, by its first CTA
+  if (rank == 0)
+    for (int i = (bad ? 0 : total) + tid; i < K; i += kTopThreads) put(i, 0ull, false, lse, bad);
 }
 
 // ---------------------------------------------------------------------------
