@@ -88,7 +88,7 @@ struct DistillArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
-  __shared__ int s_id[kRowWarps][kDistMax];
+  __shared__ __align__(16) int s_id[kRowWarps][kDistMax];
   __shared__ double s_p[kRowWarps][kDistMax];
   __shared__ double scratch[kRowWarps];
   cudaTriggerProgrammaticLaunchCompletion();  // the rows' copies may start; they wait for this grid themselves
@@ -166,19 +166,31 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
   entropy = warp_sum64(entropy);
   lean = warp_sum64(lean);
   __syncwarp();
-  // an id's first entry takes the sum of all
-  int held = 0;
+  // an id's first entry takes the sum of all; few rows name an id twice, which
+  // ids alone tell
+  int held = 0, same[kDistHeld] = {};
 #pragma unroll 4
-  for (int j = 0; j < K; ++j) {
-    const int other = s_id[warp][j];
-    const double more = s_p[warp][j];
+  for (int j = 0; j < K; j += 4) {
+    const int4 o = *reinterpret_cast<const int4*>(&s_id[warp][j]);
 #pragma unroll
-    for (int i = 0; i < kDistHeld; ++i) {
-      const int k = i * 32 + lane;
-      if (i * 32 >= K) break;
-      if (other == id[i] && other >= 0) {
-        if (j > k) p[i] += more;
-        else if (j < k) id[i] = -1;
+    for (int i = 0; i < kDistHeld; ++i)
+      if (i * 32 < K) same[i] += (o.x == id[i]) + (o.y == id[i]) + (o.z == id[i]) + (o.w == id[i]);
+  }
+  bool twice = false;
+#pragma unroll
+  for (int i = 0; i < kDistHeld; ++i) twice |= id[i] >= 0 && same[i] > 1;
+  if (__any_sync(kFull, twice)) {
+    for (int j = 0; j < K; ++j) {
+      const int other = s_id[warp][j];
+      const double more = s_p[warp][j];
+#pragma unroll
+      for (int i = 0; i < kDistHeld; ++i) {
+        const int k = i * 32 + lane;
+        if (i * 32 >= K) break;
+        if (other == id[i] && other >= 0) {
+          if (j > k) p[i] += more;
+          else if (j < k) id[i] = -1;
+        }
       }
     }
   }
