@@ -607,106 +607,55 @@ struct PickArgs {
   pm_beam_out out;
 };
 
-__device__ __forceinline__ void pick_merge(const PickArgs& a, int64_t row0, int* s_par, int* s_tok, double* s_tot) {
-  const int lane = threadIdx.x & 31, W = a.beams, n = a.n;
-  const double none = kNegInf64;
-  double score[2], lse[2], div[2], head[2];
-  int at[2];
-  bool ended[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int w = lane + 32 * h;
-    at[h] = 0;
-    head[h] = none;
-    score[h] = lse[h] = 0.0;
-    div[h] = 1.0;
-    ended[h] = false;
-    if (w < W) {
-      const int64_t r = row0 + w;
-      score[h] = (double)a.scores[r];
-      ended[h] = a.done && a.done[r];
-      lse[h] = a.lse64[r];
-      if (a.lengths && a.alpha != 0.0) {
-        const int len = a.lengths[r] + (ended[h] ? 0 : 1);
-        div[h] = pow((double)(len > 1 ? len : 1), a.alpha);
-      }
-    }
-  }
-  auto total = [&](int h) -> double {
-    const int w = lane + 32 * h;
-    if (w >= W || at[h] >= n || !(score[h] > none)) return none;
-    if (ended[h]) return at[h] == 0 ? score[h] : none;
-    if (!(lse[h] == lse[h])) return none;
-    const int64_t i = (row0 + w) * n + at[h];
-    return a.ids[i] < 0 ? none : score[h] + ((double)a.vals[i] - lse[h]);
-  };
-  head[0] = total(0);
-  head[1] = total(1);
-  for (int j = 0; j < n; ++j) {
-    // best of this lane's two heads, then of the warp; ties: the lower beam
-    double k0 = head[0] / div[0], k1 = head[1] / div[1];
-    double best = k0;
-    int who = lane;
-    if (k1 > k0) { best = k1; who = lane + 32; }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double ob = __shfl_xor_sync(kFull, best, o);
-      const int ow = __shfl_xor_sync(kFull, who, o);
-      if (ob > best || (ob == best && ow < who)) { best = ob; who = ow; }
-    }
-    const bool have = best > none;
-    if (have && lane == (who & 31)) {
-      const int h = who >> 5;
-      s_par[j] = who;
-      s_tot[j] = h ? head[1] : head[0];
-      const int p = h ? at[1] : at[0];
-      s_tok[j] = (h ? ended[1] : ended[0]) ? a.eos : a.ids[(row0 + who) * n + p];
-      if (h) { ++at[1]; head[1] = total(1); } else { ++at[0]; head[0] = total(0); }
-    }
-    if (!have && lane == 0) { s_par[j] = -1; s_tok[j] = -1; s_tot[j] = none; }
-  }
-}
-
 // One CTA per item.  Up to 256 candidates (beams x n) are ranked by counting,
 // one a thread: a candidate's place is the number of better ones, and of
-// equal ones before it.  More are merged by the first warp, which takes the
-// best head n times; lane l holds the heads of beams l and l + 32.
-constexpr int kPickThreads = 256;
+// equal ones before it.  More are merged two beams' lists at a time, each
+// candidate searching the other list for its place, until one list is left:
+// 2 W n searches of log n steps in log W rounds.
+constexpr int kPickThreads = 256;   // counting
+constexpr int kPickMerge = 1024;    // merging
 
-__global__ void __launch_bounds__(kPickThreads) k_beam_pick(PickArgs a) {
+__global__ void __launch_bounds__(kPickMerge) k_beam_pick(PickArgs a) {
+  extern __shared__ __align__(16) unsigned char pick_bytes[];
+  double* s_rank = reinterpret_cast<double*>(pick_bytes);  // [W n]; then, for merging, two lists of [W n] indexes
   __shared__ int s_par[kTopMax], s_tok[kTopMax];
-  __shared__ double s_tot[kTopMax];
-  __shared__ double s_rank[kPickThreads];
+  __shared__ double s_tot[kTopMax], s_div[kBeamMax];
   __shared__ int s_slot[kTopMax];
   const int64_t item = blockIdx.x;
-  const int tid = threadIdx.x, W = a.beams, n = a.n, all = W * n;
+  const int tid = threadIdx.x, threads = blockDim.x, W = a.beams, n = a.n, all = W * n;
   const double none = kNegInf64;
   const int64_t row0 = item * W;
   cudaGridDependencySynchronize();
+  // candidate j of beam w: its score and token
+  auto total_of = [&](int w, int j, int* token) {
+    const int64_t r = row0 + w;
+    const double score = (double)a.scores[r];
+    if (!(score > none)) return none;
+    if (a.done && a.done[r]) {
+      *token = a.eos;
+      return j == 0 ? score : none;
+    }
+    const double lse = a.lse64[r];
+    const int id = a.ids[r * n + j];
+    if (!(lse == lse) || id < 0) return none;
+    *token = id;
+    return score + ((double)a.vals[r * n + j] - lse);
+  };
+  auto divisor = [&](int w) {
+    if (!a.lengths || a.alpha == 0.0) return 1.0;
+    const int len = a.lengths[row0 + w] + (a.done && a.done[row0 + w] ? 0 : 1);
+    return pow((double)(len > 1 ? len : 1), a.alpha);
+  };
+  for (int i = tid; i < n; i += threads) { s_par[i] = -1; s_tok[i] = -1; s_tot[i] = none; }
   if (all <= kPickThreads) {
     double total = none, rank = none;
     int token = -1;
     const int w = tid / n, j = tid % n;
     if (tid < all) {
-      const int64_t r = row0 + w;
-      const double score = (double)a.scores[r], lse = a.lse64[r];
-      const bool ended = a.done && a.done[r];
-      if (score > none) {
-        if (ended) {
-          if (j == 0) { total = score; token = a.eos; }
-        } else if (lse == lse) {
-          const int id = a.ids[r * n + j];
-          if (id >= 0) { total = score + ((double)a.vals[r * n + j] - lse); token = id; }
-        }
-      }
-      rank = total;
-      if (a.lengths && a.alpha != 0.0) {
-        const int len = a.lengths[r] + (ended ? 0 : 1);
-        rank = total / pow((double)(len > 1 ? len : 1), a.alpha);
-      }
+      total = total_of(w, j, &token);
+      rank = total / divisor(w);
       s_rank[tid] = rank;
     }
-    for (int i = tid; i < n; i += kPickThreads) { s_par[i] = -1; s_tok[i] = -1; s_tot[i] = none; }
     __syncthreads();
     if (tid < all && rank > none) {
       int place = 0;
@@ -715,11 +664,50 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(PickArgs a) {
     }
     __syncthreads();
   } else {
-    if (tid < 32) pick_merge(a, row0, s_par, s_tok, s_tot);
+    if (tid < W) s_div[tid] = divisor(tid);
+    __syncthreads();
+    for (int i = tid; i < all; i += threads) {
+      int token;
+      const int w = i / n;
+      s_rank[i] = total_of(w, i - w * n, &token) / s_div[w];
+    }
+    __syncthreads();
+    // a beam's list is in order already: larger logits first
+    uint16_t* out = reinterpret_cast<uint16_t*>(s_rank + all);
+    const uint16_t* in = nullptr;
+    for (int lists = W; lists > 1; lists = (lists + 1) / 2) {  // n is 256 at most: there are two at least
+      for (int i = tid; i < lists * n; i += threads) {
+        const int l = i / n, p = i - l * n, me = in ? in[i] : i;
+        int place = p;
+        if ((l ^ 1) < lists) {
+          // those of the other list that come first, equal ones of lower beams too
+          const int base = (l ^ 1) * n;
+          const double rank = s_rank[me];
+          int lo = 0, hi = n - p;
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            const double other = s_rank[in ? in[base + mid] : base + mid];
+            if (other > rank || ((l & 1) && other == rank)) lo = mid + 1; else hi = mid;
+          }
+          place += lo;
+        }
+        if (place < n) out[(l >> 1) * n + place] = (uint16_t)me;
+      }
+      __syncthreads();
+      in = out;
+      out = reinterpret_cast<uint16_t*>(s_rank + all) + (out == reinterpret_cast<uint16_t*>(s_rank + all) ? all : 0);
+    }
+    for (int j = tid; j < n; j += threads) {
+      const int i = in[j];
+      if (s_rank[i] > none) {
+        s_par[j] = i / n;
+        s_tot[j] = total_of(i / n, i % n, &s_tok[j]);
+      }
+    }
     __syncthreads();
   }
   if (!a.keep_slots) {
-    for (int j = tid; j < n; j += kPickThreads) s_slot[j] = j;
+    for (int j = tid; j < n; j += threads) s_slot[j] = j;
   } else if (tid == 0) {
     uint64_t taken = 0;
     for (int j = 0; j < n; ++j) {
@@ -735,7 +723,7 @@ __global__ void __launch_bounds__(kPickThreads) k_beam_pick(PickArgs a) {
       }
   }
   __syncthreads();
-  for (int j = tid; j < n; j += kPickThreads) {
+  for (int j = tid; j < n; j += threads) {
     const int64_t o = item * n + s_slot[j];
     const int p = s_par[j];
     a.out.scores[o] = (float)s_tot[j];
@@ -913,16 +901,26 @@ extern "C" int pm_beam_select(const pm_beam* b, const pm_beam_out* out, void* wo
   p.vals = a.vals;
   p.lse64 = a.lse64;
   p.out = *out;
+  const int all = b->beams * b->n;
+  const bool merge = all > pm::kPickThreads;
+  static pmh::DeviceOnce once;
+  cudaError_t e = cudaSuccess;
+  once([&] {
+    e = cudaFuncSetAttribute(pm::k_beam_pick, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             pm::kBeamMax * pm::kTopMax * 12);
+  });
+  if (e != cudaSuccess) return pmh::cuda_fail(e);
   // launched while the rows' kernel drains; it waits for that grid itself
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)b->items);
-  cfg.blockDim = dim3(pm::kPickThreads);
+  cfg.blockDim = dim3(merge ? pm::kPickMerge : pm::kPickThreads);
+  cfg.dynamicSmemBytes = (size_t)all * (merge ? 12 : 8);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, pm::k_beam_pick, p);
+  e = cudaLaunchKernelEx(&cfg, pm::k_beam_pick, p);
   return e == cudaSuccess ? PM_OK : pmh::cuda_fail(e);
 }
