@@ -15,7 +15,7 @@
 // are read once more, about 1.2 k to 2 k of them, and only elements that
 // reach it become keys, (ordered logit bits, ~id): larger logits first, then
 // lower ids, all keys different.  Up to 256 keys are ranked by counting, one
-// a thread; more are sorted.  A part with more keys than the buffer holds
+// a thread; of more, histograms leave that many first.  A part with more keys than the buffer holds
 // (long ties, as in a constant row) takes the plain way: one vector of every
 // thread at a time against a running threshold.
 // The cluster's CTAs put their lists and sums into one another's shared memory;
@@ -43,8 +43,7 @@ constexpr int kTopMax = 256;      // largest k
 constexpr int kTopSplit = 8;      // most CTAs of a row (a portable cluster)
 constexpr int kTopBuf = 2560;     // keys: 2 x the largest k, and one vector of every thread
 constexpr int kTopList = 2048;    // threads' tiles that are read once more
-constexpr int kTopFew = 256;      // keys that are ranked by counting, one a thread
-constexpr int kTopSort = 2048;    // keys that are sorted
+constexpr int kTopFew = 256;      // keys that are ranked, one a thread
 
 struct TopArgs {
   const void* logits;
@@ -80,7 +79,8 @@ struct alignas(16) TopShared {
   float top[1], tops[kTopSplit];     // likewise the largest elements
   int parts_got[kTopSplit];
   unsigned hist[256];
-  int scal[4];
+  int scal[kTopWarps];
+  int bin[3];
   double lse;             // of the row
   int bad;                // the row has no distribution
   int count;              // keys in buf
@@ -109,69 +109,102 @@ __device__ __forceinline__ float float_below(float x) {
   return key_value((uint64_t)o << 32);
 }
 
-// Sorts buf[0, cnt) in descending order, cnt <= kTopSort: a bitonic network over
-// the next power of two.  Pairs at most 32 apart lie in 64 keys of one warp,
-// so that only the wider steps need the CTA's barrier.
-__device__ __forceinline__ void top_sort(uint64_t* buf, int cnt) {
-  const int tid = threadIdx.x;
-  int P = 64;
-  while (P < cnt) P <<= 1;
-  for (int i = cnt + tid; i < P; i += kTopThreads) buf[i] = 0ull;
-  __syncthreads();
-  for (int k = 2; k <= P; k <<= 1) {
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int p = tid; p < P / 2; p += kTopThreads) {
-        const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1));
-        const uint64_t a = buf[i], b = buf[i + j];
-        if ((i & k) == 0 ? a < b : a > b) { buf[i] = b; buf[i + j] = a; }
-      }
-      if (j > 32 || (j == 1 && k >= 64)) __syncthreads(); else __syncwarp();
-    }
+// Copies keys of buf[0, cnt), K <= kTopFew < cnt, to best: the K largest and at
+// most kTopFew in all.  Returns their number.  Histograms of 256 bins over the
+// keys' range, then over the bin that holds the K-th, until few enough are
+// left: all keys differ, so that it ends.
+__device__ __noinline__ int top_narrow(TopShared& sh, int cnt, int K) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint64_t* buf = sh.buf();
+  uint32_t least = ~0u, most = 0u;
+  for (int i = tid; i < cnt; i += kTopThreads) {
+    const uint32_t v = (uint32_t)(buf[i] >> 32);
+    least = v < least ? v : least;
+    most = v > most ? v : most;
   }
+  least = __reduce_min_sync(kFull, least);
+  most = __reduce_max_sync(kFull, most);
+  if (lane == 0) { sh.hist[warp] = least; sh.hist[kTopWarps + warp] = most; }
+  __syncthreads();
+  least = __reduce_min_sync(kFull, sh.hist[lane % kTopWarps]);
+  most = __reduce_max_sync(kFull, sh.hist[kTopWarps + lane % kTopWarps]);
+  uint64_t lo = (uint64_t)least << 32, hi = ((uint64_t)most << 32) | 0xffffffffu;
+  int need = K, sure = 0;  // of the keys in [lo, hi]; those above
+  for (;;) {
+    const int top = 64 - __clzll((long long)(hi - lo)), shift = top > 8 ? top - 8 : 0;
+    __syncthreads();
+    sh.hist[tid] = 0;
+    __syncthreads();
+#pragma unroll 2
+    for (int i = tid; i < cnt; i += kTopThreads) {
+      const uint64_t key = buf[i];
+      if (key >= lo && key <= hi) atomicAdd(&sh.hist[(int)((key - lo) >> shift)], 1u);
+    }
+    __syncthreads();
+    // keys in this thread's bin and above it
+    const int mine = (int)sh.hist[tid];
+    int at_least = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_down_sync(kFull, at_least, o);
+      if (lane + o < 32) at_least += v;
+    }
+    if (lane == 0) sh.scal[warp] = at_least;
+    __syncthreads();
+    for (int w = warp + 1; w < kTopWarps; ++w) at_least += sh.scal[w];
+    if (at_least >= need && at_least - mine < need) {
+      sh.bin[0] = tid;
+      sh.bin[1] = at_least;
+      sh.bin[2] = mine;
+    }
+    __syncthreads();
+    lo += (uint64_t)sh.bin[0] << shift;
+    if (sure + sh.bin[1] <= kTopFew) break;
+    const int above = sh.bin[1] - sh.bin[2];
+    sure += above;
+    need -= above;
+    hi = lo + ((1ull << shift) - 1ull);
+  }
+  if (tid == 0) sh.scal[0] = 0;
+  __syncthreads();
+  for (int i = tid; i < cnt; i += kTopThreads) {
+    const uint64_t key = buf[i];
+    if (key >= lo) sh.best[atomicAdd(&sh.scal[0], 1)] = key;
+  }
+  __syncthreads();
+  return sh.scal[0];
 }
 
 // Cuts buf[0, cnt) to its K largest, sorted, in buf and best; sets count, got
 // and the threshold.  Every thread, between barriers.
 __device__ __forceinline__ void top_cut(TopShared& sh, int cnt, int K) {
   const int tid = threadIdx.x;
-  if (cnt <= kTopFew) {
-    // one key a thread: its rank is the number of larger keys
-    const uint64_t key = tid < cnt ? sh.buf()[tid] : 0ull;
-    int rank = 0;
-    if (tid < cnt) {
-      int j = 0;
+  const uint64_t* from = sh.buf();
+  if (cnt > kTopFew) {
+    cnt = top_narrow(sh, cnt, K);
+    from = sh.best;
+  }
+  // one key a thread: its rank is the number of larger keys
+  const uint64_t key = tid < cnt ? from[tid] : 0ull;
+  int rank = 0;
+  if (tid < cnt) {
+    int j = 0;
 #pragma unroll 8
-      for (; j + 1 < cnt; j += 2) {
-        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.buf()[j]);
-        rank += (o.x > key) + (o.y > key);
-      }
-      if (j < cnt) rank += sh.buf()[j] > key;
+    for (; j + 1 < cnt; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&from[j]);
+      rank += (o.x > key) + (o.y > key);
     }
-    __syncthreads();
-    if (tid < cnt && rank < K) {
-      sh.buf()[rank] = key;
-      sh.best[rank] = key;
-      if (rank == K - 1) sh.thr = key_value(key);
-    }
-    if (tid == 0) {
-      sh.count = sh.got = cnt < K ? cnt : K;
-      if (cnt < K) sh.thr = kNegInf;
-    }
-  } else if (cnt <= kTopSort) {
-    top_sort(sh.buf(), cnt);
-    const int got = cnt < K ? cnt : K;
-    if (tid < got) sh.best[tid] = sh.buf()[tid];
-    if (tid == 0) {
-      sh.count = sh.got = got;
-      sh.thr = got == K ? key_value(sh.buf()[K - 1]) : kNegInf;
-    }
-  } else {
-    const int got = block_topk_sorted(sh.buf(), cnt, K, sh.best, kTopMax, sh.hist, sh.scal);
-    for (int i = tid; i < got; i += kTopThreads) sh.buf()[i] = sh.best[i];
-    if (tid == 0) {
-      sh.count = sh.got = got;
-      sh.thr = got == K ? key_value(sh.best[K - 1]) : kNegInf;
-    }
+    if (j < cnt) rank += from[j] > key;
+  }
+  __syncthreads();
+  if (tid < cnt && rank < K) {
+    sh.buf()[rank] = key;
+    sh.best[rank] = key;
+    if (rank == K - 1) sh.thr = key_value(key);
+  }
+  if (tid == 0) {
+    sh.count = sh.got = cnt < K ? cnt : K;
+    if (cnt < K) sh.thr = kNegInf;
   }
   __syncthreads();
 }
@@ -208,9 +241,9 @@ __device__ __forceinline__ uint4 top_load(const T* row, int off, const uint8_t* 
 }
 
 // The plain way through elements [i0, i1): any order, any ties.  A step offers
-// at most one vector of half the threads, so that the 2 K keys that stay and
-// the new ones can be sorted; elements come in ascending order of ids, so that
-// one which only equals the threshold is out.
+// at most one vector of every thread, so that the 2 K keys that stay and the
+// new ones fit; elements come in ascending order of ids, so that one which only
+// equals the threshold is out.
 template <typename T, bool MASKED, bool ALIGNED>
 __device__ __noinline__ void top_plain(TopShared& sh, const T* row, int off, const uint8_t* mask, int i0, int i1,
                                        int V, int K) {
@@ -219,11 +252,9 @@ __device__ __noinline__ void top_plain(TopShared& sh, const T* row, int off, con
   __syncthreads();
   if (tid == 0) { sh.count = 0; sh.thr = kNegInf; }
   __syncthreads();
-  constexpr int kHalf = kTopThreads / 2;
-  static_assert(2 * kTopMax + kHalf * RowVec<T>::n <= kTopSort, "a step's keys can be sorted");
-  for (int i = i0; i < i1; i += kHalf * n) {
-    if (tid < kHalf)
-      top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i + tid * n, V), (uint32_t)(i + tid * n), sh.thr);
+  static_assert(2 * kTopMax + kTopThreads * RowVec<T>::n <= kTopBuf, "a step's keys fit");
+  for (int i = i0; i < i1; i += kTopThreads * n) {
+    top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i + tid * n, V), (uint32_t)(i + tid * n), sh.thr);
     __syncthreads();
     const int cnt = sh.count;
     __syncthreads();
@@ -484,7 +515,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
     // a part of few tiles at a large k: the k-th of some of its elements is a
     // better bound, once
     __syncthreads();
-    top_cut(sh, kTopSort, K);
+    top_cut(sh, kTopBuf, K);
     const float better = float_below(sh.thr);
     __syncthreads();
     if (tid == 0) sh.count = 0;
