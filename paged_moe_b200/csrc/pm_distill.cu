@@ -39,6 +39,7 @@ constexpr int kDistThreads = 384;
 constexpr int kDistWarps = kDistThreads / 32;
 constexpr int kDistResident = 2;               // CTAs of an SM
 constexpr int kDistMax = 256;                  // largest k
+constexpr int kDistTableBits = 9;              // a table for twice as many ids
 constexpr int kDistHeld = kDistMax / 32;       // entries of a lane
 constexpr int64_t kDistVocab = 262144;
 constexpr int kDistSplit = 8;                  // most CTAs of a row
@@ -88,9 +89,10 @@ struct DistillArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
-  __shared__ __align__(16) int s_id[kRowWarps][kDistMax];
+  __shared__ int s_id[kRowWarps][kDistMax];
   __shared__ double s_p[kRowWarps][kDistMax];
   __shared__ double scratch[kRowWarps];
+  __shared__ int s_table[kRowWarps][1 << kDistTableBits];
   cudaTriggerProgrammaticLaunchCompletion();  // the rows' copies may start; they wait for this grid themselves
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.k, V = (int)a.vocab;
   if (blockIdx.x == 0) {
@@ -107,6 +109,9 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < 1 << kDistTableBits; i += 32) s_table[warp][i + lane] = -1;
+  __syncwarp();
   const int64_t r = (int64_t)blockIdx.x * kRowWarps + warp;
   if (r >= a.rows || (a.weights && a.weights[r] == 0.0f)) return;
   const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
@@ -167,18 +172,22 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
   lean = warp_sum64(lean);
   __syncwarp();
   // an id's first entry takes the sum of all; few rows name an id twice, which
-  // ids alone tell
-  int held = 0, same[kDistHeld] = {};
-#pragma unroll 4
-  for (int j = 0; j < K; j += 4) {
-    const int4 o = *reinterpret_cast<const int4*>(&s_id[warp][j]);
-#pragma unroll
-    for (int i = 0; i < kDistHeld; ++i)
-      if (i * 32 < K) same[i] += (o.x == id[i]) + (o.y == id[i]) + (o.z == id[i]) + (o.w == id[i]);
-  }
+  // a table with open addressing tells
+  int held = 0;
   bool twice = false;
 #pragma unroll
-  for (int i = 0; i < kDistHeld; ++i) twice |= id[i] >= 0 && same[i] > 1;
+  for (int i = 0; i < kDistHeld; ++i) {
+    if (i * 32 >= K) break;
+    if (id[i] >= 0) {
+      uint32_t at = (uint32_t)id[i] * 2654435761u >> (32 - kDistTableBits);  // the golden ratio's multiple of 2^32
+      for (;;) {
+        const int there = atomicCAS(&s_table[warp][at], -1, id[i]);
+        if (there == -1) break;
+        if (there == id[i]) { twice = true; break; }
+        at = (at + 1) & ((1u << kDistTableBits) - 1u);
+      }
+    }
+  }
   if (__any_sync(kFull, twice)) {
     for (int j = 0; j < K; ++j) {
       const int other = s_id[warp][j];
