@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_prep(DistillArgs a) {
 // ---------------------------------------------------------------------------
 // A CTA's share of a row.
 struct DistillPart {
-  double all, rest, rho;
+  double all, rest;  // multiples of 2^rho
+  int rho;
   float top;
   int flags;
 };
@@ -295,8 +296,9 @@ __device__ __forceinline__ V* dist_of(V* p, uint32_t rank) {
 
 // The warp's parts as one.
 __device__ __forceinline__ DistillPart dist_reduce(DistillPart p) {
-  const double to = warp_max64(p.rho);
-  const double f = p.rho > kNegInf64 ? pow2_down(p.rho - to) : 1.0;  // nothing: 0, or a NaN that stays
+  const int to = __reduce_max_sync(kFull, p.rho), apart = to - p.rho;
+  // nothing: 0, or a NaN that stays
+  const double f = p.rho > StepSum::kNothing ? __hiloint2double((1023 - (apart < 1000 ? apart : 1000)) << 20, 0) : 1.0;
   p.all = warp_sum64(p.all * f);
   p.rest = warp_sum64(p.rest * f);
   p.rho = to;
@@ -310,7 +312,7 @@ __device__ __forceinline__ DistillPart dist_reduce(DistillPart p) {
 __device__ __forceinline__ DistillPart dist_join(DistillShared& sh, DistillPart part, int joins, uint32_t rank,
                                                  uint32_t split) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const DistillPart none = {0.0, 0.0, kNegInf64, kNegInf, 0};
+  const DistillPart none = {0.0, 0.0, StepSum::kNothing, kNegInf, 0};
   part = dist_reduce(part);
   if (lane == 0) sh.warps[joins & 1][warp] = part;
   __syncthreads();
@@ -625,7 +627,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       }
     }
     if (lost) sums.all = sums.rest = nan64();
-    DistillPart part = {sums.all, sums.rest, sums.rho > StepSum::kNothing ? (double)sums.rho : kNegInf64, m, flags};
+    DistillPart part = {sums.all, sums.rest, sums.rho, m, flags};
     part = dist_join(sh, part, joins, rank, split);
     ++joins;
     const Row next = ask(after);
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       // every CTA sums the whole row
       double all = 0.0, rest = 0.0;
       dist_wild<T>(a, r, 0, V, top, 0.0, 0.0, 0.0, false, &all, &rest);
-      part = {all, rest, 0.0, top, 0};
+      part = {all, rest, 0, top, 0};
       part = dist_join(sh, part, joins, 0, 1);
       ++joins;
     }
@@ -648,7 +650,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       DistillRow& out = a.row[r];
       out.all = all;
       out.rest = part.rest;
-      out.rho = part.rho;
+      out.rho = (double)part.rho;
       out.top = top;
       out.wild = wild;
     }
