@@ -14,8 +14,8 @@
 //   the logits come from L2: 95 MB are in work at 320 KB a row, of which half
 //   is still wanted on average; what was read last is read first, the first
 //   reading asks L2 to keep the data and the second and the stores to let go of
-//   it.  The last CTA to end computes the rows' losses from their sums and adds
-//   them up in a fixed order.
+//   it.  A CTA computes its rows' losses from their sums; the last one adds all
+//   of them up in a fixed order.
 //
 // Memory is cut at 16-byte boundaries: granule j of a row holds the elements
 // whose bytes share the j-th aligned 16 bytes.  The gradient's rows start as
@@ -62,6 +62,7 @@ struct DistillRow {
   double all, rest, rho;  // sums, as multiples of 2^rho
   float top;       // the largest logit
   int wild;        // the sums are multiples of 2^(top c), not of 2^rho
+  double loss;     // times its weight
 };
 
 struct DistillArgs {
@@ -728,7 +729,32 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   if (joins == 0 && split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (rank != 0 || !a.loss) return;
 
-  // the last CTA computes the losses
+  // the losses of this CTA's rows, a thread each; a row that was not read has none
+  __syncthreads();
+  for (int64_t i = row0 + (int64_t)tid * row_step; i < rows; i += (int64_t)kDistThreads * row_step) {
+    const double w = a.weights ? (double)a.weights[i] : 1.0;
+    double l = 0.0;
+    DistillRow* k = a.row + i;
+    if (w != 0.0) {
+      const double mass = k->mass, all = k->all, top = (double)k->top, ref = (double)k->ref;
+      if (BUCKET || mass != 0.0) {
+        // log of the sum of e^((x - top) / T)
+        double logS = log(all);
+        if (!k->wild) logS += (k->rho + top * (kLog2e64 * a.inv_t - (double)c)) * kLn264 - top * a.inv_t;
+        if (mass != 0.0) l = k->entropy - (k->lean + (ref - top) * mass) * a.inv_t + mass * logS;
+        if (BUCKET && k->held < V) {
+          const double left = mass != mass ? mass : fmax(0.0, 1.0 - mass);
+          if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(k->rest, all)));
+        }
+      }
+      l *= w;
+    }
+    if (a.each) a.loss[i] = (float)l;
+    else k->loss = l;
+  }
+  if (a.each) return;
+  // the last CTA adds them up, in an order of its own
+  __syncthreads();
   if (tid == 0) {
     __threadfence();
     sh.last = atomicAdd(a.ticket, 1u) == (unsigned)row_step - 1u;
@@ -737,29 +763,8 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   if (!sh.last) return;
   __threadfence();
   double s = 0.0;
-  for (int64_t i = tid; i < a.rows; i += kDistThreads) {
-    const double w = a.weights ? (double)a.weights[i] : 1.0;
-    double l = 0.0;
-    if (w != 0.0) {
-      const DistillRow* k = a.row + i;
-      const double mass = k->mass, all = __ldcg(&k->all), rest = __ldcg(&k->rest), rho = __ldcg(&k->rho);
-      const double top = (double)__ldcg(&k->top), ref = (double)k->ref;
-      if (BUCKET || mass != 0.0) {
-        // log of the sum of e^((x - top) / T)
-        double logS = log(all);
-        if (!__ldcg(&k->wild)) logS += (rho + top * (kLog2e64 * a.inv_t - (double)c)) * kLn264 - top * a.inv_t;
-        if (mass != 0.0) l = k->entropy - (k->lean + (ref - top) * mass) * a.inv_t + mass * logS;
-        if (BUCKET && k->held < V) {
-          const double left = mass != mass ? mass : fmax(0.0, 1.0 - mass);
-          if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(rest, all)));
-        }
-      }
-      l *= w;
-    }
-    if (a.each) a.loss[i] = (float)l;
-    s += l;
-  }
-  if (a.each) return;
+#pragma unroll 4
+  for (int i = tid; i < rows; i += kDistThreads) s += __ldcg(&a.row[i].loss);
   s = warp_sum64(s);
   if (lane == 0) sh.loss[warp] = s;
   __syncthreads();
