@@ -18,6 +18,8 @@
 // a thread; of more, histograms leave that many first.  A part with more keys than the buffer holds
 // (long ties, as in a constant row) takes the plain way: one vector of every
 // thread at a time against a running threshold.
+// A part whose mask allows few tokens is not streamed: those elements are
+// gathered, and all of them become keys.
 // The cluster's CTAs put their lists and sums into one another's shared memory;
 // each finds its own keys' places in the row and writes those.
 //
@@ -293,6 +295,77 @@ __device__ __noinline__ ExpSum top_wild(const T* row, int off, const uint8_t* ma
   return acc;
 }
 
+// A part of a row whose mask allows few of its tokens.
+struct TopFound {
+  StepSum acc;  // the thread's share
+  float m;
+  bool all;     // the part's tokens were few enough
+};
+
+// Where [t0, t1) allows at most `cap` tokens, which shared memory holds next to
+// their ids, every allowed element becomes a key: only the mask and the sectors
+// of those elements are read, and no bound is needed.  Ids are placed by a scan
+// over the threads, so that a thread's share of the sum is the same every time.
+template <typename T>
+__device__ __noinline__ TopFound top_gather(TopShared& sh, const T* row, const uint32_t* words, int t0, int t1, int V,
+                                            int cap, float c) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int w0 = t0 * (kTopTile / 32), w1 = min(t1 * (kTopTile / 32), (V + 31) / 32);
+  auto word = [&](int w) { return __ldg(words + w) & (w * 32 + 32 > V ? (1u << (V & 31)) - 1u : ~0u); };
+  TopFound found;
+  found.acc.clear();
+  found.m = kNegInf;
+  int mine = 0;
+#pragma unroll 4
+  for (int w = w0 + tid; w < w1; w += kTopThreads) mine += __popc(word(w));
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kFull, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sh.scal[warp] = upto;
+  __syncthreads();
+  int total = 0, at = upto - mine;
+#pragma unroll
+  for (int i = 0; i < kTopWarps; ++i) {
+    if (i < warp) at += sh.scal[i];
+    total += sh.scal[i];
+  }
+  found.all = total <= cap;
+  if (!found.all) return found;
+  int* ids = reinterpret_cast<int*>(sh.buf() + cap);
+  for (int w = w0 + tid; w < w1; w += kTopThreads)
+    for (uint32_t bits = word(w); bits; bits &= bits - 1u) ids[at++] = w * 32 + __ffs(bits) - 1;
+  __syncthreads();
+  constexpr int U = 4;
+  for (int j = tid; j < total; j += U * kTopThreads) {
+    int id[U];
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      id[u] = j + u * kTopThreads < total ? ids[j + u * kTopThreads] : -1;
+      x[u] = id[u] >= 0 ? RowVec<T>::get(row + id[u]) : kNegInf;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      found.m = fmaxf(found.m, x[u]);
+      const float top = x[u] * c;
+      if (fabsf(top) < kWildExponent) {
+        const float magic = top + 12582912.0f;  // 1.5 2^23 + R
+        found.acc.add(ex2_approx(fmaf(x[u], c, 12582912.0f - magic)), (int)(__float_as_uint(magic) - 0x4B400000u));
+      } else if (x[u] < 0.0f) {
+        found.acc.low = found.acc.low || x[u] > kNegInf;
+      } else {
+        found.acc.high = true;
+        if (x[u] != x[u]) found.acc.s = nan64();
+      }
+      if (x[u] > kNegInf) sh.buf()[atomicAdd(&sh.count, 1)] = rankkey(x[u], (uint32_t)id[u]);
+    }
+  }
+  return found;
+}
+
 // The place-th largest of the warp's 64 values a, b; -inf if place > 64.
 __device__ __forceinline__ float warp_place(float a, float b, int place) {
   const int lane = threadIdx.x & 31;
@@ -362,133 +435,126 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   // element u of thread g in tile t
   auto at = [&](int t, int u, int g) { return t * kTopTile + (g >> 5) * kChunk + (u * 32 + (g & 31)) * n; };
 
-  // the warp's ring
-  unsigned char* ring = sh.rings() + warp * S * kTopStageBytes;
-  uint64_t* bar = sh.bar[warp];
-  const uint64_t policy = policy_evict_first();
-  auto issue = [&](int q, int st) {  // step q counts from t0
-    const int first = (t0 + q / kSteps) * kTopTile + warp * kChunk + q % kSteps * kStepElems;
-    if (q >= (t1 - t0) * kSteps || first >= V) return;
-    const char* src = reinterpret_cast<const char*>(row + first) - off;
-    // up to the 16-byte boundary at or behind the row's end
-    const int64_t left = (reinterpret_cast<const char*>(row + V) - src + 15) & ~(int64_t)15;
-    constexpr int most = ALIGNED ? kTopStep * 512 : kTopStep * 512 + 16;
-    const uint32_t bytes = left < most ? (uint32_t)left : (uint32_t)most;
-    mbar_arrive_expect_tx(&bar[st], bytes);
-    bulk_copy_g2s(ring + st * kTopStageBytes, src, bytes, &bar[st], policy);
-  };
-  if (lane == 0) {
-#pragma unroll
-    for (int st = 0; st < S; ++st) mbar_init(&bar[st], 1);
-    fence_proxy_async_smem();
-#pragma unroll
-    for (int st = 0; st < S; ++st) issue(st, st);
-  }
   if (tid == 0) { sh.count = 0; sh.got = 0; sh.listed = 0; sh.thr = kNegInf; }
-  // the allowed bits of the thread's U vectors, 32 in all
-  auto load_bits = [&](int t) {
-    uint32_t b = 0;
-    if (MASKED && t < t1) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) b |= top_bits<T>(mask, at(t, u, tid), V) << (u * n);
-    }
-    return b;
-  };
-  uint32_t bits = load_bits(t0);
-  __syncwarp();
-
   StepSum acc;
   acc.clear();
   float m0 = kNegInf, m1 = kNegInf;  // of every second tile each
-  int st = 0, q = 0;
-  uint32_t parity = 0;
-  bool arrived = true;
-  for (int t = t0; t < t1 && arrived; ++t) {
-    const uint32_t next_bits = load_bits(t + 1);
-    float tile_max = kNegInf;
+  bool gathered = false;
+  if (MASKED) {
+    // 12 bytes a key in the place of the rings and of the tiles' maxima; a part
+    // of which more is allowed is streamed as fast (1,030 rows of 35,439 fp32,
+    // gathered against streamed: 29 to 45 us at 2 %, 43 to 50 at 7 %; 600 of
+    // 20,000 bf16 at 14 %: 33 to 31)
+    const int room = (kTopRingBytes + per * kTopThreads * 2) / 12, few = (t1 - t0) * (kTopTile / 12);
+    const TopFound found = top_gather<T>(sh, row, reinterpret_cast<const uint32_t*>(mask), t0, t1, V,
+                                         room < few ? room : few, scale.c);
+    gathered = found.all;
+    if (gathered) {
+      acc = found.acc;
+      m0 = found.m;
+    }
+  }
+  if (!gathered) {
+    // the warp's ring
+    unsigned char* ring = sh.rings() + warp * S * kTopStageBytes;
+    uint64_t* bar = sh.bar[warp];
+    const uint64_t policy = policy_evict_first();
+    auto issue = [&](int q, int st) {  // step q counts from t0
+      const int first = (t0 + q / kSteps) * kTopTile + warp * kChunk + q % kSteps * kStepElems;
+      if (q >= (t1 - t0) * kSteps || first >= V) return;
+      const char* src = reinterpret_cast<const char*>(row + first) - off;
+      // up to the 16-byte boundary at or behind the row's end
+      const int64_t left = (reinterpret_cast<const char*>(row + V) - src + 15) & ~(int64_t)15;
+      constexpr int most = ALIGNED ? kTopStep * 512 : kTopStep * 512 + 16;
+      const uint32_t bytes = left < most ? (uint32_t)left : (uint32_t)most;
+      mbar_arrive_expect_tx(&bar[st], bytes);
+      bulk_copy_g2s(ring + st * kTopStageBytes, src, bytes, &bar[st], policy);
+    };
+    if (lane == 0) {
 #pragma unroll
-    for (int h = 0; h < kSteps; ++h, ++q) {
-      const int first = t * kTopTile + warp * kChunk + h * kStepElems;
-      if (first < V && arrived) {
-        arrived = __all_sync(kFull, mbar_wait(&bar[st], parity));
-        const unsigned char* from = ring + st * kTopStageBytes + lane * 16;
-        uint4 raw[kTopStep];
+      for (int st = 0; st < S; ++st) mbar_init(&bar[st], 1);
+      fence_proxy_async_smem();
 #pragma unroll
-        for (int u = 0; u < kTopStep; ++u) {
-          raw[u] = *reinterpret_cast<const uint4*>(from + u * 512);
-          if (!ALIGNED) raw[u] = shift_raw<T>(raw[u], *reinterpret_cast<const uint4*>(from + u * 512 + 16), off);
-        }
-        __syncwarp();
-        if (lane == 0 && arrived) {
-          fence_proxy_async_smem();
-          issue(q + S, st);
-        }
-        if (first + kStepElems > V) {
+      for (int st = 0; st < S; ++st) issue(st, st);
+    }
+    // the allowed bits of the thread's U vectors, 32 in all
+    auto load_bits = [&](int t) {
+      uint32_t b = 0;
+      if (MASKED && t < t1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) b |= top_bits<T>(mask, at(t, u, tid), V) << (u * n);
+      }
+      return b;
+    };
+    uint32_t bits = load_bits(t0);
+    __syncwarp();
+
+    int st = 0, q = 0;
+    uint32_t parity = 0;
+    bool arrived = true;
+    for (int t = t0; t < t1 && arrived; ++t) {
+      const uint32_t next_bits = load_bits(t + 1);
+      float tile_max = kNegInf;
+#pragma unroll
+      for (int h = 0; h < kSteps; ++h, ++q) {
+        const int first = t * kTopTile + warp * kChunk + h * kStepElems;
+        if (first < V && arrived) {
+          arrived = __all_sync(kFull, mbar_wait(&bar[st], parity));
+          const unsigned char* from = ring + st * kTopStageBytes + lane * 16;
+          uint4 raw[kTopStep];
 #pragma unroll
           for (int u = 0; u < kTopStep; ++u) {
-            const int left = V - (first + (u * 32 + lane) * n);
-            if (left < n) raw[u] = RowVec<T>::select(raw[u], left <= 0 ? 0u : (1u << left) - 1u);
+            raw[u] = *reinterpret_cast<const uint4*>(from + u * 512);
+            if (!ALIGNED) raw[u] = shift_raw<T>(raw[u], *reinterpret_cast<const uint4*>(from + u * 512 + 16), off);
           }
-        }
-        float vm[kTopStep];
+          __syncwarp();
+          if (lane == 0 && arrived) {
+            fence_proxy_async_smem();
+            issue(q + S, st);
+          }
+          if (first + kStepElems > V) {
 #pragma unroll
-        for (int u = 0; u < kTopStep; ++u) {
-          if (MASKED) raw[u] = RowVec<T>::select(raw[u], bits >> ((h * kTopStep + u) * n));
-          vm[u] = RowVec<T>::largest(raw[u]);
+            for (int u = 0; u < kTopStep; ++u) {
+              const int left = V - (first + (u * 32 + lane) * n);
+              if (left < n) raw[u] = RowVec<T>::select(raw[u], left <= 0 ? 0u : (1u << left) - 1u);
+            }
+          }
+          float vm[kTopStep];
+#pragma unroll
+          for (int u = 0; u < kTopStep; ++u) {
+            if (MASKED) raw[u] = RowVec<T>::select(raw[u], bits >> ((h * kTopStep + u) * n));
+            vm[u] = RowVec<T>::largest(raw[u]);
+          }
+          const float tm = max_nan(max_nan(vm[0], vm[1]), vm[2], vm[3]);
+          add_exps<T, kTopStep>(acc, raw, tm, scale.c);
+          tile_max = max_nan(tile_max, tm);
+          if (++st == S) { st = 0; parity ^= 1; }
         }
-        const float tm = max_nan(max_nan(vm[0], vm[1]), vm[2], vm[3]);
-        add_exps<T, kTopStep>(acc, raw, tm, scale.c);
-        tile_max = max_nan(tile_max, tm);
+      }
+      tops[(t - t0) * kTopThreads + tid] = (uint16_t)(ordkey(tile_max) >> 16);
+      const float mx = fmaxf(m0, tile_max);
+      m0 = m1;
+      m1 = mx;
+      bits = next_bits;
+    }
+    if (!arrived) {
+      // give the copies in flight their time before their memory is used again
+      for (int j = 1; j < S; ++j) {
+        mbar_wait(&bar[st], parity);
         if (++st == S) { st = 0; parity ^= 1; }
       }
+      acc.s = nan64();
+      m0 = m1 = kNegInf;
     }
-    tops[(t - t0) * kTopThreads + tid] = (uint16_t)(ordkey(tile_max) >> 16);
-    const float mx = fmaxf(m0, tile_max);
-    m0 = m1;
-    m1 = mx;
-    bits = next_bits;
-  }
-  if (!arrived) {
-    // give the copies in flight their time before their memory is used again
-    for (int j = 1; j < S; ++j) {
-      mbar_wait(&bar[st], parity);
-      if (++st == S) { st = 0; parity ^= 1; }
-    }
-    acc.s = nan64();
-    m0 = m1 = kNegInf;
   }
 
-  // the bound: the warp's `place`-th largest of its lanes' 64 maxima
+  // the warp's largest exponent and element
   const float m = fmaxf(m0, m1);
-  float o = warp_place(m0, m1, (K + kTopWarps - 1) / kTopWarps);
-  // and the largest exponent and element
   const double wrho = warp_max64(acc.sum().rho);
   const float wm = warp_max_ordered(m);
-  if (lane == 0) { sh.wbound[warp] = o; sh.wrho[warp] = wrho; sh.wmax[warp] = wm; }
-  __syncthreads();
-  float bound = -warp_max_ordered(-sh.wbound[lane % kTopWarps]);
-  // warps that hold nothing (behind the row's end, nothing allowed): the
-  // others' share is larger
-  const int holding = __popc(__ballot_sync(kFull, sh.wmax[lane % kTopWarps] > kNegInf)) / (32 / kTopWarps);
-  if (holding > 0 && holding < kTopWarps) {
-    o = warp_place(m0, m1, (K + holding - 1) / holding);
-    __syncthreads();
-    if (lane == 0) sh.wbound[warp] = wm > kNegInf ? o : -kNegInf;
-    __syncthreads();
-    bound = -warp_max_ordered(-sh.wbound[lane % kTopWarps]);
-  }
-  const float below = bound > kNegInf ? float_below(bound) : kNegInf;
-  if (m > below) {
-    // without a bound every tile that holds anything
-    const uint32_t least = (ordkey(bound) >> 16) + (bound > kNegInf ? 0u : 1u);
-    for (int t = t0; t < t1; ++t)
-      if (tops[(t - t0) * kTopThreads + tid] >= least) {
-        const int pos = atomicAdd(&sh.listed, 1);
-        if (pos < kTopList) sh.list()[pos] = (uint16_t)((t - t0) * kTopThreads + tid);
-      }
-  }
-  __syncthreads();
-  const int listed = sh.listed;
+  if (lane == 0) { sh.wrho[warp] = wrho; sh.wmax[warp] = wm; }
+  int listed = 0;
+  float below = kNegInf;
   auto offer = [&](float above) {
     for (int j = tid; j < listed * U; j += kTopThreads) {
       const int g = sh.list()[j / U];
@@ -496,7 +562,38 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
       top_offer<T>(sh, top_load<T, MASKED, ALIGNED>(row, off, mask, i, V), (uint32_t)i, above);
     }
   };
-  if (listed <= kTopList) offer(below);
+  if (!gathered) {
+    // the bound: the warp's `place`-th largest of its lanes' 64 maxima
+    float o = warp_place(m0, m1, (K + kTopWarps - 1) / kTopWarps);
+    if (lane == 0) sh.wbound[warp] = o;
+    __syncthreads();
+    float bound = -warp_max_ordered(-sh.wbound[lane % kTopWarps]);
+    // warps that hold nothing (behind the row's end, nothing allowed): the
+    // others' share is larger
+    const int holding = __popc(__ballot_sync(kFull, sh.wmax[lane % kTopWarps] > kNegInf)) / (32 / kTopWarps);
+    if (holding > 0 && holding < kTopWarps) {
+      o = warp_place(m0, m1, (K + holding - 1) / holding);
+      __syncthreads();
+      if (lane == 0) sh.wbound[warp] = wm > kNegInf ? o : -kNegInf;
+      __syncthreads();
+      bound = -warp_max_ordered(-sh.wbound[lane % kTopWarps]);
+    }
+    if (bound > kNegInf) below = float_below(bound);
+    if (m > below) {
+      // without a bound every tile that holds anything
+      const uint32_t least = (ordkey(bound) >> 16) + (bound > kNegInf ? 0u : 1u);
+      for (int t = t0; t < t1; ++t)
+        if (tops[(t - t0) * kTopThreads + tid] >= least) {
+          const int pos = atomicAdd(&sh.listed, 1);
+          if (pos < kTopList) sh.list()[pos] = (uint16_t)((t - t0) * kTopThreads + tid);
+        }
+    }
+    __syncthreads();
+    listed = sh.listed;
+    if (listed <= kTopList) offer(below);
+  } else {
+    __syncthreads();
+  }
   double rho = warp_max64(sh.wrho[lane % kTopWarps]);
   ExpSum mine = acc.sum();
   if (__syncthreads_or(acc.wild(warp_max_ordered(sh.wmax[lane % kTopWarps]), scale.c) && acc.s == acc.s)) {
@@ -511,7 +608,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   __syncthreads();
   if (listed > kTopList) {
     top_plain<T, MASKED, ALIGNED>(sh, row, off, mask, t0 * kTopTile, t1 * kTopTile, V, K);
-  } else if (sh.count > kTopBuf) {
+  } else if (!gathered && sh.count > kTopBuf) {
     // a part of few tiles at a large k: the k-th of some of its elements is a
     // better bound, once
     __syncthreads();

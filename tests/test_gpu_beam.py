@@ -314,3 +314,29 @@ def test_top_short_parts_with_ties():
     x[2, 5000:] = 2.0
     _check_top(x, 256)
     _check_top(x.to(torch.bfloat16), 200)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V,k,allowed", [
+    (3, 151937, 64, 3000), (2, 8192, 256, 682), (2, 8192, 256, 683), (2, 8192, 256, 684), (700, 40001, 130, 800),
+    (400, 163840, 20, 3605), (400, 163840, 20, 3606), (3, 70001, 5, 0), (3, 70001, 5, 3)])
+def test_top_few_allowed(dtype, rows, V, k, allowed):
+    """Masks of an exact number of tokens, on both sides of where a part's
+    tokens are gathered, the last token and the first among them; bits behind
+    the vocabulary are set."""
+    rng = np.random.default_rng(rows + V + allowed)
+    keep = np.zeros((8, V), dtype=bool)
+    for r in range(8):
+        at = [0, V - 1][:allowed]
+        keep[r, np.concatenate([at, rng.permutation(np.arange(1, V - 1))[:max(allowed - 2, 0)]]).astype(np.int64)] = True
+    words = P.pack_bits(np.pad(keep, ((0, 0), (0, -V % 32)), constant_values=True))
+    base = _logits(7, 8, V, dtype)
+    x = base.repeat((rows + 7) // 8, 1)[:rows].contiguous()
+    mask = torch.from_numpy(words.view(np.int32)).to(DEV).repeat((rows + 7) // 8, 1)[:rows].contiguous()
+    got = pm.top_logprobs(x, k, mask=mask, return_lse=True)
+    n = min(8, rows)
+    ids, lp, lse = P.top_logprobs(base[:n].double().cpu().numpy(), k, 1.0, keep[:n])
+    for first in (0, (rows - n) // 8 * 8):
+        np.testing.assert_array_equal(got["ids"][first:first + n].cpu().numpy(), ids)
+        _close(got["logprobs"][first:first + n], lp)
+        _close(got["lse"][first:first + n], lse)
