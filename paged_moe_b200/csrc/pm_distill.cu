@@ -1,9 +1,10 @@
 // pm_distill.cu -- distillation loss from a teacher's top log-probabilities,
-// and its gradient.  Two kernels:
+// and its gradient.  The entries' kernel and one of two for the rows:
 //
 // k_distill_prep, a warp per row: the row's entries become probabilities in
 //   64 bits (the mass they leave is a difference of nearly equal numbers), the
 //   entries of one id added up, next to their logits.
+// k_distill_short, a warp per row, where there are many short ones.
 // k_distill_rows, two CTAs per SM that take row after row, or a cluster per
 //   row where there are few.  Every warp streams its chunks through a ring in
 //   shared memory that its first lane keeps full with bulk copies: once forward
@@ -38,6 +39,8 @@ namespace pm {
 constexpr int kDistThreads = 384;
 constexpr int kDistWarps = kDistThreads / 32;
 constexpr int kDistResident = 2;               // CTAs of an SM
+constexpr int kShortThreads = 256, kShortWarps = kShortThreads / 32;
+constexpr int64_t kShortBytes = 64 << 10;      // of a row that a warp takes alone, half as many for its gradient
 constexpr int kDistMax = 256;                  // largest k
 constexpr int kDistTableBits = 9;              // a table for twice as many ids
 constexpr int kDistHeld = kDistMax / 32;       // entries of a lane
@@ -352,13 +355,13 @@ __device__ __forceinline__ double dist_factor(double mass, double rest, double a
 // once they are known (S > 0) the gradient.
 template <typename T>
 __device__ __noinline__ void dist_wild(const DistillArgs& a, int64_t r, int i0, int i1, float top, double on, double off,
-                                       double by, bool store, double* all, double* rest) {
+                                       double by, bool store, int first, int step, double* all, double* rest) {
   const int K = a.k;
   const T* x = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
   T* g = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
   const float c = (float)(kLog2e64 * a.inv_t);
   const int32_t* at = a.at + r * K;
-  for (int i = i0 + (int)threadIdx.x; i < i1; i += kDistThreads) {
+  for (int i = i0 + first; i < i1; i += step) {
     const double e = (double)ex2_approx((RowVec<T>::get(x + i) - top) * c);
     int k = 0;
     while (k < K && at[k] != i) ++k;
@@ -393,6 +396,113 @@ __device__ __noinline__ void dist_edge(T* grow, uint4 r0, uint4 r1, uint4 r2, ui
       if (i >= 0 && i < V) put_grad(grow + i, v[e]);
     }
   }
+}
+
+// Adds four vectors to a thread's sums, those whose bit of `marked` is set to
+// the first only.
+template <typename T, bool BUCKET>
+__device__ __forceinline__ void dist_add(const uint4 (&raw)[kDistStep], uint32_t marked, float c, DistillSum& sums,
+                                         float& m, int& flags) {
+  constexpr int n = RowVec<T>::n;
+  const uint64_t c2 = pk(c, c);
+  const float tm = max_nan(max_nan(RowVec<T>::largest(raw[0]), RowVec<T>::largest(raw[1])),
+                           RowVec<T>::largest(raw[2]), RowVec<T>::largest(raw[3]));
+  m = fmaxf(m, tm);
+  const float top = tm * c;
+  if (fabsf(top) < kWildExponent) {
+    const float magic = top + 12582912.0f;  // 1.5 2^23 + R
+    const float R = magic - 12582912.0f;
+    const uint64_t r2 = pk(-R, -R);
+    uint64_t sum0 = 0, sum1 = 0;     // of vectors without a mark
+    float with = 0.0f, kept = 0.0f;  // of those with one: all elements, and the unmarked
+#pragma unroll
+    for (int u = 0; u < kDistStep; ++u) {
+      float v[n];
+      RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+      for (int e = 0; e < n; e += 2) {
+        const uint64_t x = fma2(pk(v[e], v[e + 1]), c2, r2);
+        v[e] = ex2_approx(lo_f(x));
+        v[e + 1] = ex2_approx(hi_f(x));
+      }
+      const uint32_t bits = BUCKET ? (marked >> (u * n)) & ((1u << n) - 1u) : 0u;
+      if (bits == 0) {
+#pragma unroll
+        for (int e = 0; e < n; e += 4) {
+          sum0 = add2(sum0, pk(v[e], v[e + 1]));
+          sum1 = add2(sum1, pk(v[e + 2], v[e + 3]));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+          with += v[e];
+          kept += (bits >> e) & 1 ? 0.0f : v[e];
+        }
+      }
+    }
+    const uint64_t sum = add2(sum0, sum1);
+    const float plain = lo_f(sum) + hi_f(sum);
+    sums.template add<BUCKET>(plain + with, plain + kept, (int)(__float_as_uint(magic) - 0x4B400000u));
+  } else if (tm < 0.0f) {
+    flags |= tm > kNegInf ? kPartLow : 0;
+  } else {
+    flags |= kPartHigh;
+    if (tm != tm) sums.all = sums.rest = nan64();
+  }
+}
+
+// Four vectors' gradients: 2^(x c - R) f.
+template <typename T>
+__device__ __forceinline__ void dist_grads(uint4 (&raw)[kDistStep], uint64_t c2, uint64_t r2, uint64_t f2) {
+  constexpr int n = RowVec<T>::n;
+#pragma unroll
+  for (int u = 0; u < kDistStep; ++u) {
+    float v[n];
+    RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+    for (int e = 0; e < n; e += 2) {
+      const uint64_t x = fma2(pk(v[e], v[e + 1]), c2, r2);
+      const uint64_t y = mul2(pk(ex2_approx(lo_f(x)), ex2_approx(hi_f(x))), f2);
+      v[e] = lo_f(y);
+      v[e + 1] = hi_f(y);
+    }
+    raw[u] = pack_grad(v);
+  }
+}
+
+// Whether a row's sums have left something out that counts.
+__device__ __forceinline__ bool dist_is_wild(const DistillPart& p, float c) {
+  return ((p.flags & kPartHigh) || ((p.flags & kPartLow) && !(p.top * c > -kWildExponent + 4096.0f))) && p.all == p.all;
+}
+
+// What the gradient of logits x is: 2^(x c - rho) `factor`, at an entry
+// 2^(x c - rho) `on` - p `by`.
+struct DistillFactors {
+  double by, on, factor;
+};
+template <bool BUCKET>
+__device__ __forceinline__ DistillFactors dist_factors(double by, double mass, int held, int V, double all, double rest) {
+  const double inverse = dist_inverse(all), on = by * inverse;
+  // without a token outside the entries nothing is left for the bucket
+  return {by, on, BUCKET && held < V ? on * dist_factor(mass, rest, all, inverse) : on};
+}
+
+// The loss of a row whose sums are known.
+template <bool BUCKET>
+__device__ __forceinline__ double dist_loss(const DistillArgs& a, const DistillRow& k, float c) {
+  double l = 0.0;
+  if (BUCKET || k.mass != 0.0) {
+    const double top = (double)k.top, ref = (double)k.ref;
+    // log of the sum of e^((x - top) / T)
+    double logS = log(k.all);
+    if (!k.wild) logS += (k.rho + top * (kLog2e64 * a.inv_t - (double)c)) * kLn264 - top * a.inv_t;
+    if (k.mass != 0.0) l = k.entropy - (k.lean + (ref - top) * k.mass) * a.inv_t + k.mass * logS;
+    if (BUCKET && k.held < a.vocab) {
+      const double left = k.mass != k.mass ? k.mass : fmax(0.0, 1.0 - k.mass);
+      if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(k.rest, k.all)));
+    }
+  }
+  return l;
 }
 
 template <typename T, bool BUCKET>
@@ -582,50 +692,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
 #pragma unroll
         for (int u = 0; u < kDistStep; ++u) raw[u] = dist_clip<T>(raw[u], p.first + (j0 + u * 32 + lane) * n, V);
       }
-      const float tm = max_nan(max_nan(RowVec<T>::largest(raw[0]), RowVec<T>::largest(raw[1])),
-                               RowVec<T>::largest(raw[2]), RowVec<T>::largest(raw[3]));
-      m = fmaxf(m, tm);
-      const float top = tm * c;
-      if (fabsf(top) < kWildExponent) {
-        const float magic = top + 12582912.0f;  // 1.5 2^23 + R
-        const float R = magic - 12582912.0f;
-        const uint64_t r2 = pk(-R, -R);
-        uint64_t sum0 = 0, sum1 = 0;     // of vectors without a mark
-        float with = 0.0f, kept = 0.0f;  // of those with one: all elements, and the unmarked
-#pragma unroll
-        for (int u = 0; u < kDistStep; ++u) {
-          float v[n];
-          RowVec<T>::unpack(raw[u], v);
-#pragma unroll
-          for (int e = 0; e < n; e += 2) {
-            const uint64_t x = fma2(pk(v[e], v[e + 1]), c2, r2);
-            v[e] = ex2_approx(lo_f(x));
-            v[e + 1] = ex2_approx(hi_f(x));
-          }
-          const uint32_t bits = BUCKET ? (marked >> (u * n)) & ((1u << n) - 1u) : 0u;
-          if (bits == 0) {
-#pragma unroll
-            for (int e = 0; e < n; e += 4) {
-              sum0 = add2(sum0, pk(v[e], v[e + 1]));
-              sum1 = add2(sum1, pk(v[e + 2], v[e + 3]));
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < n; ++e) {
-              with += v[e];
-              kept += (bits >> e) & 1 ? 0.0f : v[e];
-            }
-          }
-        }
-        const uint64_t sum = add2(sum0, sum1);
-        const float plain = lo_f(sum) + hi_f(sum);
-        sums.template add<BUCKET>(plain + with, plain + kept, (int)(__float_as_uint(magic) - 0x4B400000u));
-      } else if (tm < 0.0f) {
-        flags |= tm > kNegInf ? kPartLow : 0;
-      } else {
-        flags |= kPartHigh;
-        if (tm != tm) sums.all = sums.rest = nan64();
-      }
+      dist_add<T, BUCKET>(raw, marked, c, sums, m, flags);
     }
     if (lost) sums.all = sums.rest = nan64();
     DistillPart part = {sums.all, sums.rest, sums.rho, m, flags};
@@ -633,13 +700,12 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
     ++joins;
     const Row next = ask(after);
     const float top = part.top;
-    const bool wild = ((part.flags & kPartHigh) || ((part.flags & kPartLow) && !(top * c > -kWildExponent + 4096.0f))) &&
-                      part.all == part.all;
+    const bool wild = dist_is_wild(part, c);
     const int i0 = p.first > 0 ? p.first : 0, i1 = p.first + p.count * n < V ? p.first + p.count * n : V;
     if (wild) {
       // every CTA sums the whole row
       double all = 0.0, rest = 0.0;
-      dist_wild<T>(a, r, 0, V, top, 0.0, 0.0, 0.0, false, &all, &rest);
+      dist_wild<T>(a, r, 0, V, top, 0.0, 0.0, 0.0, false, tid, kDistThreads, &all, &rest);
       part = {all, rest, 0, top, 0};
       part = dist_join(sh, part, joins, 0, 1);
       ++joins;
@@ -660,9 +726,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
       T* grow = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
       const bool vectors = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
       uint4* out = reinterpret_cast<uint4*>(grow + p.first);
-      const double by = scale * (double)now.w, inverse = dist_inverse(all), on = by * inverse;
-      // without a token outside the entries nothing is left for the bucket
-      const double factor = BUCKET && now.held < V ? on * dist_factor(now.mass, part.rest, all, inverse) : on;
+      const DistillFactors f = dist_factors<BUCKET>(scale * (double)now.w, now.mass, now.held, V, all, part.rest);
       if (wild || empty) {
         // the copies are not wanted, but others follow them
         uint4 raw[kDistStep];
@@ -671,34 +735,22 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
           zeros(r, p);
         } else {
           double s0 = 0.0, s1 = 0.0;
-          dist_wild<T>(a, r, i0, i1, top, on, factor, by, true, &s0, &s1);
+          dist_wild<T>(a, r, i0, i1, top, f.on, f.factor, f.by, true, tid, kDistThreads, &s0, &s1);
         }
         if (BUCKET) {
           if (after < rows) mark(after, next.id);
           __syncthreads();
         }
       } else {
-        const float f = (float)factor;
-        const uint64_t r2 = pk(-(float)part.rho, -(float)part.rho), f2 = pk(f, f);
+        const float by = (float)f.factor;
+        const uint64_t r2 = pk(-(float)part.rho, -(float)part.rho), f2 = pk(by, by);
         // chunks from lo to hi lie wholly inside the row
         const int lo = vectors ? p.whole0 : 0x7fffffff, hi = p.whole1 - kDistChunk;
         for (int t = p.chunks - 1; t >= 0; --t) {
           const int j0 = t * kDistTile + warp * kDistChunk;
           uint4 raw[kDistStep];
           take(raw);
-#pragma unroll
-          for (int u = 0; u < kDistStep; ++u) {
-            float v[n];
-            RowVec<T>::unpack(raw[u], v);
-#pragma unroll
-            for (int e = 0; e < n; e += 2) {
-              const uint64_t x = fma2(pk(v[e], v[e + 1]), c2, r2);
-              const uint64_t y = mul2(pk(ex2_approx(lo_f(x)), ex2_approx(hi_f(x))), f2);
-              v[e] = lo_f(y);
-              v[e + 1] = hi_f(y);
-            }
-            raw[u] = pack_grad(v);
-          }
+          dist_grads<T>(raw, c2, r2, f2);
           if (j0 >= lo && j0 <= hi) {
             uint4* to = out + j0 + lane;
 #pragma unroll
@@ -712,7 +764,7 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
         __syncthreads();
         if (now.id >= i0 && now.id < i1) {  // none is -1, i0 is at least 0
           const double q = (double)ex2_approx(fmaf(now.x, c, -(float)part.rho));
-          put_grad(grow + now.id, (float)(q * on - now.p * by));
+          put_grad(grow + now.id, (float)(q * f.on - now.p * f.by));
         }
       }
     } else if (BUCKET) {
@@ -733,24 +785,9 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   __syncthreads();
   for (int64_t i = row0 + (int64_t)tid * row_step; i < rows; i += (int64_t)kDistThreads * row_step) {
     const double w = a.weights ? (double)a.weights[i] : 1.0;
-    double l = 0.0;
-    DistillRow* k = a.row + i;
-    if (w != 0.0) {
-      const double mass = k->mass, all = k->all, top = (double)k->top, ref = (double)k->ref;
-      if (BUCKET || mass != 0.0) {
-        // log of the sum of e^((x - top) / T)
-        double logS = log(all);
-        if (!k->wild) logS += (k->rho + top * (kLog2e64 * a.inv_t - (double)c)) * kLn264 - top * a.inv_t;
-        if (mass != 0.0) l = k->entropy - (k->lean + (ref - top) * mass) * a.inv_t + mass * logS;
-        if (BUCKET && k->held < V) {
-          const double left = mass != mass ? mass : fmax(0.0, 1.0 - mass);
-          if (!(left <= 0.0)) l += left * (log(left) - log(dist_tail(k->rest, all)));
-        }
-      }
-      l *= w;
-    }
+    const double l = w != 0.0 ? dist_loss<BUCKET>(a, a.row[i], c) * w : 0.0;
     if (a.each) a.loss[i] = (float)l;
-    else k->loss = l;
+    else a.row[i].loss = l;
   }
   if (a.each) return;
   // the last CTA adds them up, in an order of its own
@@ -770,6 +807,175 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   __syncthreads();
   if (tid == 0) {
     for (int i = 1; i < kDistWarps; ++i) s += sh.loss[i];
+    if (a.mean) {
+      const double weights = a.weights ? *a.weight_sum : (double)a.rows;
+      s = weights != 0.0 ? s / weights : 0.0;
+    }
+    *a.loss = (float)s;
+  }
+}
+
+// Short rows: a warp each, in chunks of four vectors a lane that are read from
+// memory, and from L1 for the gradient.  There is no barrier, and what a row
+// costs besides its elements (its sums' joining, its factors, its loss) is one
+// warp's work instead of twelve.
+template <typename T, bool BUCKET>
+__global__ void __launch_bounds__(kShortThreads, 2) k_distill_short(DistillArgs a) {
+  constexpr int n = RowVec<T>::n;
+  constexpr int kChunks = (int)(kShortBytes / 16 / kDistChunk) + 1;  // a row off a boundary has a granule more
+  __shared__ uint32_t s_marks[kShortWarps][BUCKET ? kChunks * 32 : 1];
+  __shared__ double s_loss[kShortWarps];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = (int)a.vocab, K = a.k;
+  const int64_t r = (int64_t)blockIdx.x * kShortWarps + warp;
+  const float c = (float)(kLog2e64 * a.inv_t);
+  const uint64_t c2 = pk(c, c);
+  const float weight = r >= a.rows ? 0.0f : a.weights ? a.weights[r] : 1.0f;
+  const bool read = r < a.rows && weight != 0.0f;
+  const T* row = reinterpret_cast<const T*>(a.logits) + r * a.row_stride;
+  T* grow = reinterpret_cast<T*>(a.grad) + r * a.grad_stride;
+  const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);
+  const int granules = (off + V + n - 1) / n, chunks = (granules + kDistChunk - 1) / kDistChunk;
+  const int whole0 = off ? 1 : 0, whole1 = granules * n - off > V ? granules - 1 : granules;  // those inside the row
+  const bool vectors = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grow)) & 15) == 0;
+  auto load = [&](int t, uint4 (&raw)[kDistStep]) {
+    const uint4* src = reinterpret_cast<const uint4*>(row - off);
+#pragma unroll
+    for (int u = 0; u < kDistStep; ++u) {
+      const int j = t * kDistChunk + u * 32 + lane;
+      raw[u] = j < granules ? __ldg(src + j) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  DistillSum sums = {0.0, 0.0, StepSum::kNothing};
+  float m = kNegInf;
+  int flags = 0;
+  auto forward = [&] {
+    uint4 next[kDistStep];
+    load(0, next);
+    for (int t = 0; t < chunks; ++t) {
+      uint4 raw[kDistStep];
+#pragma unroll
+      for (int u = 0; u < kDistStep; ++u) raw[u] = next[u];
+      if (t + 1 < chunks) load(t + 1, next);
+      if (t * kDistChunk < whole0 || (t + 1) * kDistChunk > whole1) {
+#pragma unroll
+        for (int u = 0; u < kDistStep; ++u) raw[u] = dist_clip<T>(raw[u], (t * kDistChunk + u * 32 + lane) * n - off, V);
+      }
+      dist_add<T, BUCKET>(raw, BUCKET ? s_marks[warp][t * 32 + lane] : 0u, c, sums, m, flags);
+    }
+  };
+  if (!BUCKET && read) forward();
+  cudaGridDependencySynchronize();  // the entries, and the sum of the weights
+  if (BUCKET && read) {
+    for (int t = 0; t < chunks; ++t) s_marks[warp][t * 32 + lane] = 0;
+    __syncwarp();
+    for (int i = lane; i < K; i += 32) {
+      const int id = a.at[r * K + i], j = (id + off) / n;
+      if (id >= 0)
+        atomicOr(&s_marks[warp][j / kDistChunk * 32 + j % 32], 1u << (j % kDistChunk / 32 * n + (id + off) % n));
+    }
+    __syncwarp();
+    forward();
+  }
+  // every granule of the gradient's row
+  auto store = [&](int t, const uint4 (&raw)[kDistStep]) {
+#pragma unroll
+    for (int u = 0; u < kDistStep; ++u) {
+      const int j = t * kDistChunk + u * 32 + lane;
+      if (vectors && j >= whole0 && j < whole1) {
+        __stcs(reinterpret_cast<uint4*>(grow - off) + j, raw[u]);
+      } else if (j < granules) {
+        float v[n];
+        RowVec<T>::unpack(raw[u], v);
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+          const int i = j * n + e - off;
+          if (i >= 0 && i < V) put_grad(grow + i, v[e]);
+        }
+      }
+    }
+  };
+  auto zeros = [&] {
+    const uint4 none[kDistStep] = {};
+    for (int t = 0; t < chunks; ++t) store(t, none);
+  };
+  double loss = 0.0;
+  if (read) {
+    DistillPart part = dist_reduce({sums.all, sums.rest, sums.rho, m, flags});
+    const float top = part.top;
+    const bool wild = dist_is_wild(part, c);
+    if (wild) {
+      double all = 0.0, rest = 0.0;
+      dist_wild<T>(a, r, 0, V, top, 0.0, 0.0, 0.0, false, lane, 32, &all, &rest);
+      part = dist_reduce({all, rest, 0, top, 0});
+    }
+    DistillRow k = a.row[r];
+    k.all = top == kNegInf ? nan64() : part.all;  // no finite logit: no distribution
+    k.rest = part.rest;
+    k.rho = (double)part.rho;
+    k.top = top;
+    k.wild = wild;
+    if (a.grad) {
+      double scale = a.inv_t;
+      if (a.mean) {
+        const double weights = a.weights ? *a.weight_sum : (double)a.rows;
+        scale = weights != 0.0 ? scale / weights : 0.0;
+      }
+      if (a.grad_loss) scale *= (double)a.grad_loss[a.each ? r : 0];
+      const DistillFactors f = dist_factors<BUCKET>(scale * (double)weight, k.mass, k.held, V, k.all, k.rest);
+      if (!BUCKET && k.mass == 0.0) {
+        zeros();
+      } else if (wild) {
+        double s0 = 0.0, s1 = 0.0;
+        dist_wild<T>(a, r, 0, V, top, f.on, f.factor, f.by, true, lane, 32, &s0, &s1);
+      } else {
+        const float by = (float)f.factor;
+        const uint64_t r2 = pk(-(float)part.rho, -(float)part.rho), f2 = pk(by, by);
+        for (int t = 0; t < chunks; ++t) {
+          uint4 raw[kDistStep];
+          load(t, raw);
+          dist_grads<T>(raw, c2, r2, f2);
+          store(t, raw);
+        }
+        // the entries' elements once more, q - p, behind the warp's own stores
+        __syncwarp();
+        for (int i = lane; i < K; i += 32) {
+          const int id = a.at[r * K + i];
+          if (id < 0) continue;
+          const double q = (double)ex2_approx(fmaf(a.x[r * K + i], c, -(float)part.rho));
+          put_grad(grow + id, (float)(q * f.on - a.p[r * K + i] * f.by));
+        }
+      }
+    }
+    if (a.loss && lane == 0) loss = dist_loss<BUCKET>(a, k, c) * (double)weight;
+  } else if (r < a.rows && a.grad) {
+    zeros();
+  }
+  if (!a.loss) return;
+  if (a.each) {
+    if (lane == 0 && r < a.rows) a.loss[r] = (float)loss;
+    return;
+  }
+  // the CTA's sum, and all CTAs' in the last one
+  if (lane == 0) s_loss[warp] = loss;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < kShortWarps; ++i) loss += s_loss[i];
+    a.row[r].loss = loss;
+    __threadfence();
+    s_last = atomicAdd(a.ticket, 1u) == gridDim.x - 1u;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = tid; i < (int)gridDim.x; i += kShortThreads) s += __ldcg(&a.row[(int64_t)i * kShortWarps].loss);
+  s = warp_sum64(s);
+  if (lane == 0) s_loss[warp] = s;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < kShortWarps; ++i) s += s_loss[i];
     if (a.mean) {
       const double weights = a.weights ? *a.weight_sum : (double)a.rows;
       s = weights != 0.0 ? s / weights : 0.0;
@@ -874,12 +1080,21 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
   pm::k_distill_prep<T><<<(unsigned)row_grid, pm::kRowThreads, 0, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
+  const int64_t slots = (int64_t)pmh::num_sms() * pm::kDistResident;
+  // Many short rows go to a warp each.  A CTA's rows follow one another, a warp
+  // is slower on its row: 2,007 rows of 2,401 fp32 take 27 us against 49, 2,048
+  // of 16,384 bf16 47 against 66, 600 of those 32 against 29, 2,048 of 32,768
+  // 45 against 60 for the loss alone but 93 against 93 with the gradient.
+  const int64_t bytes_of_row = a.vocab * (int64_t)sizeof(T), unit = 16 << 10;
+  if (bytes_of_row * (a.grad ? 2 : 1) <= pm::kShortBytes &&
+      a.rows * 4 * unit > slots * 5 * (bytes_of_row > unit ? bytes_of_row : unit))
+    return launch_after(pm::k_distill_short<T, BUCKET>, (a.rows + pm::kShortWarps - 1) / pm::kShortWarps, pm::kShortThreads,
+                        0, 1, st, a);
   // CTAs of a row: as many as keep every SM's two, no more than it has tiles
   auto* kernel = pm::k_distill_rows<T, BUCKET>;
   constexpr int n = pm::RowVec<T>::n;
   const int64_t granules = (a.vocab + n - 1) / n + 1;  // one more where a row starts off a boundary
   const int64_t tiles = (granules + pm::kDistTile - 1) / pm::kDistTile;
-  const int64_t slots = (int64_t)pmh::num_sms() * pm::kDistResident;
   int split = 1;
   while (split < pm::kDistSplit && 2 * split <= tiles && a.rows * 2 * split <= slots) split *= 2;
   const int64_t mark_tiles = (tiles + split - 1) / split;

@@ -345,3 +345,50 @@ def test_no_second_derivative(reduction):
     grad = torch.autograd.grad(loss, x, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="second derivative"):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("tail", ["drop", "bucket"])
+@pytest.mark.parametrize("N,V,dtype", [(371, 60, torch.float32), (400, 8191, torch.bfloat16), (380, 4096, torch.float32),
+                                       (2, 20011, torch.float32), (300, 5000, torch.bfloat16)])
+def test_rows_that_need_care(N, V, dtype, tail):
+    """Rows for a warp each and rows for CTAs and clusters: constant rows,
+    rows far from zero, rows with few finite logits, ids twice, outside and
+    none, weights of zero, one row on its own in the last CTA."""
+    x, ids, lps = _case(50 + N, N, V, 7, dtype, pad=3, offset=1)
+    x[0] = 2.0
+    x[1] *= 1000.0
+    if N > 2:
+        x[2] = float("-inf")
+        x[2, [0, V // 2, V - 1]] = torch.tensor([1.0, 2.0, 0.5], dtype=dtype, device=DEV)
+        ids[2, :3] = torch.tensor([V - 1, 0, V // 2], dtype=torch.int32, device=DEV)  # an entry of no mass has an infinite loss
+        ids[2, 3:] = -1
+        x[3] -= 60000.0
+        x[4] *= 3.0e6
+        ids[5, 1] = ids[5, 0]
+        ids[6] = -1
+        ids[7, 2] = V
+        ids[8, 3] = ids[8, 1] = ids[8, 0]
+    lps = torch.log_softmax(lps, 1) - 0.1
+    w = np.ones(N, dtype=np.float32)
+    w[N // 2:N // 2 + 9] = 0.0
+    w[N - 1] = 2.5
+    _check(x, ids, lps, temp=1.3, tail=tail, weights=w, reduction="mean")
+    _check(x, ids, lps, temp=1.3, tail=tail, weights=w, reduction="none", up=np.ones(N, dtype=np.float32))
+
+
+def test_no_distribution_and_no_weight_on_both_sides():
+    for N, V in ((400, 500), (3, 30011)):
+        x, ids, lps = _case(60, N, V, 4)
+        x[1] = float("-inf")
+        x[2, 7] = float("nan")
+        leaf = x.clone().requires_grad_()
+        loss = pm.distill_loss(leaf, ids, lps, reduction="none")
+        grad = torch.autograd.grad(loss.sum(), leaf)[0]
+        assert torch.isnan(loss[1:3]).all() and torch.isnan(grad[1:3]).all()
+        assert not torch.isnan(loss[0]) and not torch.isnan(grad[0]).any()
+        zero = torch.zeros(N, device=DEV)
+        for tail in ("drop", "bucket"):
+            for reduction in ("mean", "sum"):
+                loss = pm.distill_loss(leaf, ids, lps, weights=zero, tail=tail, reduction=reduction)
+                assert float(loss.detach()) == 0.0
+                assert not torch.autograd.grad(loss, leaf)[0].any()
