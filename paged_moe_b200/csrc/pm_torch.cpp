@@ -460,21 +460,22 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
       bad_value("lengths must be [items, beams] or [items * beams]");
     lengths = lengths->contiguous();
   }
+  const bool graded = at::GradMode::is_enabled();
   std::vector<pm_state> s(states.size());
-  std::vector<const void*> read, written;
-  struct Extent {  // of a tensor that fills it
+  struct Extent {  // of a tensor that fills it, or of its first byte
     const char *from, *to;
     bool written;
   };
   std::vector<Extent> extents;
-  auto add_extent = [&](const torch::Tensor& t, bool write) {
-    const char* from = reinterpret_cast<const char*>(t.data_ptr());
-    if (t.is_non_overlapping_and_dense()) extents.push_back({from, from + t.nbytes(), write});
+  extents.reserve(2 * states.size());
+  auto add_extent = [&](const torch::Tensor& t, const void* at, bool write) {
+    const char* from = reinterpret_cast<const char*>(at);
+    extents.push_back({from, from + (t.is_non_overlapping_and_dense() ? t.numel() * t.element_size() : 1), write});
   };
   for (size_t i = 0; i < states.size(); ++i) {
     const torch::Tensor& a = states[i];
     const std::string name = "state " + std::to_string(i);
-    if (at::GradMode::is_enabled() && (out.has_value() ? (*out)[i] : a).requires_grad())
+    if (graded && (out.has_value() ? (*out)[i] : a).requires_grad())
       bad_value(name + " requires a gradient, which the reorder does not carry; call it under torch.no_grad()");
     if (a.dim() < 1 || a.size(0) != B * W) bad_value(name + " must have items * beams rows");
     int64_t dim = dims[i];
@@ -505,23 +506,16 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
       }
     }
     if (a.numel() == 0) { s[i].run_bytes = 0; continue; }
-    read.push_back(s[i].src);
-    written.push_back(s[i].dst);
-    add_extent(a, !out.has_value());
-    if (out.has_value()) add_extent(b, true);
+    add_extent(a, s[i].src, !out.has_value());
+    if (out.has_value()) add_extent(b, s[i].dst, true);
   }
   // the same memory twice would be moved twice, or read after it was written
-  std::vector<const void*> seen = written;
-  std::sort(seen.begin(), seen.end());
-  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) bad_value("two states share their memory");
-  if (out.has_value())
-    for (const void* p : read)
-      if (std::binary_search(seen.begin(), seen.end(), p)) bad_value("out shares its memory with a state");
   std::sort(extents.begin(), extents.end(), [](const Extent& a, const Extent& b) { return a.from < b.from; });
   const char *end = nullptr, *written_end = nullptr;  // of those that begin before
   for (const Extent& e : extents) {
     if (e.from < (e.written ? end : written_end))
-      bad_value(out.has_value() ? "out overlaps a state or another out" : "two states overlap");
+      bad_value(out.has_value() ? "out shares its memory with a state or another out, or overlaps it"
+                                : "two states share their memory or overlap");
     end = std::max(end, e.to);
     if (e.written) written_end = std::max(written_end, e.to);
   }
