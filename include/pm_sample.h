@@ -358,6 +358,7 @@ typedef struct pm_beam_out {
     uint8_t *done;               /* [items, n] (token == eos, or the parent was done), or NULL */
 } pm_beam_out;
 
+/* The workspace is 16-byte aligned. */
 PM_API size_t pm_beam_select_workspace_bytes(const pm_beam *b);
 PM_API int pm_beam_select(const pm_beam *b, const pm_beam_out *out, void *workspace, size_t workspace_bytes,
                           void *stream);
@@ -435,6 +436,7 @@ typedef struct pm_distill {
  * must not overlap the logits.  grad_loss: the gradient of whatever follows
  * with respect to the loss, [rows] under PM_REDUCE_NONE, else one value; NULL
  * means 1. */
+/* The workspace is 16-byte aligned. */
 PM_API size_t pm_distill_workspace_bytes(const pm_distill *d);
 PM_API int pm_distill_loss(const pm_distill *d, float *loss, void *grad, int64_t grad_stride,
                            const float *grad_loss, void *workspace, size_t workspace_bytes, void *stream);

@@ -877,7 +877,8 @@ int check_logits(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
                  const uint32_t* mask, int64_t mask_stride) {
   if (rows < 0 || vocab <= 0 || row_stride < vocab) return PM_ERR_ARG;
   if (dtype != PM_DTYPE_F32 && dtype != PM_DTYPE_BF16) return PM_ERR_ARG;
-  if (rows > 0 && !logits) return PM_ERR_ARG;
+  if (rows > 0 && (!logits || reinterpret_cast<uintptr_t>(logits) % (dtype == PM_DTYPE_F32 ? 4 : 2))) return PM_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(mask) % 4) return PM_ERR_ARG;
   if (mask && mask_stride != 0 && mask_stride < (vocab + 31) / 32) return PM_ERR_ARG;
   if (vocab > kMaxVocab || rows > kMaxRows) return PM_ERR_UNSUPPORTED;
   return PM_OK;
@@ -995,7 +996,8 @@ extern "C" int pm_beam_select(const pm_beam* b, const pm_beam_out* out, void* wo
   if (rc) return rc;
   if (!out) return PM_ERR_ARG;
   if (b->items == 0) return PM_OK;
-  if (!out->scores || !out->parents || !out->tokens || !workspace) return PM_ERR_ARG;
+  if (!out->scores || !out->parents || !out->tokens || !workspace || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return PM_ERR_ARG;
   if (workspace_bytes < pm_beam_select_workspace_bytes(b)) return PM_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const size_t rows = (size_t)b->items * b->beams;

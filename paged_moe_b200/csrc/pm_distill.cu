@@ -1137,7 +1137,9 @@ extern "C" int pm_distill_loss(const pm_distill* d, float* loss, void* grad, int
   }
   if (!loss && !grad) return PM_ERR_ARG;
   if (grad && (grad == d->logits || grad_stride < d->vocab)) return PM_ERR_ARG;
-  if (!workspace) return PM_ERR_ARG;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16) return PM_ERR_ARG;
+  const uintptr_t element = d->dtype == PM_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(d->logits) % element || reinterpret_cast<uintptr_t>(grad) % element) return PM_ERR_ARG;
   if (workspace_bytes < pm_distill_workspace_bytes(d)) return PM_ERR_WORKSPACE;
   const size_t rows = (size_t)d->rows, entries = rows * d->k;
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
@@ -1181,7 +1183,7 @@ extern "C" int pm_distill_scale(void* grad, int32_t dtype, int64_t rows, int64_t
   if (rows < 0 || vocab <= 0 || grad_stride < vocab || (dtype != PM_DTYPE_F32 && dtype != PM_DTYPE_BF16))
     return PM_ERR_ARG;
   if (rows == 0) return PM_OK;
-  if (!grad || !factor) return PM_ERR_ARG;
+  if (!grad || !factor || reinterpret_cast<uintptr_t>(grad) % (dtype == PM_DTYPE_F32 ? 4 : 2)) return PM_ERR_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (vocab > pm::kDistVocab) return PM_ERR_UNSUPPORTED;
   // a row covers up to two granules more than it fills

@@ -223,3 +223,13 @@ def test_beam_reorder_refuses_a_state_with_a_gradient():
         pm.beam_reorder([torch.zeros(3, 4)], parents, out=[leaf])
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
         pm.beam_reorder([leaf], parents)
+
+
+def test_c_checks_of_alignment():
+    lib = L.load()
+    for bad in (dict(logits=0x1002), dict(logits=0x1001, dtype=1), dict(mask=0x2002, mask_stride=32)):
+        assert lib.pm_top_logprobs(C.byref(_top(**bad)), 0x3000, 0x4000, None, None) == L.PM_ERR_ARG
+        assert lib.pm_beam_select_workspace_bytes(C.byref(_beam(**bad))) == 0
+    o = L.BeamOut()
+    o.scores, o.parents, o.tokens = 0x6000, 0x7000, 0x8000
+    assert lib.pm_beam_select(C.byref(_beam()), C.byref(o), 0x9008, 1 << 30, None) == L.PM_ERR_ARG

@@ -91,3 +91,15 @@ def test_plain_gradient_against_differences(tail, temp):
         diff = (P.rows(up, ids, lps, temp, tail)[0] - P.rows(dn, ids, lps, temp, tail)[0]) / (2 * h)
         # central differences: h^2 times a third derivative of at most a few, and 1e-16 / h of rounding
         np.testing.assert_allclose(g[:, v], diff, atol=1e-8)
+
+
+def test_distill_c_checks_of_alignment():
+    lib = L.load()
+    d = _d()
+    need = lib.pm_distill_workspace_bytes(C.byref(d))
+    assert lib.pm_distill_loss(C.byref(d), 0x1000, None, 0, None, 0x9008, need, None) == L.PM_ERR_ARG
+    assert lib.pm_distill_loss(C.byref(d), 0x1000, 0x2002, d.vocab, None, 0x9000, need, None) == L.PM_ERR_ARG
+    d = _d(logits=0x5002)
+    assert lib.pm_distill_loss(C.byref(d), 0x1000, None, 0, None, 0x9000, need, None) == L.PM_ERR_ARG
+    assert lib.pm_distill_scale(0x1002, 0, 1, 8, 8, 0x3000, None) == L.PM_ERR_ARG
+    assert lib.pm_distill_scale(0x1000, 0, 1, 262145, 262145, 0x3000, None) == L.PM_ERR_UNSUPPORTED
