@@ -931,9 +931,14 @@ __global__ void __launch_bounds__(kShortThreads, 2) k_distill_short(DistillArgs 
       } else {
         const float by = (float)f.factor;
         const uint64_t r2 = pk(-(float)part.rho, -(float)part.rho), f2 = pk(by, by);
-        for (int t = 0; t < chunks; ++t) {
+        // what was read last is read first: it is the likeliest to be near
+        uint4 next[kDistStep];
+        load(chunks - 1, next);
+        for (int t = chunks - 1; t >= 0; --t) {
           uint4 raw[kDistStep];
-          load(t, raw);
+#pragma unroll
+          for (int u = 0; u < kDistStep; ++u) raw[u] = next[u];
+          if (t > 0) load(t - 1, next);
           dist_grads<T>(raw, c2, r2, f2);
           store(t, raw);
         }
@@ -1082,8 +1087,8 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int64_t slots = (int64_t)pmh::num_sms() * pm::kDistResident;
   // Many short rows go to a warp each.  A CTA's rows follow one another, a warp
-  // is slower on its row: 2,007 rows of 2,401 fp32 take 27 us against 49, 2,048
-  // of 16,384 bf16 47 against 66, 600 of those 32 against 29, 2,048 of 32,768
+  // is slower on its row: 2,007 rows of 2,401 fp32 take 27 us against 48, 2,048
+  // of 16,384 bf16 45 against 66, 600 of those 32 against 29, 2,048 of 32,768
   // 45 against 60 for the loss alone but 93 against 93 with the gradient.
   const int64_t bytes_of_row = a.vocab * (int64_t)sizeof(T), unit = 16 << 10;
   if (bytes_of_row * (a.grad ? 2 : 1) <= pm::kShortBytes &&
