@@ -15,13 +15,21 @@
 // are read once more, about 1.2 k to 2 k of them, and only elements that
 // reach it become keys, (ordered logit bits, ~id): larger logits first, then
 // lower ids, all keys different.  Up to 256 keys are ranked by counting, one
-// a thread; of more, histograms leave that many first.  A part with more keys than the buffer holds
-// (long ties, as in a constant row) takes the plain way: one vector of every
-// thread at a time against a running threshold.
+// a thread; of more, histograms leave that many first.  A part with more keys
+// than the buffer holds (long ties, as in a constant row) takes the plain way:
+// one vector of every thread at a time against a running threshold.
 // A part whose mask allows few tokens is not streamed: those elements are
 // gathered, and all of them become keys.
 // The cluster's CTAs put their lists and sums into one another's shared memory;
 // each finds its own keys' places in the row and writes those.
+//
+// Measured: 2,048 rows of 163,840 bf16, k = 64, 133 us, 5.0 TB/s with a tenth
+// of the data read twice for its candidates; what is issued bounds it (four
+// instructions an element, 72 % of the issue slots) and the ends of rows, where
+// a CTA searches while its SM's other three stream.  512 rows of fp32 at
+// k = 16, 67 us, 5.2 TB/s.  Single rows cost the latency of their phases: 8 us
+// for 4 rows of 32,768, of which a copy is 2, the bound 1, the candidates 1,
+// their ranks 1, the cluster's exchange 1, the ends 2.
 //
 // Every wait on a copy is bounded; a row whose copy does not arrive gives
 // NaN and ids -1.
@@ -739,7 +747,9 @@ struct PickArgs {
 // one a thread: a candidate's place is the number of better ones, and of
 // equal ones before it.  More are merged two beams' lists at a time, each
 // candidate searching the other list for its place, until one list is left:
-// 2 W n searches of log n steps in log W rounds.
+// 2 W n searches of log n steps in log W rounds.  64 items of 8 beams and 16
+// candidates take 4.4 us, 4 of 16 and 64 7.8 us (merging costs the first 4 us
+// more).
 constexpr int kPickThreads = 256;   // counting
 constexpr int kPickMerge = 1024;    // merging
 
@@ -891,15 +901,13 @@ size_t top_bytes(int64_t tiles, int split, int k) {
          (split > 1 ? (size_t)split * k * 8 : 0);
 }
 
-// CTAs of a row: enough to fill every SM with resident CTAs, no more than it
-// has tiles.
-int top_split(int64_t rows, int64_t tiles, int k) {
+// CTAs of a row: as many as give every SM two, no more than it has tiles.  One
+// CTA takes 29 us for each of 5 rows of 151,552 fp32, eight 14; more than two an
+// SM cost more in lists to join than they hide (64 rows of 151,936 bf16 at
+// k = 256: 42 us with 512 CTAs, 35 with 256; 74 of 163,840 fp32: 33 and 24).
+int top_split(int64_t rows, int64_t tiles) {
   int c = 1;
-  while (c < pm::kTopSplit && 2 * c <= tiles) {
-    const int64_t resident = 232448 / (int64_t)(top_bytes(tiles, 2 * c, k) + 1024);
-    if (rows * 2 * c > (int64_t)pmh::num_sms() * resident) break;
-    c *= 2;
-  }
+  while (c < pm::kTopSplit && 2 * c <= tiles && rows * c <= (int64_t)pmh::num_sms()) c *= 2;
   return c;
 }
 
@@ -915,7 +923,7 @@ cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
   });
   if (e != cudaSuccess) return e;
   const int64_t tiles = (a.vocab + pm::kTopTile - 1) / pm::kTopTile;
-  const int split = top_split(a.rows, tiles, a.k);
+  const int split = top_split(a.rows, tiles);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * split));
   cfg.blockDim = dim3(pm::kTopThreads);
