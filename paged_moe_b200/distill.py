@@ -40,8 +40,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
                      one more outcome.
     The usual factor temp ** 2 is left to the caller.
 
-    weights [...] fp32 multiply the rows; a row of weight 0 (padding) is not
-    read, and neither its loss nor its gradient depends on what it holds.
+    weights [...] fp32, constants too, multiply the rows; a row of weight 0
+    (padding) is not read, and neither its loss nor its gradient depends on
+    what it holds.
     reduction: "mean" (divided by the sum of the weights), "sum", or "none"
     (a loss per row, [...]).  A row whose entries hold no mass has loss 0
     under "drop".

@@ -340,3 +340,30 @@ def test_top_few_allowed(dtype, rows, V, k, allowed):
         np.testing.assert_array_equal(got["ids"][first:first + n].cpu().numpy(), ids)
         _close(got["logprobs"][first:first + n], lp)
         _close(got["lse"][first:first + n], lse)
+
+
+@pytest.mark.parametrize("B,Wb,n,slots", [(2, 21, 21, True), (2, 21, 30, False), (3, 64, 64, True), (1, 5, 256, False)])
+@pytest.mark.parametrize("alpha", [0.0, 0.8])
+def test_select_more_than_256_candidates(B, Wb, n, slots, alpha):
+    """Lists merged in pairs: beams with the same logits and scores, ended and
+    missing beams, rows with fewer allowed tokens than candidates."""
+    rng = np.random.default_rng(60)
+    V = 700
+    x = _logits(61, B * Wb, V, torch.float32).view(B, Wb, V)
+    x[:, 2] = x[:, 1]
+    x[0, Wb - 1] = x[0, 0]
+    x[B - 1, 3] = float("-inf")
+    x[B - 1, 3, 9] = 1.0
+    s = _scores(62, B, Wb)
+    s[:, 2] = s[:, 1]
+    s[0, Wb - 1] = s[0, 0]
+    s[B - 1, 4] = -np.inf
+    done = rng.random((B, Wb)) < 0.2
+    done[:, :3] = False
+    lengths = rng.integers(1, 40, (B, Wb)).astype(np.int32)
+    lengths[:, 2] = lengths[:, 1]
+    lengths[0, Wb - 1] = lengths[0, 0]
+    _check_select(x, s, n, done=done, eos=5, lengths=lengths, alpha=alpha, slots=slots)
+    _check_select(x, np.full_like(s, -np.inf), n, done=done, eos=5, lengths=lengths, alpha=alpha, slots=slots)
+    words = _mask(63, B * Wb, V, 0.01)
+    _check_select(x, s, n, words=words, lengths=lengths, alpha=alpha, slots=slots)

@@ -392,3 +392,53 @@ def test_no_distribution_and_no_weight_on_both_sides():
                 loss = pm.distill_loss(leaf, ids, lps, weights=zero, tail=tail, reduction=reduction)
                 assert float(loss.detach()) == 0.0
                 assert not torch.autograd.grad(loss, leaf)[0].any()
+
+
+def test_two_captured_graphs_of_many_short_rows_and_their_inputs_change():
+    """Two graphs of the same leaf replayed in turn, with other logits each
+    time: neither keeps anything of the other's or of its last run."""
+    x, ids, lps = _case(70, 500, 900, 12)
+    y = _case(71, 500, 900, 12)[0]
+    w = torch.rand(500, device=DEV)
+    w[::7] = 0.0
+    leaf = x.detach().clone().requires_grad_()
+    kinds = (dict(tail="bucket", weights=w), dict(tail="drop", reduction="sum", temp=0.5))
+    graphs = []
+    for kw in kinds:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            loss = pm.distill_loss(leaf, ids, lps, **kw)
+            (grad,) = torch.autograd.grad(loss, leaf)
+        graphs.append((g, loss, grad, kw))
+    for source in (x, y, x):
+        with torch.no_grad():
+            leaf.copy_(source)
+        for g, _, _, _ in graphs:
+            g.replay()
+        for _, loss, grad, kw in graphs:
+            eager = source.detach().clone().requires_grad_()
+            want = pm.distill_loss(eager, ids, lps, **kw)
+            assert torch.equal(loss.detach(), want.detach())
+            assert torch.equal(grad, torch.autograd.grad(want, eager)[0])
+
+
+def test_same_bits_of_many_short_rows_and_on_two_streams_at_once():
+    x, ids, lps = _case(72, 900, 3001, 20, torch.bfloat16)
+    w = torch.rand(900, device=DEV)
+
+    def run():
+        leaf = x.detach().requires_grad_()
+        loss = pm.distill_loss(leaf, ids, lps, weights=w, tail="bucket")
+        return loss.detach(), torch.autograd.grad(loss, leaf)[0]
+
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for l, g in got:
+        assert torch.equal(l, want[0]) and torch.equal(g, want[1])
