@@ -19,7 +19,8 @@
 // than the buffer holds (long ties, as in a constant row) takes the plain way:
 // one vector of every thread at a time against a running threshold.
 // A part whose mask allows few tokens is not streamed: those elements are
-// gathered, and all of them become keys.
+// gathered, and all of them become keys.  So do all of a part of which so much
+// is wanted that the threads' maxima bound nothing.
 // The cluster's CTAs put their lists and sums into one another's shared memory;
 // each finds its own keys' places in the row and writes those.
 //
@@ -62,6 +63,7 @@ struct TopArgs {
   int64_t mask_stride;
   int k;
   double inv_t;
+  int direct;        // keys that a part has room for without a bound, 0: parts are streamed
   // beam search: rows that offer no logits (finished, or dead)
   const float* scores;
   const uint8_t* done;
@@ -310,6 +312,46 @@ struct TopFound {
   bool all;     // the part's tokens were few enough
 };
 
+// A single element joins the thread's share and becomes a key.
+__device__ __forceinline__ void top_take(TopShared& sh, TopFound& found, float x, int id, float c) {
+  found.m = fmaxf(found.m, x);
+  const float top = x * c;
+  if (fabsf(top) < kWildExponent) {
+    const float magic = top + 12582912.0f;  // 1.5 2^23 + R
+    found.acc.add(ex2_approx(fmaf(x, c, 12582912.0f - magic)), (int)(__float_as_uint(magic) - 0x4B400000u));
+  } else if (x < 0.0f) {
+    found.acc.low = found.acc.low || x > kNegInf;
+  } else {
+    found.acc.high = true;
+    if (x != x) found.acc.s = nan64();
+  }
+  if (x > kNegInf) sh.buf()[atomicAdd(&sh.count, 1)] = rankkey(x, (uint32_t)id);
+}
+
+// A short part of which much is wanted: maxima of 32 elements bound nothing
+// there, so that every element [i0, i1) becomes a key.
+template <typename T, bool MASKED>
+__device__ __noinline__ TopFound top_direct(TopShared& sh, const T* row, const uint32_t* words, int i0, int i1, float c) {
+  TopFound found;
+  found.acc.clear();
+  found.m = kNegInf;
+  found.all = true;
+  constexpr int U = 4;
+  __syncthreads();  // the count is zero
+  for (int i = i0 + (int)threadIdx.x; i < i1; i += U * kTopThreads) {
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int id = i + u * kTopThreads;
+      const bool on = id < i1 && (!MASKED || ((__ldg(words + (id >> 5)) >> (id & 31)) & 1u));
+      x[u] = on ? RowVec<T>::get(row + id) : kNegInf;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) top_take(sh, found, x[u], i + u * kTopThreads, c);
+  }
+  return found;
+}
+
 // Where [t0, t1) allows at most `cap` tokens, which shared memory holds next to
 // their ids, every allowed element becomes a key: only the mask and the sectors
 // of those elements are read, and no bound is needed.  Ids are placed by a scan
@@ -356,20 +398,7 @@ __device__ __noinline__ TopFound top_gather(TopShared& sh, const T* row, const u
       x[u] = id[u] >= 0 ? RowVec<T>::get(row + id[u]) : kNegInf;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      found.m = fmaxf(found.m, x[u]);
-      const float top = x[u] * c;
-      if (fabsf(top) < kWildExponent) {
-        const float magic = top + 12582912.0f;  // 1.5 2^23 + R
-        found.acc.add(ex2_approx(fmaf(x[u], c, 12582912.0f - magic)), (int)(__float_as_uint(magic) - 0x4B400000u));
-      } else if (x[u] < 0.0f) {
-        found.acc.low = found.acc.low || x[u] > kNegInf;
-      } else {
-        found.acc.high = true;
-        if (x[u] != x[u]) found.acc.s = nan64();
-      }
-      if (x[u] > kNegInf) sh.buf()[atomicAdd(&sh.count, 1)] = rankkey(x[u], (uint32_t)id[u]);
-    }
+    for (int u = 0; u < U; ++u) top_take(sh, found, x[u], id[u], c);
   }
   return found;
 }
@@ -447,8 +476,13 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   StepSum acc;
   acc.clear();
   float m0 = kNegInf, m1 = kNegInf;  // of every second tile each
-  bool gathered = false;
-  if (MASKED) {
+  bool gathered = a.direct > 0;
+  if (gathered) {
+    const TopFound found = top_direct<T, MASKED>(sh, row, reinterpret_cast<const uint32_t*>(mask), t0 * kTopTile,
+                                                 min(t1 * kTopTile, V), scale.c);
+    acc = found.acc;
+    m0 = found.m;
+  } else if (MASKED) {
     // 12 bytes a key in the place of the rings and of the tiles' maxima; a part
     // of which more is allowed is streamed as fast (1,030 rows of 35,439 fp32,
     // gathered against streamed: 29 to 45 us at 2 %, 43 to 50 at 7 %; 600 of
@@ -649,7 +683,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
     if (a.vals) a.vals[r * K + i] = x;
     if (a.logprobs) a.logprobs[r * K + i] = bad ? (float)lse : have ? (float)((double)x * a.inv_t - lse) : kNegInf;
   };
-  uint64_t* keys = reinterpret_cast<uint64_t*>(tops + per * kTopThreads);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(sh.rings() + (a.direct ? a.direct * 8 : kTopRingBytes + per * kTopThreads * 2));
   int total = sh.got;  // keys of the row
   if (split > 1) {
     // every CTA gets all the lists and places its own
@@ -894,13 +928,13 @@ int check_logits(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
   return PM_OK;
 }
 
-// Shared memory of a CTA: the rings, a part's maxima, and the parts' lists of
-// a row that is split.
-size_t top_bytes(int64_t tiles, int split, int k) {
-  return sizeof(pm::TopShared) + pm::kTopRingBytes + (size_t)((tiles + split - 1) / split) * pm::kTopThreads * 2 +
+// Shared memory of a CTA: the rings and a part's maxima, or room for all of its
+// keys; and the parts' lists of a row that is split.
+size_t top_bytes(int64_t tiles, int split, int k, int direct) {
+  return sizeof(pm::TopShared) +
+         (direct ? (size_t)direct * 8 : pm::kTopRingBytes + (size_t)((tiles + split - 1) / split) * pm::kTopThreads * 2) +
          (split > 1 ? (size_t)split * k * 8 : 0);
 }
-
 // CTAs of a row: as many as give every SM two, no more than it has tiles.  One
 // CTA takes 29 us for each of 5 rows of 151,552 fp32, eight 14; more than two an
 // SM cost more in lists to join than they hide (64 rows of 151,936 bf16 at
@@ -917,9 +951,8 @@ cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
   static pmh::DeviceOnce once;
   cudaError_t e = cudaSuccess;
   once([&] {
-    constexpr int64_t most = kMaxVocab / pm::kTopTile;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(top_bytes(most, 1, pm::kTopMax) + (size_t)pm::kTopSplit * pm::kTopMax * 8));
+                             (int)top_bytes(1, pm::kTopSplit, pm::kTopMax, pm::kTopTile));
   });
   if (e != cudaSuccess) return e;
   const int64_t tiles = (a.vocab + pm::kTopTile - 1) / pm::kTopTile;
@@ -927,7 +960,15 @@ cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * split));
   cfg.blockDim = dim3(pm::kTopThreads);
-  cfg.dynamicSmemBytes = top_bytes(tiles, split, a.k);
+  pm::TopArgs b = a;
+  // A part of one tile has a maximum a thread, 32 for 1,024 elements: fewer than
+  // k bound nothing (1,608 rows of 4,597 fp32 at k = 189: 64 us against 106; where
+  // they do, the bound is worth its time: 1,000 rows of 4,096 bf16 at k = 128
+  // 29 us against 37).
+  constexpr int64_t chunk = pm::kTopTile / pm::kTopWarps;  // a warp's elements of a tile
+  const int64_t part = a.vocab < pm::kTopTile ? (a.vocab + 15) / 16 * 16 : pm::kTopTile;
+  b.direct = tiles <= split && a.k > (part + chunk - 1) / chunk * 32 ? (int)part : 0;
+  cfg.dynamicSmemBytes = top_bytes(tiles, split, a.k, b.direct);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -935,7 +976,7 @@ cudaError_t launch_top_v(const pm::TopArgs& a, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  return cudaLaunchKernelEx(&cfg, kernel, b);
 }
 
 template <typename T>
