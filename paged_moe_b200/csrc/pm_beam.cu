@@ -72,7 +72,7 @@ struct TopArgs {
   float* logprobs;   // [rows, k] or NULL
   float* vals;       // [rows, k] the logits themselves, or NULL
   float* lse;        // [rows] or NULL
-  double* lse64;     // [rows] or NULL; NaN: the row offers nothing
+  double* above;     // [rows] or NULL: lse - largest / T; NaN: the row offers nothing
 };
 
 // A step is four vectors of every lane, 2 KB of a warp's chunk and one stage
@@ -93,7 +93,8 @@ struct alignas(16) TopShared {
   unsigned hist[256];
   int scal[kTopWarps];
   int bin[3];
-  double lse;             // of the row
+  double above;           // the row's lse - its largest / T
+  float largest;
   int bad;                // the row has no distribution
   int count;              // keys in buf
   int got;                // keys in best
@@ -457,7 +458,7 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   uint16_t* tops = reinterpret_cast<uint16_t*>(sh.rings() + kTopRingBytes);
   // the whole cluster leaves here or none of it
   if (a.scores && (!(a.scores[r] > kNegInf) || (a.done && a.done[r]))) {
-    if (tid == 0 && rank == 0) a.lse64[r] = nan64();
+    if (tid == 0 && rank == 0) a.above[r] = nan64();
     return;
   }
   if (split > 1) cluster_arrive();  // waited for before the first store into another CTA
@@ -677,11 +678,15 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
   top_cut(sh, sh.count, K);
 
   // the row's key of rank i
-  auto put = [&](int i, uint64_t key, bool have, double lse, bool bad) {
+  auto put = [&](int i, uint64_t key, bool have, bool bad) {
     const float x = have ? key_value(key) : kNegInf;
     a.ids[r * K + i] = have ? (int32_t)key_index(key) : -1;
     if (a.vals) a.vals[r * K + i] = x;
-    if (a.logprobs) a.logprobs[r * K + i] = bad ? (float)lse : have ? (float)((double)x * a.inv_t - lse) : kNegInf;
+    // no difference of numbers as large as the logits: log S is left in it
+    if (a.logprobs)
+      a.logprobs[r * K + i] =
+          bad ? __int_as_float(0x7fffffff)
+              : have ? (float)(((double)x - (double)sh.largest) * a.inv_t - sh.above) : kNegInf;
   };
   uint64_t* keys = reinterpret_cast<uint64_t*>(sh.rings() + (a.direct ? a.direct * 8 : kTopRingBytes + per * kTopThreads * 2));
   int total = sh.got;  // keys of the row
@@ -720,13 +725,14 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
       M = warp_max_ordered(on ? sh.tops[lane] : kNegInf);
     }
     const bool bad = !(sum.s == sum.s) || M == -kNegInf;
-    const double lse = bad ? nan64() : M > kNegInf ? scale.log_of(sum, M) : kNegInf64;
+    const double above = !bad && M > kNegInf ? scale.log_above(sum, M) : nan64();
     if (lane == 0) {
-      sh.lse = lse;
+      sh.above = above;
+      sh.largest = M;
       sh.bad = bad;
       if (rank == 0) {
-        if (a.lse) a.lse[r] = (float)lse;
-        if (a.lse64) a.lse64[r] = M > kNegInf ? lse : nan64();
+        if (a.lse) a.lse[r] = bad || M > kNegInf ? (float)((double)M * a.inv_t + above) : kNegInf;
+        if (a.above) a.above[r] = above;
       }
     }
   }
@@ -752,12 +758,11 @@ __global__ void __launch_bounds__(kTopThreads, 4) k_top_rows(TopArgs a) {
     for (int d = 0; d < kTopSplit; ++d) place += found[d];
   }
   __syncthreads();
-  const double lse = sh.lse;
   const bool bad = sh.bad;
-  if (!bad && place < K) put(place, key, true, lse, false);
+  if (!bad && place < K) put(place, key, true, false);
   // what the row lacks, by its first CTA
   if (rank == 0)
-    for (int i = (bad ? 0 : total) + tid; i < K; i += kTopThreads) put(i, 0ull, false, lse, bad);
+    for (int i = (bad ? 0 : total) + tid; i < K; i += kTopThreads) put(i, 0ull, false, bad);
 }
 
 // ---------------------------------------------------------------------------
@@ -773,7 +778,7 @@ struct PickArgs {
   const int32_t* lengths;
   const int32_t* ids;   // [items * beams, n] each beam's continuations, best first
   const float* vals;    // [items * beams, n] their logits
-  const double* lse64;  // [items * beams]
+  const double* above;  // [items * beams] log-sum-exp less the largest logit
   pm_beam_out out;
 };
 
@@ -807,11 +812,11 @@ __global__ void __launch_bounds__(kPickMerge) k_beam_pick(PickArgs a) {
       *token = a.eos;
       return j == 0 ? score : none;
     }
-    const double lse = a.lse64[r];
+    const double above = a.above[r];
     const int id = a.ids[r * n + j];
-    if (!(lse == lse) || id < 0) return none;
+    if (!(above == above) || id < 0) return none;
     *token = id;
-    return score + ((double)a.vals[r * n + j] - lse);
+    return score + (((double)a.vals[r * n + j] - (double)a.vals[r * n]) - above);  // the first is the largest
   };
   auto divisor = [&](int w) {
     if (!a.lengths || a.alpha == 0.0) return 1.0;
@@ -1062,7 +1067,7 @@ extern "C" int pm_beam_select(const pm_beam* b, const pm_beam_out* out, void* wo
   a.inv_t = 1.0;
   a.scores = b->scores;
   a.done = b->done;
-  a.lse64 = reinterpret_cast<double*>(ws);
+  a.above = reinterpret_cast<double*>(ws);
   a.ids = reinterpret_cast<int32_t*>(ws + round16(8 * rows));
   a.vals = reinterpret_cast<float*>(ws + round16(8 * rows) + round16(4 * rows * b->n));
   const int rc2 = launch_top(b->dtype, a, st);
@@ -1078,7 +1083,7 @@ extern "C" int pm_beam_select(const pm_beam* b, const pm_beam_out* out, void* wo
   p.lengths = b->lengths;
   p.ids = a.ids;
   p.vals = a.vals;
-  p.lse64 = a.lse64;
+  p.above = a.above;
   p.out = *out;
   const int all = b->beams * b->n;
   const bool merge = all > pm::kPickThreads;

@@ -226,10 +226,11 @@ struct ExpScale {
   float c;        // fl32(log2(e) / T)
   double exact;   // log2(e) / T
   __device__ __forceinline__ explicit ExpScale(double inv_t) : exact(kLog2e64 * inv_t) { c = (float)exact; }
-  // natural log of s 2^rho for a row of maximum m
-  __device__ __forceinline__ double log_of(const ExpSum& a, float m) const {
-    const double lost = fabsf(m * c) < kWildExponent ? (double)m * (exact - (double)c) : 0.0;
-    return (a.rho + lost) * kLn264 + log(a.s);
+  // natural log of the sum of e^((x - m) / T), s 2^rho being the row's sum and m
+  // its maximum: nothing as large as m itself is left in it (the product is
+  // rounded as it is in a.rho, or their difference would be its last bit)
+  __device__ __forceinline__ double log_above(const ExpSum& a, float m) const {
+    return (a.rho - __dmul_rn((double)m, fabsf(m * c) < kWildExponent ? (double)c : exact)) * kLn264 + log(a.s);
   }
 };
 
@@ -274,7 +275,7 @@ __device__ __forceinline__ void add_wild(ExpSum& acc, uint4 raw, const ExpScale&
   RowVec<T>::unpack(raw, v);
 #pragma unroll
   for (int e = 0; e < RowVec<T>::n; ++e) sum += ex2_approx((v[e] - tm) * k.c);
-  acc.add((double)sum, tm == tm ? (double)tm * k.exact : kNegInf64);
+  acc.add((double)sum, tm == tm ? __dmul_rn((double)tm, k.exact) : kNegInf64);
 }
 
 }  // namespace pm

@@ -26,6 +26,15 @@ def row_lse(z):
     return m if np.isneginf(m) else m + np.log(np.exp(z - m).sum())
 
 
+def log_softmax(z):
+    """z - row_lse(z) without a difference of numbers as large as z: at
+    z = 3e38 the logarithm of the sum would be lost in row_lse."""
+    m = z.max()
+    with np.errstate(invalid="ignore"):
+        d = z - m
+    return d - np.log(np.exp(d).sum())
+
+
 def row_best(z, n):
     """Ids of the n best finite values: larger first, then the lower id."""
     order = np.lexsort((np.arange(z.size), -z))
@@ -46,7 +55,7 @@ def top_logprobs(x, k, temp=1.0, allowed=None):
             continue
         best = row_best(z, k)
         ids[r, :len(best)] = best
-        lp[r, :len(best)] = z[best] / temp - lse[r]
+        lp[r, :len(best)] = log_softmax(z / temp)[best]
     return ids, lp, lse
 
 
@@ -72,8 +81,9 @@ def beam_select(x, scores, n, allowed=None, done=None, eos=-1, lengths=None, alp
             lse = row_lse(z)
             if not np.isfinite(lse):
                 continue
+            logq = log_softmax(z)
             for j, v in enumerate(row_best(z, n)):
-                t = s + (z[v] - lse)
+                t = s + logq[v]
                 cand.append((-t / max(base + 1, 1) ** alpha, w, j, t, v, base + 1, v == eos))
         cand.sort(key=lambda c: c[:3])
         cand = cand[:n]

@@ -61,7 +61,8 @@ def _check_top(x, k, temp=1.0, words=None, per_row=True):
     ids, lp, lse = P.top_logprobs(x.double().cpu().numpy(), k, temp, allowed)
     np.testing.assert_array_equal(got["ids"].cpu().numpy(), ids)
     _close(got["logprobs"], lp)
-    _close(got["lse"], lse)
+    # what fp32 cannot hold is infinite: from half a step behind its largest on
+    _close(got["lse"], np.where(np.abs(lse) >= 2.0 ** 128 * (1 - 2.0 ** -25), np.sign(lse) * np.inf, lse))
     return got
 
 
@@ -367,3 +368,43 @@ def test_select_more_than_256_candidates(B, Wb, n, slots, alpha):
     _check_select(x, np.full_like(s, -np.inf), n, done=done, eos=5, lengths=lengths, alpha=alpha, slots=slots)
     words = _mask(63, B * Wb, V, 0.01)
     _check_select(x, s, n, words=words, lengths=lengths, alpha=alpha, slots=slots)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V,k,share", [
+    (3, 1024, 32, None), (3, 1024, 33, None), (3, 1025, 64, None), (3, 1025, 65, None), (700, 4597, 161, None),
+    (2, 7169, 256, None), (2, 7168, 225, None), (2, 7168, 224, 0.5), (2, 7168, 225, 0.5), (3, 1, 1, None), (5, 40, 256, 0.3)])
+def test_top_more_wanted_than_threads_hold(dtype, rows, V, k, share):
+    """Both sides of where every element of a short row becomes a key, with
+    ties, infinities and offsets."""
+    x = _logits(70, min(rows, 9), V, dtype, pad=3, offset=1)
+    if V > 100:
+        x[0, 10:90] = x[0, 5]
+        x[1, ::2] = float("-inf")
+        x[2 % x.shape[0], :] = torch.finfo(dtype).min
+    if rows > x.shape[0]:
+        big = torch.zeros(rows, V + 1, dtype=dtype, device=DEV)[:, :V]
+        big.copy_(x.repeat((rows + 8) // 9, 1)[:rows])
+        got = pm.top_logprobs(big, k)
+        ids, lp, _ = P.top_logprobs(x.double().cpu().numpy(), k)
+        for first in (0, (rows - 9) // 9 * 9):
+            np.testing.assert_array_equal(got["ids"][first:first + 9].cpu().numpy(), ids)
+            _close(got["logprobs"][first:first + 9], lp)
+        return
+    _check_top(x, k, temp=0.9, words=None if share is None else _mask(71, x.shape[0], V, share))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [900, 30000])
+def test_rows_at_the_lowest_value_are_uniform(dtype, V):
+    """All tokens at the type's lowest value, or far from zero: log V is not
+    lost next to the logits."""
+    x = torch.full((3, V), torch.finfo(dtype).min, dtype=dtype, device=DEV)
+    x[1] = 2.0 ** 60
+    x[2] = -70000.0
+    for temp in (1.0, 0.7):
+        lp = pm.top_logprobs(x, 4, temp=temp)["logprobs"].double().cpu().numpy()
+        assert (np.abs(lp + np.log(V)) <= LSE_TOL + np.log(V) * 2.0 ** -24).all(), lp
+    got = pm.beam_select(x.view(1, 3, V), torch.tensor([[-1.0, -2.0, -3.0]], device=DEV), n=4)
+    assert got["parents"].tolist() == [[0, 0, 0, 0]] and got["tokens"].tolist() == [[0, 1, 2, 3]]
+    assert (np.abs(got["scores"].double().cpu().numpy() + 1 + np.log(V)) <= LSE_TOL + 12 * 2.0 ** -24).all()
