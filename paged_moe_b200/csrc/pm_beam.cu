@@ -43,7 +43,6 @@
 #include "pm_device.cuh"
 #include "pm_host.h"
 #include "pm_rowvec.cuh"
-#include "pm_select.cuh"
 #include "pm_tma.cuh"
 
 namespace pm {

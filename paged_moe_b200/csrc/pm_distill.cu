@@ -521,7 +521,6 @@ __global__ void __launch_bounds__(kDistThreads, kDistResident) k_distill_rows(Di
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   DistillShared& sh = *reinterpret_cast<DistillShared*>(shared_bytes);
   constexpr int n = RowVec<T>::n;
-  constexpr uint32_t kBits = (1u << n) - 1u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = dist_rank(), split = dist_split();
   const int V = (int)a.vocab, K = a.k;
