@@ -467,7 +467,7 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
     bool written;
   };
   std::vector<Extent> extents;
-  extents.reserve(2 * states.size());
+  extents.reserve(2 * states.size() + 2);
   auto add_extent = [&](const torch::Tensor& t, const void* at, bool write) {
     const char* from = reinterpret_cast<const char*>(at);
     extents.push_back({from, from + (t.is_non_overlapping_and_dense() ? t.numel() * t.element_size() : 1), write});
@@ -509,13 +509,16 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
     add_extent(a, s[i].src, !out.has_value());
     if (out.has_value()) add_extent(b, s[i].dst, true);
   }
+  // parents and lengths are read while states are written
+  if (parents.numel()) add_extent(parents, parents.data_ptr(), false);
+  if (lengths.has_value() && lengths->numel()) add_extent(*lengths, lengths->data_ptr(), false);
   // the same memory twice would be moved twice, or read after it was written
   std::sort(extents.begin(), extents.end(), [](const Extent& a, const Extent& b) { return a.from < b.from; });
   const char *end = nullptr, *written_end = nullptr;  // of those that begin before
   for (const Extent& e : extents) {
     if (e.from < (e.written ? end : written_end))
       bad_value(out.has_value() ? "out shares its memory with a state or another out, or overlaps it"
-                                : "two states share their memory or overlap");
+                                : "two states (or a state and parents or lengths) share their memory or overlap");
     end = std::max(end, e.to);
     if (e.written) written_end = std::max(written_end, e.to);
   }

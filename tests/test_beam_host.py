@@ -233,3 +233,19 @@ def test_c_checks_of_alignment():
     o = L.BeamOut()
     o.scores, o.parents, o.tokens = 0x6000, 0x7000, 0x8000
     assert lib.pm_beam_select(C.byref(_beam()), C.byref(o), 0x9008, 1 << 30, None) == L.PM_ERR_ARG
+
+
+def test_beam_reorder_refuses_to_write_what_it_reads():
+    """lengths or parents among the states: other states' moves read them."""
+    parents = torch.zeros(2, 3, dtype=torch.int32)
+    lengths = torch.ones(6, dtype=torch.int32)
+    cache = torch.zeros(6, 5, 4)
+    with pytest.raises(ValueError, match="share"):
+        pm.beam_reorder([cache, lengths], parents, lengths=lengths, seq_dim=[1, None])
+    with pytest.raises(ValueError, match="share"):
+        pm.beam_reorder([parents.view(6, 1)], parents)
+    with pytest.raises(ValueError, match="share"):
+        pm.beam_reorder([torch.zeros(6, dtype=torch.int32)], parents, out=[lengths], lengths=lengths)
+    with pytest.raises(ValueError, match="CUDA"):  # all that is left to refuse
+        pm.beam_reorder([cache, lengths], parents, out=[torch.zeros_like(cache), torch.zeros_like(lengths)],
+                        lengths=lengths, seq_dim=[1, None])
