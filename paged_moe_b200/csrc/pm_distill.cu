@@ -28,10 +28,9 @@
 // issue slots (ten instructions an element forward, eight backward); clusters
 // of two, whose rows all stay in L2, take as long.  257 rows of 151,937 fp32:
 // 72 us, 4.7 TB/s.  8,000 rows of 16,384 bf16 in k_distill_short: 150 us, 4.4
-// TB/s.  Twelve warps and three stages, twice an SM, were the best of 8 to 16
-// warps, two to four stages and one to three CTAs (334 us against 363 for eight
-// warps at the time).  A cluster a row where there are few: 16 rows of 163,840
-// fp32 21 us, 43 with one CTA each.
+// TB/s.  Twelve warps with three stages, twice an SM, were faster than eight
+// warps, two or three times an SM, and than fourteen.  A cluster a row where
+// there are few: 16 rows of 163,840 fp32 21 us, 43 with one CTA each.
 //
 // Every wait on a copy is bounded; a row whose copy does not arrive gives NaN.
 #include <cuda_bf16.h>
