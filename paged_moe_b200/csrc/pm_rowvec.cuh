@@ -14,7 +14,10 @@
 // (masks of the type's lowest value) are left out: they add nothing to a row
 // that holds anything else.  A row, or part of one, that reaches far above,
 // or holds nothing but such values, is wild: it is summed once more, as
-// 2^((x - m) c) with rho = m log2(e) / T.
+// 2^((x - m) c) with rho = m c, which 64 bits hold exactly.  Every exponent has
+// the same c, so that parts of either kind join and any maximum may be taken
+// off their sum: log2(e) / T here and c there would differ by m 2^-25, 0.02
+// where |m c| is 2^20.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -221,16 +224,16 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// Constants of a row's exponentials.
+// The constant of a row's exponentials.
 struct ExpScale {
-  float c;        // fl32(log2(e) / T)
-  double exact;   // log2(e) / T
-  __device__ __forceinline__ explicit ExpScale(double inv_t) : exact(kLog2e64 * inv_t) { c = (float)exact; }
+  float c;  // fl32(log2(e) / T)
+  __device__ __forceinline__ explicit ExpScale(double inv_t) : c((float)(kLog2e64 * inv_t)) {}
+  // m c, exact in 64 bits
+  __device__ __forceinline__ double exponent(float m) const { return (double)m * (double)c; }
   // natural log of the sum of e^((x - m) / T), s 2^rho being the row's sum and m
-  // its maximum: nothing as large as m itself is left in it (the product is
-  // rounded as it is in a.rho, or their difference would be its last bit)
+  // its maximum: nothing as large as m itself is left in it
   __device__ __forceinline__ double log_above(const ExpSum& a, float m) const {
-    return (a.rho - __dmul_rn((double)m, fabsf(m * c) < kWildExponent ? (double)c : exact)) * kLn264 + log(a.s);
+    return (a.rho - exponent(m)) * kLn264 + log(a.s);
   }
 };
 
@@ -275,7 +278,7 @@ __device__ __forceinline__ void add_wild(ExpSum& acc, uint4 raw, const ExpScale&
   RowVec<T>::unpack(raw, v);
 #pragma unroll
   for (int e = 0; e < RowVec<T>::n; ++e) sum += ex2_approx((v[e] - tm) * k.c);
-  acc.add((double)sum, tm == tm ? __dmul_rn((double)tm, k.exact) : kNegInf64);
+  acc.add((double)sum, tm == tm ? k.exponent(tm) : kNegInf64);
 }
 
 }  // namespace pm
