@@ -397,19 +397,21 @@ PM_API int pm_beam_reorder(const pm_state *states, int32_t n_states, const int32
  * teacher entries (ids, logprobs), those of pm_top_logprobs at the same
  * temperature T; ids outside [0, vocab) are no entries.  With q = softmax(x / T):
  *   PM_TAIL_DROP    p = the entries' probabilities divided by their sum:
- *       loss = sum p_v (log p_v - log q_v)
+ *       loss = sum over the entries e of token v of p_e (log p_e - log q_v)
  *       dloss/dx_v = (q_v - p_v) / T
  *   PM_TAIL_BUCKET  p as given; the rest p_t = max(0, 1 - sum p) and q_t = the
  *       student's mass outside the entries are one more outcome:
- *       loss = sum p_v (log p_v - log q_v) + p_t (log p_t - log q_t)
+ *       loss = sum p_e (log p_e - log q_v) + p_t (log p_t - log q_t)
  *       dloss/dx_v = (q_v - p_v) / T on the entries, q_v (1 - p_t / q_t) / T elsewhere
  *       (q_t below 2^-100 counts as 2^-100; without a token outside the
  *       entries the bucket is left out)
- * An id listed twice has the sum of its entries' probabilities.  A row whose
- * entries hold no mass has loss 0 and gradient 0 under PM_TAIL_DROP.  weights
- * [rows] multiply the rows; a row of weight 0 is not read, its loss and
- * gradient are 0.  PM_REDUCE_MEAN divides by the sum of the weights (by
- * rows without weights; a sum of 0 gives 0).  1 <= k <= 256. */
+ * p_v is the sum of the token's entries.  Entries that list an id twice stay two
+ * outcomes of the teacher: the loss is the divergence of the summed
+ * probabilities plus sum p_e log(p_e / p_v), a constant that may take it below
+ * 0.  A row whose entries hold no mass has loss 0 and gradient 0 under
+ * PM_TAIL_DROP.  weights [rows] multiply the rows; a row of weight 0 is not
+ * read, its loss and gradient are 0.  PM_REDUCE_MEAN divides by the sum of the
+ * weights (by rows without weights; a sum of 0 gives 0).  1 <= k <= 256. */
 #define PM_TAIL_DROP 0
 #define PM_TAIL_BUCKET 1
 #define PM_REDUCE_NONE 0

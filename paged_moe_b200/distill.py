@@ -35,17 +35,23 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
       tail "drop":   p = the entries' probabilities divided by their sum (raw
                      logits divided by temp will do);
                      loss = sum p (log p - log q), gradient (q - p) / temp.
+                     A row whose entries hold no mass has loss 0.
       tail "bucket": p as given; the teacher's remaining mass 1 - sum p is
                      matched with the student's mass outside the entries, as
-                     one more outcome.
+                     one more outcome; that mass counts as 2**-100 at least,
+                     and without a token outside the entries there is no such
+                     outcome.
+    The sums run over the entries as they are listed.  An id listed twice takes
+    the sum of both in the gradient; in the loss they stay two outcomes of the
+    teacher: it is the divergence of the sums plus p log(p / sum) of each such
+    entry, a constant that may take it below 0.
     The usual factor temp ** 2 is left to the caller.
 
     weights [...] fp32, constants too, multiply the rows; a row of weight 0
     (padding) is not read, and neither its loss nor its gradient depends on
     what it holds.
     reduction: "mean" (divided by the sum of the weights), "sum", or "none"
-    (a loss per row, [...]).  A row whose entries hold no mass has loss 0
-    under "drop".
+    (a loss per row, [...]).
 
     With "mean" and "sum" the forward pass leaves the gradient behind (of the
     logits' type; the logits are not kept), so backward runs once per call.
