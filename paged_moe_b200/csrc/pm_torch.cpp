@@ -7,6 +7,7 @@
 // ABI on the current CUDA stream and raise on a bad status.  No arithmetic
 // happens here: every kernel is in libpm_sample.so.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -259,6 +260,11 @@ void on_device(const torch::Tensor& t, const torch::Device& dev, const char* nam
 
 void need_cuda(const torch::Tensor& t, const char* name) {
   if (!t.is_cuda()) bad_value(std::string(name) + " must be a CUDA tensor");
+}
+
+// Whether a forward-mode derivative (a dual tensor's tangent) rides on t.
+bool has_tangent(const torch::Tensor& t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
 }
 
 // The allowed-token words of `rows` rows: contiguous [rows, words], or [words]
@@ -694,6 +700,8 @@ struct DistillPerRow : torch::autograd::Function<DistillPerRow> {
 // The loss of logits [..., V]: one value, or one per row [N] without a reduction.
 torch::Tensor distill_loss(torch::Tensor logits, torch::Tensor ids, torch::Tensor logprobs, double temp, int64_t tail,
                            OptT weights, int64_t reduction) {
+  // its loss would come back without a tangent, as if it did not depend on the logits
+  if (has_tangent(logits)) bad_value("distill_loss has no forward-mode derivative; its gradient comes from backward");
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     if (reduction == PM_REDUCE_NONE)
       return DistillPerRow::apply(logits, ids, logprobs, temp, tail, weights, reduction);

@@ -56,7 +56,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logpro
     With "mean" and "sum" the forward pass leaves the gradient behind (of the
     logits' type; the logits are not kept), so backward runs once per call.
     Capture forward and backward into one CUDA graph with torch.autograd.grad
-    or leaves that no eager graph still holds.  K <= 256.
+    or leaves that no eager graph still holds.  There is no second derivative
+    and no forward-mode one.  K <= 256.
     """
     if tail not in _TAILS:
         raise ValueError(f"tail must be one of {sorted(_TAILS)}")
