@@ -481,8 +481,10 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
   for (size_t i = 0; i < states.size(); ++i) {
     const torch::Tensor& a = states[i];
     const std::string name = "state " + std::to_string(i);
-    if (graded && (out.has_value() ? (*out)[i] : a).requires_grad())
+    const torch::Tensor& b = out.has_value() ? (*out)[i] : a;
+    if (graded && (a.requires_grad() || b.requires_grad()))
       bad_value(name + " requires a gradient, which the reorder does not carry; call it under torch.no_grad()");
+    if (has_tangent(a) || has_tangent(b)) bad_value(name + " has a tangent, which the reorder does not carry");
     if (a.dim() < 1 || a.size(0) != B * W) bad_value(name + " must have items * beams rows");
     int64_t dim = dims[i];
     if (dim >= 0 && !lengths.has_value()) bad_value("seq_dim needs lengths");
@@ -492,7 +494,6 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
     const int64_t size = a.element_size();
     s[i].src = a.data_ptr();
     s[i].src_row_stride = a.stride(0) * size;
-    const torch::Tensor& b = out.has_value() ? (*out)[i] : a;
     s[i].dst = b.data_ptr();
     s[i].dst_row_stride = b.stride(0) * size;
     s[i].dst_outer_stride = s[i].src_outer_stride;
