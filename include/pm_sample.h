@@ -372,7 +372,7 @@ PM_API int pm_beam_select(const pm_beam *b, const pm_beam_out *out, void *worksp
  * runs of run_bytes bytes each.  With lengths [items, beams] and pos_bytes >
  * 0 only the first lengths[parent's row] positions of a run move, pos_bytes
  * bytes each; what lies behind them in the destination stays as it was.
- * States must not overlap one another. */
+ * States must not overlap one another, nor a state's rows and runs each other. */
 #define PM_MAX_STATES 128
 
 typedef struct pm_state {

@@ -79,8 +79,8 @@ def beam_reorder(states: Union[torch.Tensor, Sequence[torch.Tensor]], parents: t
 
     A state has to be dense from its position dimension on (without
     positions: any split into leading dimensions that collapse and a dense
-    rest), and states, out, parents and lengths must not overlap.  All states
-    move in one launch (up to 128).  No derivative is carried: where autograd is
+    rest), and its rows must not overlap, nor states, out, parents and lengths
+    one another.  All states move in one launch (up to 128).  No derivative is carried: where autograd is
     on, states and outs that require a gradient are refused, and dual tensors
     always.  Returns out, or the states.
     """

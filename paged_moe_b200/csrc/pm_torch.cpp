@@ -422,7 +422,7 @@ std::vector<torch::Tensor> beam_select(torch::Tensor logits, torch::Tensor score
 
 // One state of beam_reorder as (row, run) geometry.  dim: the dimension of
 // positions, or -1.  The dimensions from `dim` on have to be dense; those
-// between the rows and it have to collapse into one.
+// between the rows and it have to collapse into one.  No two rows share memory.
 void state_geometry(const torch::Tensor& t, int64_t dim, const std::string& name, int64_t* outer, int64_t* outer_stride,
                     int64_t* run, int64_t* pos) {
   const int64_t size = t.element_size(), D = t.dim();
@@ -449,6 +449,15 @@ void state_geometry(const torch::Tensor& t, int64_t dim, const std::string& name
     *outer *= t.size(d);
   }
   if (*outer == 0) { *outer = 1; *run = 0; }
+  // rows and runs behind one another, whichever of them lies closer together
+  if (t.numel() == 0) return;
+  int64_t near = t.size(0), near_stride = t.stride(0) * size, far = *outer, far_stride = *outer_stride;
+  if (near == 1 || (far > 1 && far_stride < near_stride)) {
+    std::swap(near, far);
+    std::swap(near_stride, far_stride);
+  }
+  if ((near > 1 && near_stride < *run) || (far > 1 && far_stride < near_stride * (near - 1) + *run))
+    bad_value(name + " has rows or elements that share memory (overlapping windows)");
 }
 
 // pm_beam_reorder over any number of states, PM_MAX_STATES a launch.
