@@ -509,6 +509,9 @@ void beam_reorder(std::vector<torch::Tensor> states, torch::Tensor parents,
     if (out.has_value()) {
       if (b.sizes() != a.sizes() || b.scalar_type() != a.scalar_type())
         bad_value("out of " + name + " must have its shape and type");
+      // bytes are moved: a conjugation or a sign that is still to be taken is not
+      if (b.is_conj() != a.is_conj() || b.is_neg() != a.is_neg())
+        bad_value("out of " + name + " must be conjugated or negated lazily where it is");
       int64_t outer, run, pos;
       state_geometry(b, dim, "out of " + name, &outer, &s[i].dst_outer_stride, &run, &pos);
       if (run != s[i].run_bytes || outer != s[i].outer) {
