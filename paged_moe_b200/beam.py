@@ -43,6 +43,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
     given and "done" [B, n] bool when eos is.  Places without a candidate
     hold -inf, -1, -1, length 0.  W <= 64, n <= 256.
     """
+    if eos is not None and eos < 0:  # -1 is how the library is told that there is none
+        raise ValueError("eos must be a token id, None without one")
     if n is None:
         n = scores.shape[-1] if keep_slots else 2 * scores.shape[-1]
     out = L.ext().beam_select(logits, scores, n, mask, done, -1 if eos is None else eos, lengths, length_penalty,
