@@ -310,7 +310,7 @@ typedef struct pm_top_rows {
     const uint32_t *mask;        /* [rows, mask_stride] allowed-token bits, or NULL */
     int64_t mask_stride;         /* words, >= ceil(vocab / 32); 0: one mask for every row */
     int32_t k;
-    double inv_temperature;      /* > 0 */
+    double inv_temperature;      /* > 0; log2(e) times it fits fp32 (4.3e-39 <= T <= 2e45) */
 } pm_top_rows;
 
 /* ids, logprobs: [rows, k]; lse: [rows] log-sum-exp of logits *
@@ -427,7 +427,7 @@ typedef struct pm_distill {
     const int32_t *ids;          /* [rows, k] */
     const float *logprobs;       /* [rows, k] */
     int32_t k;
-    double inv_temperature;
+    double inv_temperature;      /* as in pm_top_rows */
     int32_t tail;                /* PM_TAIL_* */
     int32_t reduction;           /* PM_REDUCE_* */
     const float *weights;        /* [rows], or NULL */

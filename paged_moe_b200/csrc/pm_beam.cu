@@ -1015,7 +1015,7 @@ size_t round16(size_t v) { return (v + 15) / 16 * 16; }
 }  // namespace
 
 extern "C" int pm_top_logprobs(const pm_top_rows* t, int32_t* ids, float* logprobs, float* lse, void* stream) {
-  if (!t || t->k < 1 || !(t->inv_temperature > 0.0) || std::isinf(t->inv_temperature)) return PM_ERR_ARG;
+  if (!t || t->k < 1 || !pm::scale_fits(t->inv_temperature)) return PM_ERR_ARG;
   const int rc = check_logits(t->logits, t->dtype, t->rows, t->vocab, t->row_stride, t->mask, t->mask_stride);
   if (rc) return rc;
   if (t->k > pm::kTopMax) return PM_ERR_UNSUPPORTED;

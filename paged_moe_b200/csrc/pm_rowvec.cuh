@@ -224,6 +224,13 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
+// Whether c is a number that exponents may be multiplied by: for T below
+// 4.3e-39 it is infinite (0 c is no number then), above 2e45 it is 0 (-inf c).
+inline bool scale_fits(double inv_t) {
+  const float c = (float)(kLog2e64 * inv_t);
+  return c > 0.0f && c <= 3.402823466e38f;
+}
+
 // The constant of a row's exponentials.
 struct ExpScale {
   float c;  // fl32(log2(e) / T)

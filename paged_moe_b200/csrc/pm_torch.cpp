@@ -267,6 +267,12 @@ bool has_tangent(const torch::Tensor& t) {
   return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
 }
 
+// A temperature whose inverse the kernels' fp32 exponents can hold.
+void check_temp(double temp) {
+  if (!(temp > 0.0) || std::isinf(temp)) bad_value("temp must be positive");
+  if (temp < 4.3e-39 || temp > 2e45) bad_value("temp must lie within [4.3e-39, 2e45]");
+}
+
 // The allowed-token words of `rows` rows: contiguous [rows, words], or [words]
 // for every row (stride 0).
 struct Mask {
@@ -306,7 +312,7 @@ std::vector<torch::Tensor> top_logprobs(torch::Tensor logits, int64_t k, double 
   t.dtype = logits_code(logits);
   if (logits.dim() != 2) bad_value("logits must be [rows, vocab]");
   if (k < 1) bad_value("k must be at least 1");
-  if (!(temp > 0.0) || std::isinf(temp)) bad_value("temp must be positive");
+  check_temp(temp);
   torch::Tensor x = as_rows(logits);
   const Mask m = check_mask(mask, x.size(0), x.size(1));
   need_cuda(x, "logits");
@@ -568,7 +574,7 @@ std::vector<torch::Tensor> distill(torch::Tensor logits, torch::Tensor ids, torc
   pm_distill d;
   std::memset(&d, 0, sizeof(d));
   d.dtype = logits_code(logits);
-  if (!(temp > 0.0) || std::isinf(temp)) bad_value("temp must be positive");
+  check_temp(temp);
   torch::Tensor x = as_rows(logits.detach());
   const int64_t N = x.size(0), V = x.size(1);
   if (ids.dim() < 1 || ids.size(-1) < 1 || ids.numel() != N * ids.size(-1))
