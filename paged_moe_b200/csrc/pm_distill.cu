@@ -322,7 +322,11 @@ __device__ __forceinline__ DistillPart dist_reduce(DistillPart p) {
 }
 
 // The row's part from its warps', through the cluster; every thread gets it.
-// Between one call and the next but one lies a barrier, so two places do.
+// Two places do for `warps`: the next call's barrier lies between this one's
+// reads and the next but one's writes.  `parts` is written once: a cluster of
+// several CTAs has one row (launch_distill).  With more, a row that is summed
+// once more on its own (split 1 here) would leave no cluster barrier between
+// the reads of its parts and the next row's writes.
 __device__ __forceinline__ DistillPart dist_join(DistillShared& sh, DistillPart part, int joins, uint32_t rank,
                                                  uint32_t split) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1125,7 +1129,9 @@ cudaError_t launch_distill(const pm::DistillArgs& a, cudaStream_t st) {
   pm::DistillArgs b = a;
   b.vectors = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
   b.mark_tiles = (int)mark_tiles;
-  const int64_t clusters = a.rows < slots / split ? a.rows : slots / split;
+  // where rows are split there are places for all: each cluster has one row, on
+  // which dist_join relies
+  const int64_t clusters = split > 1 || a.rows < slots ? a.rows : slots;
   return launch_after(kernel, clusters * split, pm::kDistThreads, bytes(BUCKET ? mark_tiles : 0), split,
                       st, b);
 }
