@@ -28,7 +28,7 @@
 // of the data read twice for its candidates; what is issued bounds it (four
 // instructions an element, 72 % of the issue slots) and the ends of rows, where
 // a CTA searches while its SM's other three stream.  512 rows of fp32 at
-// k = 16, 67 us, 5.2 TB/s.  Single rows cost the latency of their phases: 8 us
+// k = 16, 67 us, 5.2 TB/s (up to 86 where their allocation lies worse).  Single rows cost the latency of their phases: 8 us
 // for 4 rows of 32,768, of which a copy is 2, the bound 1, the candidates 1,
 // their ranks 1, the cluster's exchange 1, the ends 2.
 //

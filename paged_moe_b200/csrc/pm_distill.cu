@@ -27,10 +27,13 @@
 // logits that L2 has let go (1.4 reads of the logits for one), and 60 % of the
 // issue slots (ten instructions an element forward, eight backward); clusters
 // of two, whose rows all stay in L2, take as long.  257 rows of 151,937 fp32:
-// 72 us, 4.7 TB/s.  8,000 rows of 16,384 bf16 in k_distill_short: 150 us, 4.4
+// 72 us, 4.7 TB/s.  8,000 rows of 16,384 bf16 in k_distill_short: 143 us, 4.4
 // TB/s.  Twelve warps with three stages, twice an SM, were faster than eight
-// warps, two or three times an SM, and than fourteen.  A cluster a row where
-// there are few: 16 rows of 163,840 fp32 21 us, 43 with one CTA each.
+// warps, two or three times an SM, and than fourteen; their 80 registers spill
+// 88 to 136 bytes.  A cluster a row where there are few: 16 rows of 163,840 fp32
+// 20 us, 43 with one CTA each.  The bucket's marks of an unsplit row of more
+// than 159,740 fp32 tokens leave room for one CTA an SM, half of the grid at a
+// time: 480 rows of 163,840 take 166 us, of 159,740 160.
 //
 // Every wait on a copy is bounded; a row whose copy does not arrive gives NaN.
 #include <cuda_bf16.h>
@@ -48,7 +51,7 @@ namespace pm {
 
 constexpr int kDistThreads = 384;
 constexpr int kDistWarps = kDistThreads / 32;
-constexpr int kDistResident = 2;               // CTAs of an SM
+constexpr int kDistResident = 2;               // CTAs of an SM that the grid counts on
 constexpr int kShortThreads = 256, kShortWarps = kShortThreads / 32;
 constexpr int64_t kShortBytes = 64 << 10;      // of a row that a warp takes alone, half as many for its gradient
 constexpr int kDistMax = 256;                  // largest k

@@ -18,8 +18,10 @@
 //
 // Both are bound by memory.  Eight key-value states of 4 x 8 beams, 8 heads,
 // 2,048 positions of 128 bf16, in place with the beams that live on in their
-// slots: 95 us, 5.3 TB/s of what it reads and writes (k_reorder_bytes 150 us).  Six states of 16 x 6
-// beams, 1,001 x 3 x 65 bf16, into a double buffer: 46 us, 5.0 TB/s.  Three
+// slots: 94 us, 5.4 TB/s of what it reads and writes (k_reorder_bytes 150 us).  Six states of 16 x 6
+// beams, 1,001 x 3 x 65 bf16, up to their lengths into a double buffer: 45 us,
+// 4.4 TB/s (5.1 where whole rows move: a segment behind the lengths costs its
+// CTA two barriers).  Three
 // slots of 12 KB a warp keep 200 KB an SM in flight; two of 32 KB a CTA and
 // three CTAs an SM likewise.
 //
